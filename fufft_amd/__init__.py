@@ -113,6 +113,14 @@ def _load() -> C.CDLL:
         "fufft_plan_filter_device_f32": ([vp, vp, i64, i64, i32, i32, i32, i32, vp], i32),
         "fufft_plan_filter_large_device_f32": ([vp, vp, i64, i64, i32, i32, i32, vp], i32),
         "fufft_plan_filter2d_device_f32": ([vp, vp, i64, i64, i64, i32, i32, i32, vp], i32),
+        "fufft_mx4_padded": ([i64], i64),
+        "fufft_mx4_quantize": ([vp, i32, i64, i64, i64, i32, vp, vp, vp, vp, vp, vp], i32),
+        "fufft_mx4_dequantize": ([vp, vp, vp, i32, i64, i64, i64, vp], i32),
+        "fufft_mx4_matmul": ([vp, vp, vp, vp, vp, vp, i32, i64, i64, i64, i64, vp], i32),
+        "fufft_mx4_linear": ([vp, i32, i64, vp, vp, vp, vp, i32, i64, i64, i64, i64, vp], i32),
+        "fufft_mx4_cache_write": ([vp, i32, i64, vp, i64, i64, vp, vp, i64, vp], i32),
+        "fufft_mx4_cache_read": ([vp, vp, i64, i64, i64, vp, i64, vp, i64, i64, vp, i32, i32, vp], i32),
+        "fufft_mx4_cache_conv": ([vp, vp, i64, i64, i64, vp, i64, vp, i64, vp, i32, i64, vp, i32, vp, i64, vp], i32),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name, None)
@@ -145,7 +153,11 @@ if torch is not None:
         "exp": (torch.int8, torch.uint8),
         "scale": (torch.float32,),
         "words": (torch.int32,),
+        "bytes": (torch.uint8,),
+        "slots": (torch.int64,),
     }
+    # element types of the mx4 calls (FUFFT_F32, FUFFT_BF16, FUFFT_F16)
+    _ELEMENT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
     # the reads every launch makes, without torch.cuda's Python layer (which
     # initialises the GPU on first use: a tensor that is on one has done that)
     _TENSOR = torch.Tensor
@@ -694,3 +706,202 @@ def bfp_dequantize(q: np.ndarray, e: np.ndarray, block: int = BFP_BLOCK) -> np.n
     check(lib.fufft_bfp_dequantize(q.ctypes.data, ex.ctypes.data, npts, block, x.ctypes.data),
           "fufft_bfp_dequantize")
     return x
+
+
+# ---- microscaled 4-bit blocks (mx4) ------------------------------------------------------
+# Blocks of 32 values share a scale byte; a row's codes are uint8 (mx4_padded(k) // 2 of them),
+# its scales uint8 (mx4_padded(k) // 32).  Matrices of ordinary elements (fp32, bf16, fp16) are
+# 2D tensors whose rows may be apart (x.stride(0) >= columns) and whose elements are adjacent.
+
+MX4_BLOCK = 32
+MX4_RULE = {"fit": 0, "floor": 1}
+MX4_ORDER = {"tokens": 0, "channels": 1}
+
+
+def mx4_padded(k: int) -> int:
+    """Values of a row of k with its padding: the next multiple of 128."""
+    return (k + 127) // 128 * 128
+
+
+def mx4_empty(rows: int, k: int, device="cuda"):
+    """Uninitialised (codes, scales) for `rows` rows of k values."""
+    kp = mx4_padded(k)
+    return (torch.empty(rows, kp // 2, dtype=torch.uint8, device=device),
+            torch.empty(rows, kp // MX4_BLOCK, dtype=torch.uint8, device=device))
+
+
+def _name(table: dict, key, name: str) -> int:
+    if key not in table:
+        raise ValueError(f"{name} must be one of {sorted(table)}, not {key!r}")
+    return table[key]
+
+
+def _matrix(x, name: str):
+    """(type, leading dimension, rows, columns) of a 2D tensor of elements, checked but for
+    its device (the last check, _on_gpu)."""
+    if torch is None or not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch tensor in GPU memory, got {type(x).__name__}")
+    kind = _ELEMENT.get(x.dtype)
+    if kind is None:
+        allowed = ", ".join(str(d) for d in _ELEMENT)
+        raise ValueError(f"{name}: dtype {x.dtype} is not one of {allowed}")
+    if x.dim() != 2:
+        raise ValueError(f"{name}: expected a matrix, got {x.dim()} dimensions")
+    rows, k = x.shape
+    ld, step = x.stride()
+    if k > 1 and step != 1:
+        raise ValueError(f"{name}: the elements of a row are not contiguous")
+    if rows > 1 and ld < k:
+        raise ValueError(f"{name}: rows overlap (stride {ld}, {k} columns)")
+    return kind, max(ld, k) if rows > 1 else k, rows, k
+
+
+def _on_gpu(*pairs) -> None:
+    for x, name in pairs:
+        _check_device(x, name)
+
+
+def _blocks(codes, scales, name: str, rows: int, k: int):
+    kp = mx4_padded(k)
+    return (codes, name, rows * (kp // 2), "bytes"), (scales, name + "_scales", rows * (kp // MX4_BLOCK), "bytes")
+
+
+def _bias(bias, n: int):
+    return None if bias is None else (bias, "bias", 4 * n, "real")
+
+
+def mx4_quantize(x, codes=None, scales=None, codes_t=None, scales_t=None, *, rand=None, rule: str = "fit",
+                 stream=None) -> None:
+    """x (rows, k) as blocks along its rows (codes, scales: rows of k), along its columns
+    (codes_t, scales_t: k rows of `rows` values), or both from one reading; the pair that is
+    not wanted is None.  rand: a uint8 for each value of x, contiguous, for rounding up or
+    down at random; None rounds to the nearest.  rule: "fit" (nothing saturates) or "floor"."""
+    rule = _name(MX4_RULE, rule, "rule")
+    kind, ld, rows, k = _matrix(x, "x")
+    along, across = codes is not None or scales is not None, codes_t is not None or scales_t is not None
+    if not (along or across):
+        raise ValueError("mx4_quantize: neither blocks along rows nor along columns are asked for")
+    none = (None, None)
+    pc, ps, qc, qs, pr = _ptrs(*(_blocks(codes, scales, "codes", rows, k) if along else none),
+                               *(_blocks(codes_t, scales_t, "codes_t", k, rows) if across else none),
+                               None if rand is None else (rand, "rand", rows * k, "bytes"))
+    _on_gpu((x, "x"))
+    check(lib.fufft_mx4_quantize(x.data_ptr(), kind, ld, rows, k, rule, pr, pc, ps, qc, qs,
+                                 _stream(stream)), "fufft_mx4_quantize")
+
+
+def mx4_dequantize(codes, scales, out, stream=None) -> None:
+    """The values that blocks along rows stand for, into out (rows, k)."""
+    kind, ld, rows, k = _matrix(out, "out")
+    pc, ps = _ptrs(*_blocks(codes, scales, "codes", rows, k))
+    _on_gpu((out, "out"))
+    check(lib.fufft_mx4_dequantize(pc, ps, out.data_ptr(), kind, ld, rows, k, _stream(stream)),
+          "fufft_mx4_dequantize")
+
+
+def mx4_matmul(a, a_scales, b, b_scales, out, k: int, bias=None, stream=None) -> None:
+    """out (m, n) = a b^T + bias: a is m rows of k values in blocks, b n rows, bias fp32.
+    For y = x w^T the gradients are dx = mx4_matmul(dy, w's columns) and dw = mx4_matmul(dy's
+    columns, x's columns), all from mx4_quantize."""
+    kind, ld, m, n = _matrix(out, "out")
+    pa, pas, pb, pbs, pbias = _ptrs(*_blocks(a, a_scales, "a", m, k), *_blocks(b, b_scales, "b", n, k), _bias(bias, n))
+    _on_gpu((out, "out"))
+    check(lib.fufft_mx4_matmul(pa, pas, pb, pbs, pbias, out.data_ptr(), kind, ld, m, n, k, _stream(stream)),
+          "fufft_mx4_matmul")
+
+
+def mx4_linear(x, w, w_scales, out, bias=None, stream=None) -> None:
+    """out (m, n) = x w^T + bias with x (m, k) as it is and w n rows of k values in blocks:
+    the form for single tokens."""
+    x_kind, ldx, m, k = _matrix(x, "x")
+    kind, ld, rows, n = _matrix(out, "out")
+    if rows != m:
+        raise ValueError(f"out: {rows} rows, x has {m}")
+    pw, pws, pbias = _ptrs(*_blocks(w, w_scales, "w", n, k), _bias(bias, n))
+    _on_gpu((x, "x"), (out, "out"))
+    check(lib.fufft_mx4_linear(x.data_ptr(), x_kind, ldx, pw, pws, pbias, out.data_ptr(), kind, ld, m, n, k,
+                               _stream(stream)), "fufft_mx4_linear")
+
+
+def _cache(codes, scales, channels: int):
+    """(pages, page) of a cache's codes (pages, page, mx4_padded(channels) // 2) and scales."""
+    kp = mx4_padded(channels)
+    for x, name, last in ((codes, "codes", kp // 2), (scales, "scales", kp // MX4_BLOCK)):
+        if torch is None or not isinstance(x, torch.Tensor):
+            raise TypeError(f"{name}: expected a torch tensor in GPU memory, got {type(x).__name__}")
+        if x.dim() != 3 or x.shape[2] != last:
+            raise ValueError(f"{name}: expected (pages, page, {last}), got {tuple(x.shape)}")
+    if codes.shape[:2] != scales.shape[:2]:
+        raise ValueError(f"codes and scales: {tuple(codes.shape[:2])} and {tuple(scales.shape[:2])} pages and tokens")
+    pages, page = codes.shape[:2]
+    if page < 1 or page > 65536 or page & (page - 1):
+        raise ValueError(f"codes: {page} tokens a page, not a power of two up to 65536")
+    return pages, page
+
+
+def _table(table, lens):
+    if torch is None or not isinstance(table, torch.Tensor) or not isinstance(lens, torch.Tensor):
+        raise TypeError("pages and lens: expected torch tensors in GPU memory")
+    if table.dim() != 2 or lens.dim() != 1 or table.shape[0] != lens.shape[0]:
+        raise ValueError(f"pages and lens: expected (batch, width) and (batch), got {tuple(table.shape)} and "
+                         f"{tuple(lens.shape)}")
+    batch, width = table.shape
+    return batch, width, (table, "pages", 4 * batch * width, "words"), (lens, "lens", 4 * batch, "words")
+
+
+def mx4_cache_write(x, slots, codes, scales, stream=None) -> None:
+    """Rows of x (tokens, channels) into the slots (int64, page * page_size + offset, all
+    different) of a cache; a slot outside it, such as -1, is skipped."""
+    kind, ld, rows, channels = _matrix(x, "x")
+    pages, page = _cache(codes, scales, channels)
+    pl, pc, ps = _ptrs((slots, "slots", 8 * rows, "slots"), *_blocks(codes, scales, "codes", pages * page, channels))
+    _on_gpu((x, "x"))
+    check(lib.fufft_mx4_cache_write(x.data_ptr(), kind, ld, pl, rows, channels, pc, ps, pages * page,
+                                    _stream(stream)), "fufft_mx4_cache_write")
+
+
+def mx4_cache_read(codes, scales, pages, lens, out, order: str = "tokens", stream=None) -> None:
+    """The first tokens of every sequence (a row of pages, int32, and a length, int32), zeros
+    from its length on: out (batch, length, channels), or with order "channels" (batch,
+    channels, length), the signals that the convolutions take."""
+    turned = _name(MX4_ORDER, order, "order")
+    if torch is None or not isinstance(out, torch.Tensor):
+        raise TypeError(f"out: expected a torch tensor in GPU memory, got {type(out).__name__}")
+    if out.dtype not in _ELEMENT:
+        raise ValueError(f"out: dtype {out.dtype} is not one of {', '.join(str(d) for d in _ELEMENT)}")
+    batch, width, st, sl = _table(pages, lens)
+    if out.dim() != 3 or out.shape[0] != batch:
+        raise ValueError(f"out: expected three dimensions with {batch} sequences, got {tuple(out.shape)}")
+    if not out.is_contiguous():
+        raise ValueError("out: tensor is not contiguous")
+    channels, length = (out.shape[1], out.shape[2]) if turned else (out.shape[2], out.shape[1])
+    count, page = _cache(codes, scales, channels)
+    pc, ps, pt, pn = _ptrs(*_blocks(codes, scales, "codes", count * page, channels), st, sl)
+    _on_gpu((out, "out"))
+    check(lib.fufft_mx4_cache_read(pc, ps, count, page, channels, pt, width, pn, batch, length, out.data_ptr(),
+                                   _ELEMENT[out.dtype], turned, _stream(stream)), "fufft_mx4_cache_read")
+
+
+def mx4_cache_conv(codes, scales, pages, lens, taps, out, work=None, stream=None) -> None:
+    """out (batch, channels) = the causal convolution with taps (count, channels) at every
+    sequence's last token, read from the cache.  work: fp32 (splits, batch, channels); the
+    taps are split over at most that many workgroups.  None is allowed for fp32 results."""
+    t_kind, t_ld, tap_count, channels = _matrix(taps, "taps")
+    kind, ld, batch, out_channels = _matrix(out, "out")
+    if out_channels != channels:
+        raise ValueError(f"out: {out_channels} channels, taps have {channels}")
+    if (tap_count > 1 and t_ld != channels) or (batch > 1 and ld != channels):
+        raise ValueError("taps and out: tensor is not contiguous")
+    rows, width, st, sl = _table(pages, lens)
+    if rows != batch:
+        raise ValueError(f"out: {batch} sequences, pages have {rows}")
+    count, page = _cache(codes, scales, channels)
+    splits = 0 if work is None or batch * channels == 0 else work.numel() // (batch * channels)
+    if kind != 0 and splits == 0 and batch * channels > 0:
+        raise ValueError("work: results in 16 bits need a workspace of one split at least")
+    pc, ps, pt, pn, pw = _ptrs(*_blocks(codes, scales, "codes", count * page, channels), st, sl,
+                               None if splits == 0 else (work, "work", 4 * splits * batch * channels, "real"))
+    _on_gpu((taps, "taps"), (out, "out"))
+    check(lib.fufft_mx4_cache_conv(pc, ps, count, page, channels, pt, width, pn, batch, taps.data_ptr(), t_kind,
+                                   tap_count, out.data_ptr(), kind, pw, splits, _stream(stream)),
+          "fufft_mx4_cache_conv")

@@ -161,8 +161,9 @@ def decode_name(name: str) -> dict | None:
 
 
 def load(objs=None) -> list:
-    """Every kernel of the given objects (default: all of fufft_amd/_build)."""
+    """Every kernel of the given objects (default: all of fufft_amd/_build; those of host code alone hold none)."""
     objs = sorted(OBJ.glob("*.o")) if objs is None else objs
+    objs = [obj for obj in objs if b".hip_fatbin" in obj.read_bytes()]
     rows = []
     with tempfile.TemporaryDirectory() as d:
         for obj in objs:

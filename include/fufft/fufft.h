@@ -479,6 +479,105 @@ int fufft_apply2d_f32(const void* spec, int64_t spec_stride, const void* filt,
                       int64_t filt_stride, void* out, int64_t h, int64_t w,
                       int64_t batch, int mid, int layout, void* stream);
 
+/* ---- microscaled 4-bit blocks (mx4) ---------------------------------------------------
+ * Block floating point in 4 bits, for what stands around the convolutions of a
+ * long-convolution model: its matrix products, and the history of the signals
+ * that generation convolves token by token.  No reference counterpart.
+ *
+ * Every FUFFT_MX4_BLOCK consecutive values of a row share a scale byte s that
+ * stands for 2^(s - 127) (255: NaN); a value is that times the 4-bit number
+ * (-1)^sign {0, .5, 1, 1.5, 2, 3, 4, 6}[code & 7], sign = code >> 3.  A row of k
+ * values is padded to fufft_mx4_padded(k), whole groups of 128, and takes that
+ * / 2 bytes of codes (two a byte, the earlier one in the low half) and that / 32
+ * scale bytes; rows follow each other without gaps.  The padding holds zero
+ * codes under any scale but 255; the quantizing calls write it so.  For k a
+ * multiple of 128 this is the layout microscaled 4-bit tensors have elsewhere.
+ *
+ * Codes are 16-byte and scales 4-byte aligned; the other arrays, rows x k with a
+ * leading dimension ld (elements, >= k), only need their element's alignment.
+ * Element types: FUFFT_F32, FUFFT_BF16, FUFFT_F16.  Sums are fp32, rounded once
+ * to the output's type.  Sizes of zero are allowed and pointers to nothing may
+ * then be NULL.  Inputs and outputs of a call share no byte. */
+#define FUFFT_F32   0
+#define FUFFT_BF16  1
+#define FUFFT_F16   2
+#define FUFFT_MX4_BLOCK 32
+/* the padded length of a row of k values, or FUFFT_ERR_INVALID */
+int64_t fufft_mx4_padded(int64_t k);
+
+/* Scale of a block with largest magnitude t:
+ *   FUFFT_MX4_FIT    the smallest power of two p with t <= 6 p, the rule of this
+ *                    library's block floating point: nothing saturates;
+ *   FUFFT_MX4_FLOOR  2^(floor(log2 t) - 2): magnitudes above 6 p become 6 p;
+ * 2^-127 where that is smaller (and for a block of zeros), 255 for a block with
+ * a NaN or an infinity. */
+#define FUFFT_MX4_FIT    0
+#define FUFFT_MX4_FLOOR  1
+/* x in blocks along its rows (codes, scales: rows of k), along its columns
+ * (codes_t, scales_t: k rows of `rows` values, the operand of a product that
+ * contracts over x's rows), or both from one reading of x; the pair that is not
+ * wanted is NULL.  rand NULL: to the nearest, ties to the even code.  rand, a byte
+ * r for each value (rows x k, contiguous): to the neighbour above in magnitude if
+ * the share of the step that lies below the value, plus (r + 1/2) / 256, reaches
+ * 1, else to the one below; uniform bytes make the rounding's mean the value to
+ * within 2^-9 of a step, as a gradient wants. */
+int fufft_mx4_quantize(const void* x, int type, int64_t ld, int64_t rows, int64_t k, int rule,
+                       const uint8_t* rand, void* codes, uint8_t* scales, void* codes_t,
+                       uint8_t* scales_t, void* stream);
+/* the values that blocks stand for; exact in fp32 and bf16 (but for 1.5, 3 and 6
+ * times powers that leave the range), rounded in fp16 */
+int fufft_mx4_dequantize(const void* codes, const uint8_t* scales, void* out, int type,
+                         int64_t ld, int64_t rows, int64_t k, void* stream);
+
+/* out[i][j] = bias[j] + sum over k of a[i][k] b[j][k]: a is m rows, b n rows, out
+ * m x n; bias fp32 or NULL.  A layer y = x w^T has the gradients dx = dy (w^T)^T
+ * and dw = dy^T (x^T)^T: the same product on the blocks along columns that
+ * fufft_mx4_quantize makes of w, dy and x. */
+int fufft_mx4_matmul(const void* a, const uint8_t* a_scales, const void* b,
+                     const uint8_t* b_scales, const float* bias, void* out, int type, int64_t ld,
+                     int64_t m, int64_t n, int64_t k, void* stream);
+/* out[i][j] = bias[j] + sum over k of x[i][k] w[j][k] with x (x_type, leading
+ * dimension ldx) as it is: the form for single tokens, which reads w once for up
+ * to 64 rows.  (Many rows run faster quantized, through fufft_mx4_matmul.) */
+int fufft_mx4_linear(const void* x, int x_type, int64_t ldx, const void* w,
+                     const uint8_t* w_scales, const float* bias, void* out, int type, int64_t ld,
+                     int64_t m, int64_t n, int64_t k, void* stream);
+
+/* A paged cache of signals: `pages` pages of `page` tokens (a power of two up to
+ * 65536) of `channels` values in blocks along channels.  Slot s is token
+ * s % page of page s / page.  A sequence is a row of the page table (`width`
+ * pages, int32) and a length (int32): its token t is token t % page of page
+ * table[t / page].  A page outside [0, pages) reads as zeros, a length is taken
+ * as at most width * page and at least 0.
+ * write: row r of x goes to slot slots[r] with FUFFT_MX4_FIT, to the nearest; a
+ * slot outside [0, slot_count) is skipped (-1: a token that is not kept).  The
+ * slots of one call differ.
+ * read: tokens [0, length) of every sequence, zeros from its own length on, as
+ * out[b][t][channel] (FUFFT_MX4_TOKENS) or as out[b][channel][t]
+ * (FUFFT_MX4_CHANNELS): in fp32, and with length a supported n, the zero-padded
+ * signals that fufft_conv_r2_f32 takes. */
+#define FUFFT_MX4_TOKENS    0
+#define FUFFT_MX4_CHANNELS  1
+int fufft_mx4_cache_write(const void* x, int type, int64_t ld, const int64_t* slots,
+                          int64_t rows, int64_t channels, void* codes, uint8_t* scales,
+                          int64_t slot_count, void* stream);
+int fufft_mx4_cache_read(const void* codes, const uint8_t* scales, int64_t pages, int64_t page,
+                         int64_t channels, const int32_t* table, int64_t width,
+                         const int32_t* lens, int64_t batch, int64_t length, void* out, int type,
+                         int order, void* stream);
+/* The causal convolution's value at each sequence's last token, from the cache:
+ * out[b][c] = sum over j < min(lens[b], tap_count) of taps[j][c] x[b][lens[b]-1-j][c];
+ * taps tap_count x channels, contiguous; out batch x channels.  0 for an empty
+ * sequence; taps beyond a length are not looked at.  work: fp32 space for
+ * `splits` x batch x channels sums; the taps are split over at most that many
+ * workgroups, whose sums a second launch joins in a fixed order.  0 splits (work
+ * NULL) is allowed for fp32 results; 64 are as many as help. */
+int fufft_mx4_cache_conv(const void* codes, const uint8_t* scales, int64_t pages, int64_t page,
+                         int64_t channels, const int32_t* table, int64_t width,
+                         const int32_t* lens, int64_t batch, const void* taps, int tap_type,
+                         int64_t tap_count, void* out, int type, float* work, int64_t splits,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif
