@@ -29,44 +29,42 @@ __device__ inline i32x8 operand4(u32x4 c)
 // ---- few rows: operands straight from memory, K split over the wavefronts ----------
 //
 // A workgroup computes 16 MT rows of x times 16 NT rows of w.  Its wavefronts take
-// the groups of 128 values in turn, and their sums are joined in LDS in the order
-// of the wavefronts.
+// runs of four groups of 128 values in turn, and their sums are joined in LDS in the
+// order of the wavefronts.  What bounds these kernels is w's bytes where N is large
+// and else the wait for memory, so each wavefront has DEPTH runs on their way.
+//
+// A load of 16 scale bytes or words of 16 rows takes as long as one of 16 bytes of
+// codes a lane.  So the 16 bytes of a row and run come in one load, a word for each of
+// the four lanes of a row, and the words go round between those lanes: at 16384 x 16384
+// the load of a byte for each block took 57 us where scales left out took 39.
 
-// The rows of x as the w operand meets them: a value in bf16 is one, in fp16 two, in
-// fp32 three bf16 parts (8, 11 and 24 significant bits at 8 a part, cut off rather than
-// rounded, so that no part overflows).  The parts add up to the value exactly but for
-// bits below 2^-133, so the product is that of the values themselves.
-template<class T> struct PartsOf;
-template<> struct PartsOf<bf16>  { static constexpr int value = 1; };
-template<> struct PartsOf<f16>   { static constexpr int value = 2; };
-template<> struct PartsOf<float> { static constexpr int value = 3; };
+constexpr int kRun = 4;                // groups of 128 values
 
-template<class T, int PARTS = PartsOf<T>::value>
-__device__ inline void split8(const float (&v)[8], bf16x8 (&part)[PARTS])
+// A lane's part of a run of 16 rows: its block of every group, and the word that
+// holds the four scales of group lane / 16.
+struct Run {
+   u32x4    c[kRun];
+   uint32_t s;
+};
+
+__device__ inline void fetch_run(Run& r, const uint8_t* codes, const uint8_t* scales, int64_t first, int groups)
 {
+   // first: the run's first group; the last group's scales again beyond the last
+   const int lane = threadIdx.x & 63, mine = (int)first + (lane >> 4);
 #pragma unroll
-   for(int i = 0; i < 8; i++) {
-      float left = v[i];
-#pragma unroll
-      for(int q = 0; q < PARTS; q++) {
-         const float b = __uint_as_float(__float_as_uint(left) & 0xffff0000u);
-         part[q][i] = __builtin_bit_cast(bf16, (uint16_t)(__float_as_uint(left) >> 16));
-         if(q + 1 < PARTS) left = magnitude(left) == 0x7f800000u ? 0.0f : left - b;   // all of an infinity is in one part
-      }
-   }
+   for(int g = 0; g < kRun; g++)
+      if(g == 0 || first + g < groups) r.c[g] = *reinterpret_cast<const u32x4*>(codes + (first + g) * 64);
+   r.s = *reinterpret_cast<const uint32_t*>(scales + (int64_t)(mine < groups ? mine : groups - 1) * 4);
 }
-
-__device__ inline bf16x8 decode8_bf16(uint32_t c, float p)
+// the lane's scale byte of group g of the run, in the low byte
+__device__ inline uint32_t run_scale(const Run& r, int g)
 {
-   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, p, 0);
-   const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, p, 1);
-   const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, p, 2);
-   const bf16x2 e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, p, 3);
-   return bf16x8{a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
+   const int lane = threadIdx.x & 63;
+   return (uint32_t)__builtin_amdgcn_ds_bpermute((g * 16 + (lane & 15)) * 4, (int)r.s) >> ((lane >> 4) * 8);
 }
 
 // wavefronts of a workgroup with so many 16 x 16 tiles: their sums fill at most 64 KiB of LDS
-constexpr int most_waves(int tiles) { return tiles >= 16 ? 4 : tiles >= 4 ? 8 : 16; }
+constexpr int most_waves(int tiles) { return tiles >= 8 ? 4 : 8; }
 
 // the sums of all wavefronts, joined, and stored: acc[mt][nt] holds rows
 // 4 (lane / 16) + r of w and row lane % 16 of x
@@ -86,7 +84,8 @@ __device__ inline void join_and_store(const MatmulParams& p, f32x4 (&acc)[MT][NT
    O* out = static_cast<O*>(p.out);
    for(int i = threadIdx.x; i < ROWS * COLS; i += waves * 64) {
       const int64_t m = m0 + i / COLS, n = n0 + i % COLS;
-      if(m >= p.m || n >= p.n) continue;
+      if(m >= p.m) break;
+      if(n >= p.n) continue;
       float v = 0.0f;
       for(int w = 0; w < waves; w++) v += join[w * ROWS * COLS + i];
       if(p.bias) v += p.bias[n];
@@ -94,117 +93,192 @@ __device__ inline void join_and_store(const MatmulParams& p, f32x4 (&acc)[MT][NT
    }
 }
 
-template<class O, int MT, int NT>
+// the row that a lane reads for a tile of 16: rows beyond the last read the last one
+__device__ inline int64_t row_of(int64_t first, int64_t rows)
+{
+   const int64_t r = first + (threadIdx.x & 15);
+   return r < rows ? r : rows - 1;
+}
+
+template<class O, int MT, int NT, int DEPTH>
 __global__ void __launch_bounds__(64 * most_waves(MT * NT))
-matmul_rows(MatmulParams p, int64_t groups, int waves)
+matmul_rows(MatmulParams p, int groups, int waves)
 {
    extern __shared__ float join[];
-   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
    const int64_t n0 = (int64_t)blockIdx.x * (16 * NT), m0 = (int64_t)blockIdx.y * (16 * MT);
    const uint8_t* xc[MT];
    const uint8_t* xs[MT];
    const uint8_t* wc[NT];
    const uint8_t* ws[NT];
 #pragma unroll
-   for(int a = 0; a < MT; a++) {         // rows beyond the last read the last one
-      int64_t r = m0 + a * 16 + (lane & 15);
-      r = r < p.m ? r : p.m - 1;
+   for(int a = 0; a < MT; a++) {
+      const int64_t r = row_of(m0 + a * 16, p.m);
       xc[a] = static_cast<const uint8_t*>(p.x) + r * groups * 64 + (lane >> 4) * 16;
-      xs[a] = p.x_scales + r * groups * 4 + (lane >> 4);
+      xs[a] = p.x_scales + r * groups * 4;
    }
 #pragma unroll
    for(int b = 0; b < NT; b++) {
-      int64_t r = n0 + b * 16 + (lane & 15);
-      r = r < p.n ? r : p.n - 1;
+      const int64_t r = row_of(n0 + b * 16, p.n);
       wc[b] = p.w + r * groups * 64 + (lane >> 4) * 16;
-      ws[b] = p.w_scales + r * groups * 4 + (lane >> 4);
+      ws[b] = p.w_scales + r * groups * 4;
    }
+   Run x[DEPTH][MT], w[DEPTH][NT];
+   auto fetch = [&](int d, int64_t g) {
+#pragma unroll
+      for(int b = 0; b < NT; b++) fetch_run(w[d][b], wc[b], ws[b], g, groups);
+#pragma unroll
+      for(int a = 0; a < MT; a++) fetch_run(x[d][a], xc[a], xs[a], g, groups);
+   };
    f32x4 acc[MT][NT] = {};
+   const int step = waves * kRun;
+#pragma unroll
+   for(int d = 0; d < DEPTH; d++)
+      if(wave * kRun + d * step < groups) fetch(d, wave * kRun + d * step);
 #pragma unroll 1
-   for(int64_t g = wave; g < groups; g += waves) {
-      u32x4 x[MT], w[NT];
-      int sx[MT], sw[NT];
+   for(int g0 = wave * kRun; g0 < groups; g0 += step * DEPTH) {
 #pragma unroll
-      for(int b = 0; b < NT; b++) {
-         w[b] = *reinterpret_cast<const u32x4*>(wc[b] + g * 64);
-         sw[b] = ws[b][g * 4];
+      for(int d = 0; d < DEPTH; d++) {
+         const int g = g0 + d * step;
+#pragma unroll
+         for(int i = 0; i < kRun; i++) {
+            if(g + i >= groups) break;
+            uint32_t sw[NT];
+#pragma unroll
+            for(int b = 0; b < NT; b++) sw[b] = run_scale(w[d][b], i);
+#pragma unroll
+            for(int a = 0; a < MT; a++) {
+               const uint32_t sx = run_scale(x[d][a], i);
+#pragma unroll
+               for(int b = 0; b < NT; b++)
+                  acc[a][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand4(w[d][b].c[i]), operand4(x[d][a].c[i]),
+                                                                               acc[a][b], 4, 4, 0, (int)sw[b], 0, (int)sx);
+            }
+         }
+         if(g + step * DEPTH < groups) fetch(d, g + step * DEPTH);
       }
-#pragma unroll
-      for(int a = 0; a < MT; a++) {
-         x[a] = *reinterpret_cast<const u32x4*>(xc[a] + g * 64);
-         sx[a] = xs[a][g * 4];
-      }
-#pragma unroll
-      for(int a = 0; a < MT; a++)
-#pragma unroll
-         for(int b = 0; b < NT; b++)
-            acc[a][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand4(w[b]), operand4(x[a]), acc[a][b], 4, 4,
-                                                                         0, sw[b], 0, sx[a]);
    }
    join_and_store<O, MT, NT>(p, acc, join, waves, m0, n0);
 }
 
+// The rows of x as the w operand meets them: a value in bf16 is one, in fp16 two, in
+// fp32 three bf16 parts (8, 11 and 24 significant bits at 8 a part, cut off rather than
+// rounded, so that no part overflows).  The parts add up to the value exactly but for
+// bits below 2^-133, so the product is that of the values themselves.
+template<class T> struct PartsOf;
+template<> struct PartsOf<bf16>  { static constexpr int value = 1; };
+template<> struct PartsOf<f16>   { static constexpr int value = 2; };
+template<> struct PartsOf<float> { static constexpr int value = 3; };
+
+template<class T, int PARTS = PartsOf<T>::value>
+__device__ inline void split8(const T (&v)[8], bf16x8 (&part)[PARTS])
+{
+#pragma unroll
+   for(int i = 0; i < 8; i++) {
+      if constexpr(PARTS == 1) {
+         part[0][i] = v[i];
+      } else {
+         float left = to_float(v[i]);
+#pragma unroll
+         for(int q = 0; q < PARTS; q++) {
+            const float b = __uint_as_float(__float_as_uint(left) & 0xffff0000u);
+            part[q][i] = __builtin_bit_cast(bf16, (uint16_t)(__float_as_uint(left) >> 16));
+            if(q + 1 < PARTS) left = magnitude(left) == 0x7f800000u ? 0.0f : left - b;   // all of an infinity is in one part
+         }
+      }
+   }
+}
+
+__device__ inline bf16x8 decode8_bf16(uint32_t c, float p)
+{
+   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, p, 0);
+   const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, p, 1);
+   const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, p, 2);
+   const bf16x2 e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, p, 3);
+   return bf16x8{a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
+}
+
 // The block that a lane reads holds its 8 values of each of four products, so
 // product t takes values 8 t .. 8 t + 7 of the four blocks of a group.
-template<class T, class O, int MT, int NT>
+template<class T, class O, int MT, int NT, int DEPTH>
 __global__ void __launch_bounds__(64 * most_waves(MT * NT))
-linear_rows(MatmulParams p, int64_t groups, int waves)
+linear_rows(MatmulParams p, int groups, int waves)
 {
    constexpr int PARTS = PartsOf<T>::value;
    extern __shared__ float join[];
-   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
    const int64_t n0 = (int64_t)blockIdx.x * (16 * NT), m0 = (int64_t)blockIdx.y * (16 * MT);
    const int64_t k0 = (lane >> 4) * 32;
    const T* x[MT];
    const uint8_t* wc[NT];
    const uint8_t* ws[NT];
 #pragma unroll
-   for(int a = 0; a < MT; a++) {
-      int64_t r = m0 + a * 16 + (lane & 15);
-      r = r < p.m ? r : p.m - 1;
-      x[a] = static_cast<const T*>(p.x) + r * p.ldx;
-   }
+   for(int a = 0; a < MT; a++) x[a] = static_cast<const T*>(p.x) + row_of(m0 + a * 16, p.m) * p.ldx + k0;
 #pragma unroll
    for(int b = 0; b < NT; b++) {
-      int64_t r = n0 + b * 16 + (lane & 15);
-      r = r < p.n ? r : p.n - 1;
+      const int64_t r = row_of(n0 + b * 16, p.n);
       wc[b] = p.w + r * groups * 64 + (lane >> 4) * 16;
-      ws[b] = p.w_scales + r * groups * 4 + (lane >> 4);
+      ws[b] = p.w_scales + r * groups * 4;
    }
+   Run w[DEPTH][NT];
+   auto fetch = [&](int d, int64_t g) {
+#pragma unroll
+      for(int b = 0; b < NT; b++) fetch_run(w[d][b], wc[b], ws[b], g, groups);
+   };
    f32x4 acc[MT][NT] = {};
+   const int step = waves * kRun;
+#pragma unroll
+   for(int d = 0; d < DEPTH; d++)
+      if(wave * kRun + d * step < groups) fetch(d, wave * kRun + d * step);
 #pragma unroll 1
-   for(int64_t g = wave; g < groups; g += waves) {
-      u32x4 w[NT];
-      float sw[NT];
+   for(int g0 = wave * kRun; g0 < groups; g0 += step * DEPTH) {
 #pragma unroll
-      for(int b = 0; b < NT; b++) {
-         w[b] = *reinterpret_cast<const u32x4*>(wc[b] + g * 64);
-         sw[b] = scale_operand(ws[b][g * 4]);
-      }
+      for(int d = 0; d < DEPTH; d++) {
+         const int64_t first = g0 + d * step;
+         struct __attribute__((packed, aligned(sizeof(T)))) Block { T e[4][8]; };
+         auto group = [&](int i, const Block (&v)[MT]) {
+            float sw[NT];
 #pragma unroll
-      for(int t = 0; t < 4; t++) {
-         bf16x8 part[MT][PARTS];
-         const int64_t k = g * 128 + k0 + t * 8;
+            for(int b = 0; b < NT; b++) sw[b] = scale_operand(run_scale(w[d][b], i) & 255u);
 #pragma unroll
-         for(int a = 0; a < MT; a++) {
-            float v[8];
-            if(k + 8 <= p.k) {
-               load8(x[a] + k, v);
-            } else {
+            for(int t = 0; t < 4; t++) {
+               bf16x8 part[MT][PARTS];
 #pragma unroll
-               for(int i = 0; i < 8; i++) v[i] = k + i < p.k ? to_float(x[a][k + i]) : 0.0f;
+               for(int a = 0; a < MT; a++) split8<T>(v[a].e[t], part[a]);
+#pragma unroll
+               for(int b = 0; b < NT; b++) {
+                  const bf16x8 c = decode8_bf16(w[d][b].c[i][t], sw[b]);
+#pragma unroll
+                  for(int a = 0; a < MT; a++)
+#pragma unroll
+                     for(int q = 0; q < PARTS; q++)
+                        acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(c, part[a][q], acc[a][b], 0, 0, 0);
+               }
             }
-            split8<T>(v, part[a]);
+         };
+         if((first + kRun) * 128 <= p.k) {
+            // whole runs in straight code: x's loads go ahead of the products
+#pragma unroll
+            for(int i = 0; i < kRun; i++) {
+               Block v[MT];
+#pragma unroll
+               for(int a = 0; a < MT; a++) v[a] = *reinterpret_cast<const Block*>(x[a] + (first + i) * 128);
+               group(i, v);
+            }
+         } else {
+#pragma unroll
+            for(int i = 0; i < kRun; i++) {
+               const int64_t k = (first + i) * 128;
+               if(k >= p.k) break;
+               Block v[MT];
+#pragma unroll
+               for(int a = 0; a < MT; a++)
+#pragma unroll
+                  for(int e = 0; e < 32; e++) v[a].e[e / 8][e % 8] = k + k0 + e < p.k ? x[a][k + e] : (T)0.0f;
+               group(i, v);
+            }
          }
-#pragma unroll
-         for(int b = 0; b < NT; b++) {
-            const bf16x8 v = decode8_bf16(w[b][t], sw[b]);
-#pragma unroll
-            for(int a = 0; a < MT; a++)
-#pragma unroll
-               for(int q = 0; q < PARTS; q++)
-                  acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, part[a][q], acc[a][b], 0, 0, 0);
-         }
+         if(first + step * DEPTH < groups) fetch(d, first + step * DEPTH);
       }
    }
    join_and_store<O, MT, NT>(p, acc, join, waves, m0, n0);
@@ -213,12 +287,17 @@ linear_rows(MatmulParams p, int64_t groups, int waves)
 // ---- many rows: tiles staged in LDS ---------------------------------------------------
 //
 // A workgroup of WM x WN wavefronts computes BM x BN results, a wavefront FM x FN
-// products of 32 x 32 x 64.  K goes by slabs of 256 values: BM + BN rows of 128 bytes
-// and, for two slabs at a time, of 16 scale bytes.  Two slabs are in LDS, one read, one
-// on its way there: straight from memory, so that no register waits for it.  The
-// loads write lane after lane, 8 rows of 8 chunks of 16 bytes; which chunk a lane
-// fetches is free, and slot c of row r gets chunk c ^ (r % 8) ^ (r / 8 % 2), so that
-// the lanes of a product, which read one chunk of 32 rows, meet all banks.
+// products of 32 x 32 x 64.  K goes by slabs of 256 values: BM + BN rows of 128 bytes.
+// Two slabs are in LDS, one read, one on its way there: straight from memory, so
+// that no register waits for it.  The loads write lane after lane, 8 rows of 8 chunks
+// of 16 bytes; which chunk a lane fetches is free, and slot c of row r gets chunk
+// c ^ (r % 8) ^ (r / 8 % 2), so that the lanes of a product, which read one chunk of 32
+// rows, meet all banks.
+//
+// A row's scales lie in one place for all of K, so a slab's are 8 bytes from each of BM +
+// BN places.  They come 64 bytes a row at a time, for 8 slabs, through registers (LDS has
+// no room for a second set); fetched 16 bytes a row for every two slabs, they were a
+// third of all requests to the L2 (8192 x 8192 x 8192: 286 -> 282 us).
 //
 // Block 2 t + lane / 32 of a slab takes part in product t: both its halves' scales are
 // bytes 0 and 2 (t = 0, 1) of a word shifted by 8 (lane / 32), and where K ends with
@@ -242,15 +321,16 @@ __device__ inline void fetch16(__amdgpu_buffer_rsrc_t r, uint8_t* to, uint32_t v
 }
 
 // Tile of workgroup `id` of tm x tn.  Workgroups go to the 8 XCDs in turn; each XCD,
-// with an L2 of its own, gets a run of tiles, and a run goes through strips of 8
-// tiles along m, so that the tiles that an XCD works on share rows.
+// with an L2 of its own, gets a run of tiles, and a run goes through strips of 4
+// tiles along m, so that the tiles that an XCD works on share rows (8192 x 8192 x 4096:
+// tiles in plain order 157 us, strips of 8 147, of 4 145.5).
 __device__ inline void tile_of(uint32_t id, uint32_t tm, uint32_t tn, uint32_t* m, uint32_t* n)
 {
    const uint32_t total = tm * tn, each = total / 8, more = total % 8, xcd = id % 8;
    const uint32_t i = xcd * each + (xcd < more ? xcd : more) + id / 8;
-   const uint32_t strip = i / (8 * tn), in = i - strip * 8 * tn;
-   const uint32_t high = tm - strip * 8 < 8 ? tm - strip * 8 : 8;
-   *m = strip * 8 + in % high;
+   const uint32_t strip = i / (4 * tn), in = i - strip * 4 * tn;
+   const uint32_t high = tm - strip * 4 < 4 ? tm - strip * 4 : 4;
+   *m = strip * 4 + in % high;
    *n = in / high;
 }
 
@@ -259,7 +339,7 @@ __global__ void __launch_bounds__(64 * WM * WN)
 matmul_tiles(MatmulParams p, uint32_t groups, uint32_t tm, uint32_t tn)
 {
    constexpr int WAVES = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
-   constexpr int ROWS = BM + BN, SLAB = ROWS * 128, SCALES = ROWS * 16;
+   constexpr int ROWS = BM + BN, SLAB = ROWS * 128, SCALES = ROWS * 64;
    constexpr int JOBS = ROWS / 8 / WAVES;                     // fetches of 8 rows a wavefront and slab
    extern __shared__ uint8_t lds[];
    uint8_t* const scale_lds = lds + 2 * SLAB;
@@ -297,16 +377,24 @@ matmul_tiles(MatmulParams p, uint32_t groups, uint32_t tm, uint32_t tn)
          fetch16(row < BM ? rx : rw, to + j * 1024, v, s * 128);
       }
    };
-   // the scales of slabs 2 q and 2 q + 1: 64 rows a fetch; beyond the matrix the buffer's end gives zeros
-   auto fetch_scales = [&](uint32_t q) {
+   // the scales of slabs 8 q .. 8 q + 7: 4 lanes a row, ROWS / 4 / WAVES fetches of 16 rows a wavefront; 16-byte
+   // part c of row r at slot c ^ (r / 4 % 4).  Beyond the matrix the buffer's end gives zeros.
+   constexpr int PARTS = ROWS / 16 / WAVES;
+   u32x4 next[PARTS];
+   auto load_scales = [&](uint32_t q) {
 #pragma unroll
-      for(int j = 0; j < (ROWS / 64 + WAVES - 1) / WAVES; j++) {
-         const int r = (wave + j * WAVES) * 64;
-         if(r >= ROWS) break;
-         uint8_t* const to = scale_lds + (q & 1) * SCALES + r * 16;
-         const uint32_t row = r + lane;
-         if(r < BM) fetch16(rsx, to, row * srow_bytes, q * 16);
-         else       fetch16(rsw, to, (row - BM) * srow_bytes, q * 16);
+      for(int j = 0; j < PARTS; j++) {
+         const int r = (j * WAVES + wave) * 16;
+         const uint32_t at = q * 64 + (lane & 3) * 16, row = r + (lane >> 2);
+         next[j] = __builtin_bit_cast(u32x4, r < BM ? __builtin_amdgcn_raw_buffer_load_b128(rsx, row * srow_bytes + at, 0, 0)
+                                                    : __builtin_amdgcn_raw_buffer_load_b128(rsw, (row - BM) * srow_bytes + at, 0, 0));
+      }
+   };
+   auto keep_scales = [&]() {
+#pragma unroll
+      for(int j = 0; j < PARTS; j++) {
+         const uint32_t row = (j * WAVES + wave) * 16 + (lane >> 2);
+         *reinterpret_cast<u32x4*>(scale_lds + row * 64 + ((lane & 3) ^ (row >> 2 & 3)) * 16) = next[j];
       }
    };
 
@@ -320,23 +408,28 @@ matmul_tiles(MatmulParams p, uint32_t groups, uint32_t tm, uint32_t tn)
 
    f32x16 acc[FM][FN] = {};
    if(slabs) {
-      fetch_scales(0);
+      load_scales(0);
       fetch_slab(0);
+      keep_scales();
    }
    for(uint32_t s = 0; s < slabs; s++) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      if(s + 1 < slabs) {
-         if((s & 1) == 0 && s + 2 < slabs) fetch_scales(s / 2 + 1);
-         fetch_slab(s + 1);
+      if((s & 7) == 0 && s) {
+         keep_scales();
+         __syncthreads();
       }
+      if(s + 1 < slabs) fetch_slab(s + 1);
+      if((s & 7) == 4 && s + 4 < slabs) load_scales(s / 8 + 1);
       const uint8_t* const data = lds + (s & 1) * SLAB;
-      const uint8_t* const sc = scale_lds + ((s >> 1) & 1) * SCALES + (s & 1) * 8;
+      const uint32_t sc = ((s >> 1 & 3) ^ (lane >> 2 & 3)) * 16 + (s & 1) * 8;
       u32x2 sx[FM], sw[FN];
 #pragma unroll
-      for(int a = 0; a < FM; a++) sx[a] = *reinterpret_cast<const u32x2*>(sc + xat[a] * 16) >> (uint32_t)(half * 8);
+      for(int a = 0; a < FM; a++)
+         sx[a] = *reinterpret_cast<const u32x2*>(scale_lds + xat[a] * 64 + sc) >> (uint32_t)(half * 8);
 #pragma unroll
-      for(int b = 0; b < FN; b++) sw[b] = *reinterpret_cast<const u32x2*>(sc + wat[b] * 16) >> (uint32_t)(half * 8);
+      for(int b = 0; b < FN; b++)
+         sw[b] = *reinterpret_cast<const u32x2*>(scale_lds + wat[b] * 64 + sc) >> (uint32_t)(half * 8);
       auto step = [&](auto tc) {
          constexpr int t = decltype(tc)::value;
          const uint32_t slot = ((2 * t + half) ^ turn) * 16;
@@ -349,9 +442,9 @@ matmul_tiles(MatmulParams p, uint32_t groups, uint32_t tm, uint32_t tn)
          for(int a = 0; a < FM; a++)
 #pragma unroll
             for(int b = 0; b < FN; b++)
-               acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand4(x[a]), operand4(w[b]), acc[a][b], 4, 4,
-                                                                           (t & 1) * 2, (int)sx[a][t >> 1], (t & 1) * 2,
-                                                                           (int)sw[b][t >> 1]);
+               acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand4(w[b]), operand4(x[a]), acc[a][b], 4, 4,
+                                                                           (t & 1) * 2, (int)sw[b][t >> 1], (t & 1) * 2,
+                                                                           (int)sx[a][t >> 1]);
       };
       step(std::integral_constant<int, 0>());
       step(std::integral_constant<int, 1>());
@@ -360,26 +453,61 @@ matmul_tiles(MatmulParams p, uint32_t groups, uint32_t tm, uint32_t tn)
          step(std::integral_constant<int, 3>());
       }
    }
-   // register i of a product: row 8 (i / 4) + 4 half + i % 4 of x, row lane % 32 of w
-   O* out = static_cast<O*>(p.out);
+   // Register i of a product: row 8 (i / 4) + 4 half + i % 4 of w, row lane % 32 of x.  Each
+   // wavefront turns its results in its share of the LDS and stores whole 16-byte
+   // pieces of rows.
+   constexpr int COLS = FN * 32, PITCH = COLS * (int)sizeof(O) + 16, SHARE = (2 * SLAB + SCALES) / WAVES;
+   constexpr int PASS = SHARE / (32 * PITCH) < FM ? SHARE / (32 * PITCH) : FM;    // 32-row parts at a time
+   static_assert(PASS > 0 && FM % PASS == 0, "a wavefront's share of the LDS holds whole parts");
+   constexpr int PIECE = 16 / (int)sizeof(O), ACROSS = COLS / PIECE, DOWN = 64 / ACROSS;
+   struct __attribute__((packed, aligned(sizeof(O)))) Piece { O e[PIECE]; };
+   __syncthreads();
+   uint8_t* const mine = lds + wave * SHARE;
+   O* out = static_cast<O*>(p.out) + m0 * p.ld + n0;
 #pragma unroll
-   for(int b = 0; b < FN; b++) {
-      const int j = wn + b * 32 + (lane & 31);
-      const float bias = p.bias && j < nl ? p.bias[n0 + j] : 0.0f;
+   for(int a0 = 0; a0 < FM; a0 += PASS) {
 #pragma unroll
-      for(int a = 0; a < FM; a++)
+      for(int b = 0; b < FN; b++)
 #pragma unroll
-         for(int i = 0; i < 16; i++) {
-            const int r = wm + a * 32 + 8 * (i / 4) + 4 * half + i % 4;
-            if(r < ml && j < nl) out[(m0 + r) * p.ld + n0 + j] = (O)(acc[a][b][i] + bias);
+         for(int q = 0; q < 4; q++) {
+            const int j = b * 32 + q * 8 + half * 4;
+            float bias[4] = {};
+            if(p.bias)
+#pragma unroll
+               for(int i = 0; i < 4; i++) bias[i] = wn + j + i < nl ? p.bias[n0 + wn + j + i] : 0.0f;
+#pragma unroll
+            for(int a = a0; a < a0 + PASS; a++) {
+               struct alignas(4 * sizeof(O)) Four { O e[4]; } v;
+#pragma unroll
+               for(int i = 0; i < 4; i++) v.e[i] = (O)(acc[a][b][q * 4 + i] + bias[i]);
+               *reinterpret_cast<Four*>(mine + ((a - a0) * 32 + (lane & 31)) * PITCH + j * sizeof(O)) = v;
+            }
          }
+      __builtin_amdgcn_wave_barrier();
+      const int j = wn + (lane % ACROSS) * PIECE;
+#pragma unroll 4
+      for(int i = 0; i < PASS * 32 / DOWN; i++) {
+         const int in = i * DOWN + lane / ACROSS, r = wm + a0 * 32 + in;
+         const u32x4 v = *reinterpret_cast<const u32x4*>(mine + in * PITCH + (lane % ACROSS) * 16);
+         if(r >= ml) continue;
+         const Piece piece = __builtin_bit_cast(Piece, v);
+         O* to = out + (int64_t)r * p.ld + j;
+         if(j + PIECE <= nl) {
+            *reinterpret_cast<Piece*>(to) = piece;
+         } else {
+#pragma unroll
+            for(int e = 0; e < PIECE; e++)
+               if(j + e < nl) to[e] = piece.e[e];
+         }
+      }
+      __builtin_amdgcn_wave_barrier();
    }
 }
 
 template<class O, int BM, int BN, int WM, int WN>
 hipError_t tiles_shape(const MatmulParams& p, hipStream_t s)
 {
-   constexpr size_t bytes = (size_t)(BM + BN) * (2 * 128 + 2 * 16);
+   constexpr size_t bytes = (size_t)(BM + BN) * (2 * 128 + 64);
    const int64_t groups = padded(p.k) / kGroup, tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
    if(tm * tn > 0x7fffffff) return hipErrorInvalidValue;
    static std::atomic<uint64_t> mask{0};
@@ -390,57 +518,81 @@ hipError_t tiles_shape(const MatmulParams& p, hipStream_t s)
    return hipGetLastError();
 }
 
-int wavefronts(int64_t groups, int most)
+// wavefronts for so many runs: a power of two, `most` at most
+int wavefronts(int64_t runs, int most)
 {
    int w = 1;
-   while(w < most && w * 2 <= groups) w *= 2;
+   while(w < most && w < runs) w *= 2;
    return w;
 }
 
-template<class O, int MT, int NT>
+template<class O, int MT, int NT, int DEPTH>
 hipError_t rows_shape(const MatmulParams& p, hipStream_t s)
 {
    const int64_t groups = padded(p.k) / kGroup;
-   const int waves = wavefronts(groups, most_waves(MT * NT));
+   if(groups > 0x3fffffff) return hipErrorInvalidValue;
+   const int waves = wavefronts((groups + kRun - 1) / kRun, most_waves(MT * NT));
    const int64_t gx = (p.n + 16 * NT - 1) / (16 * NT), gy = (p.m + 16 * MT - 1) / (16 * MT);
    if(gx > 0x7fffffff || gy > 65535) return hipErrorInvalidValue;
-   matmul_rows<O, MT, NT><<<dim3((unsigned)gx, (unsigned)gy), waves * 64, (size_t)waves * MT * NT * 1024, s>>>(
-      p, groups, waves);
+   matmul_rows<O, MT, NT, DEPTH><<<dim3((unsigned)gx, (unsigned)gy), waves * 64, (size_t)waves * MT * NT * 1024, s>>>(
+      p, (int)groups, waves);
    return hipGetLastError();
 }
 
+int64_t tiles(const MatmulParams& p, int64_t rows, int64_t cols)
+{
+   return ((p.m + rows - 1) / rows) * ((p.n + cols - 1) / cols);
+}
+
+// The kernel for a size, on MI355X's 256 CUs; us at m x n x k.
+//   Up to 16 rows: 16 rows of w a workgroup, 32 where 16 are more than 256 workgroups (1 x 8192
+//     x 8192 11.6 / 9.3).
+//   At most 64 tiles of 64 x 64 and k long: the largest of 16 x 16, 32 x 16 and 32 x 32 of
+//     at most 256 workgroups, with K split over their wavefronts, against 64 x 64 staged:
+//     64 x 512 x 8192 6.7 / 13.6, 32 x 4096 x 4096 5.7 / 8.3, 512 x 512 x 8192 12.4 / 17.1; at
+//     64 x 512 x 512 even.
+//   Staged tiles: 256 x 256, one a CU, runs at 1.2 times the rate of 128 x 128, two a CU, so
+//     the rounds that each needs decide: 4096 x 3200 x 2048 22.2 / 24.3, 8192 x 3200 x 2048
+//     41.7 / 43.8, but 2048 x 4096 x 4096 32.9 / 25.6, 8192 x 2560 x 4096 66.5 / 58.7.
+//     64 x 64 below 256 tiles of 128 x 128: 1001 x 2000 x 1504 8.3 -> 6.3, 256 x 4096 x 4096
+//     14.5 -> 10.3.
 template<class O>
 hipError_t matmul_typed(const MatmulParams& p, hipStream_t s)
 {
-   if(p.m <= 16) return rows_shape<O, 1, 1>(p, s);
-   if(p.m <= 32) return rows_shape<O, 2, 1>(p, s);
-   // a tile's offsets are 32-bit: 256 rows of k / 2 bytes
-   if(p.k <= (int64_t)1 << 24) {
-      const int64_t big = ((p.m + 255) / 256) * ((p.n + 255) / 256);
-      if(big >= 200) return tiles_shape<O, 256, 256, 2, 4>(p, s);
-      if(p.m > 64) return tiles_shape<O, 128, 128, 2, 2>(p, s);
+   if(p.m <= 16) return p.n > 16 * 256 ? rows_shape<O, 1, 2, 2>(p, s) : rows_shape<O, 1, 1, 2>(p, s);
+   const bool far = p.k > (int64_t)1 << 24;           // a staged tile's offsets are 32-bit: 256 rows of k / 2 bytes
+   if(p.k >= 2048 || far) {
+      if(tiles(p, 16, 16) <= 256) return rows_shape<O, 1, 1, 2>(p, s);
+      if(tiles(p, 32, 16) <= 256) return rows_shape<O, 2, 1, 2>(p, s);
+      if(tiles(p, 32, 32) <= 256 || far) return rows_shape<O, 2, 2, 2>(p, s);
    }
-   return rows_shape<O, 4, 4>(p, s);
+   const int64_t big = tiles(p, 256, 256), mid = tiles(p, 128, 128);
+   if(5 * ((big + 255) / 256) <= 3 * ((mid + 511) / 512)) return tiles_shape<O, 256, 256, 2, 4>(p, s);
+   if(mid >= 256) return tiles_shape<O, 128, 128, 2, 2>(p, s);
+   return tiles_shape<O, 64, 64, 2, 2>(p, s);
 }
 
-template<class T, class O, int MT, int NT>
+template<class T, class O, int MT, int NT, int DEPTH>
 hipError_t linear_shape(const MatmulParams& p, hipStream_t s)
 {
    const int64_t groups = padded(p.k) / kGroup;
-   const int waves = wavefronts(groups, most_waves(MT * NT));
+   if(groups > 0x3fffffff) return hipErrorInvalidValue;
+   const int waves = wavefronts((groups + kRun - 1) / kRun, most_waves(MT * NT));
    const int64_t gx = (p.n + 16 * NT - 1) / (16 * NT), gy = (p.m + 16 * MT - 1) / (16 * MT);
    if(gx > 0x7fffffff || gy > 65535) return hipErrorInvalidValue;
-   linear_rows<T, O, MT, NT><<<dim3((unsigned)gx, (unsigned)gy), waves * 64, (size_t)waves * MT * NT * 1024, s>>>(
-      p, groups, waves);
+   linear_rows<T, O, MT, NT, DEPTH><<<dim3((unsigned)gx, (unsigned)gy), waves * 64, (size_t)waves * MT * NT * 1024,
+                                      s>>>(p, (int)groups, waves);
    return hipGetLastError();
 }
 
 template<class T, class O>
 hipError_t linear_typed(const MatmulParams& p, hipStream_t s)
 {
-   if(p.m <= 16) return linear_shape<T, O, 1, 1>(p, s);
-   if(p.m <= 32) return linear_shape<T, O, 2, 1>(p, s);
-   return linear_shape<T, O, 4, 1>(p, s);
+   // 32 rows of w a workgroup share x's loads; 16 where 32 would leave CUs without one
+   const bool wide = p.n > 16 * 256;
+   if(p.m <= 16) return wide ? linear_shape<T, O, 1, 2, 2>(p, s) : linear_shape<T, O, 1, 1, 2>(p, s);
+   if(p.m <= 32) return wide ? linear_shape<T, O, 2, 2, 1>(p, s) : linear_shape<T, O, 2, 1, 1>(p, s);
+   return wide ? linear_shape<T, O, 4, 2, 1>(p, s) : linear_shape<T, O, 4, 1, 1>(p, s);
 }
 
 template<class T>
