@@ -11,36 +11,64 @@ namespace {
 
 constexpr int kLanes = 256;
 
-// v[8] of row `row` from column `col` on, zeros beyond k
+// eight consecutive elements, as they are in memory
+template<class T> struct __attribute__((packed, aligned(sizeof(T)))) Eight { T e[8]; };
+struct __attribute__((packed, aligned(1))) Bytes8 { uint32_t e[2]; };
+
+// of row `row` from column `col` on, zeros beyond k
 template<class T>
-__device__ inline void load_row8(const T* x, int64_t ld, int64_t row, int64_t col, int64_t k, float (&v)[8])
+__device__ inline Eight<T> load_row8(const T* x, int64_t ld, int64_t row, int64_t col, int64_t k)
 {
    const T* p = x + row * ld + col;
-   if(col + 8 <= k) {
-      load8(p, v);
-   } else {
+   if(col + 8 <= k) return *reinterpret_cast<const Eight<T>*>(p);
+   Eight<T> v;
 #pragma unroll
-      for(int i = 0; i < 8; i++) v[i] = col + i < k ? to_float(p[i]) : 0.0f;
-   }
+   for(int i = 0; i < 8; i++) v.e[i] = col + i < k ? p[i] : (T)0.0f;
+   return v;
 }
-__device__ inline void load_rand8(const uint8_t* rand, int64_t row, int64_t col, int64_t k, uint32_t (&r)[8])
+__device__ inline u32x2 load_rand8(const uint8_t* rand, int64_t row, int64_t col, int64_t k)
 {
    const uint8_t* p = rand + row * k + col;
    if(col + 8 <= k) {
-      struct __attribute__((packed, aligned(1))) V { uint32_t e[2]; };
-      const V t = *reinterpret_cast<const V*>(p);
-#pragma unroll
-      for(int i = 0; i < 8; i++) r[i] = (t.e[i / 4] >> (8 * (i % 4))) & 255u;
-   } else {
-#pragma unroll
-      for(int i = 0; i < 8; i++) r[i] = col + i < k ? p[i] : 0u;
+      const Bytes8 t = *reinterpret_cast<const Bytes8*>(p);
+      return u32x2{t.e[0], t.e[1]};
    }
+   u32x2 r = {0, 0};
+#pragma unroll
+   for(int i = 0; i < 8; i++)
+      if(col + i < k) r[i / 4] |= (uint32_t)p[i] << (8 * (i % 4));
+   return r;
 }
 
-// Blocks along rows.  A lane holds 8 consecutive values, four lanes a block, and
-// 16 lanes a group of 128, whose four scale bytes go out as one word.  A
-// workgroup has 2^lr lanes to a row and 256 >> lr rows at a time, ROWS of them
-// per lane in flight.
+template<class T, bool RAND>
+__device__ inline uint32_t encode(const float (&v)[8], uint32_t s, u32x2 r)
+{
+   if constexpr(RAND) return encode8_random<sizeof(T) == 2>(v, s, r);
+   else               return encode8(v, s);
+}
+
+// A block's part of a row, 8 values a lane, four lanes a block: the lane's codes, and the
+// group's four scale bytes as one word, right in the first of the group's 16 lanes.
+template<class T, bool RAND>
+__device__ inline void encode_row8(const Eight<T>& x, u32x2 r, bool fit, uint32_t* codes, uint32_t* word)
+{
+   float v[8];
+   uint32_t top = 0;
+#pragma unroll
+   for(int i = 0; i < 8; i++) {
+      v[i] = to_float(x.e[i]);
+      top = umax(top, magnitude(v[i]));
+   }
+   top = umax(top, dpp<kQuadSwap1>(top));
+   top = umax(top, dpp<kQuadSwap2>(top));
+   const uint32_t s = scale_byte(top, fit);
+   *word = s | (dpp<kRowLeft4>(s) << 8);
+   *word |= dpp<kRowLeft8>(*word) << 16;
+   *codes = encode<T, RAND>(v, s, r);
+}
+
+// Blocks along rows: 16 lanes a group of 128 values.  A workgroup has 2^lr lanes to a
+// row and 256 >> lr rows at a time, ROWS of them per lane in flight.
 template<class T, bool RAND, int ROWS>
 __global__ void __launch_bounds__(kLanes)
 quantize_rows(QuantizeParams p, int64_t kp, int lr)
@@ -50,36 +78,25 @@ quantize_rows(QuantizeParams p, int64_t kp, int lr)
    const int64_t col = ((int64_t)blockIdx.x << (lr + 3)) + lane * 8;
    const int per = kLanes >> lr;
    const int64_t row0 = ((int64_t)blockIdx.y + (int64_t)blockIdx.z * gridDim.y) * (per * ROWS) + (threadIdx.x >> lr);
-   float v[ROWS][8];
-   uint32_t r[ROWS][8];
+   Eight<T> v[ROWS];
+   u32x2 r[ROWS];
    int64_t to[ROWS];
 #pragma unroll
    for(int u = 0; u < ROWS; u++) {
       const int64_t row = row0 + u * per;
       const bool in = row < p.rows && col < kp;
       to[u] = in ? (p.slots ? p.slots[row] : row) : -1;
-#pragma unroll
-      for(int i = 0; i < 8; i++) v[u][i] = 0.0f;
-      if(in && col < p.k) load_row8(x, p.ld, row, col, p.k, v[u]);
-      if constexpr(RAND) {
-#pragma unroll
-         for(int i = 0; i < 8; i++) r[u][i] = 0;
-         if(in && col < p.k) load_rand8(p.rand, row, col, p.k, r[u]);
+      v[u] = {};
+      r[u] = u32x2{0, 0};
+      if(in && col < p.k) {
+         v[u] = load_row8(x, p.ld, row, col, p.k);
+         if constexpr(RAND) r[u] = load_rand8(p.rand, row, col, p.k);
       }
    }
 #pragma unroll
    for(int u = 0; u < ROWS; u++) {
-      uint32_t top = 0;
-#pragma unroll
-      for(int i = 0; i < 8; i++) top = umax(top, magnitude(v[u][i]));
-      top = umax(top, dpp<kQuadSwap1>(top));
-      top = umax(top, dpp<kQuadSwap2>(top));
-      const uint32_t s = scale_byte(top, p.fit != 0);
-      uint32_t word = s | (dpp<kRowLeft4>(s) << 8);
-      word |= dpp<kRowLeft8>(word) << 16;
-      uint32_t c;
-      if constexpr(RAND) c = encode8_random(v[u], s, r[u]);
-      else               c = encode8(v[u], s);
+      uint32_t c, word;
+      encode_row8<T, RAND>(v[u], r[u], p.fit != 0, &c, &word);
       if(to[u] >= 0 && to[u] < p.slot_count) {
          *reinterpret_cast<uint32_t*>(p.codes + to[u] * (kp / 2) + col / 2) = c;
          if((lane & 15) == 0) *reinterpret_cast<uint32_t*>(p.scales + to[u] * (kp / kBlock) + col / kBlock) = word;
@@ -88,55 +105,59 @@ quantize_rows(QuantizeParams p, int64_t kp, int lr)
 }
 
 // Blocks along columns, and along rows too where p.codes is given, from one
-// reading: a workgroup takes 128 rows x 128 columns.  The rows' part is the
-// kernel above; the values (and random bytes) then wait in LDS in their own
-// type, and each lane takes two neighbouring columns of 32 rows: 16 bytes of
-// codes a column, four lanes a group of 128 rows.  The pair of columns (row,
-// pair) lies at slot pair ^ 16 (row / 32), so that the four lanes of a group read
-// different banks.
-template<class T> struct Pair { T a, b; };
+// reading: a workgroup takes 128 rows x 128 columns, a lane 8 values of 8 rows.  The
+// values (and random bytes) wait in LDS in their own type, and each lane takes two
+// neighbouring columns of 32 rows: 16 bytes of codes a column, four lanes a group of
+// 128 rows.  The pair of columns (row, pair) lies at slot pair ^ 16 (row / 32), so that
+// the four lanes of a group read different banks.
+template<class T> struct alignas(2 * sizeof(T)) Pair { T a, b; };
 
 template<class T, bool RAND>
 __global__ void __launch_bounds__(kLanes)
 quantize_both(QuantizeParams p, int64_t kp, int64_t rowsp)
 {
-   __shared__ Pair<T> tile[128 * 64];
-   __shared__ Pair<uint8_t> rtile[RAND ? 128 * 64 : 1];
+   __shared__ alignas(16) Pair<T> tile[128 * 64];
+   __shared__ alignas(16) Pair<uint8_t> rtile[RAND ? 128 * 64 : 8];
    const T* x = static_cast<const T*>(p.x);
    const int64_t c0 = (int64_t)blockIdx.x * 128;
    const int64_t r0 = ((int64_t)blockIdx.y + (int64_t)blockIdx.z * gridDim.y) * 128;
    if(r0 >= rowsp) return;
    const bool fit = p.fit != 0;
-   const int lane = threadIdx.x & 15;
+   const int lane = threadIdx.x & 15, first = threadIdx.x >> 4;
    const int64_t col = c0 + lane * 8;
-#pragma unroll 2
+   Eight<T> v[8];
+   u32x2 r[8];
+   if(r0 + 128 <= p.rows && c0 + 128 <= p.k) {          // a whole tile: all loads ahead
+#pragma unroll
+      for(int u = 0; u < 8; u++) {
+         v[u] = *reinterpret_cast<const Eight<T>*>(x + (r0 + u * 16 + first) * p.ld + col);
+         if constexpr(RAND) {
+            const Bytes8 t = *reinterpret_cast<const Bytes8*>(p.rand + (r0 + u * 16 + first) * p.k + col);
+            r[u] = u32x2{t.e[0], t.e[1]};
+         }
+      }
+   } else {
+#pragma unroll
+      for(int u = 0; u < 8; u++) {
+         const int64_t row = r0 + u * 16 + first;
+         v[u] = {};
+         r[u] = u32x2{0, 0};
+         if(row < p.rows && col < p.k) {
+            v[u] = load_row8(x, p.ld, row, col, p.k);
+            if constexpr(RAND) r[u] = load_rand8(p.rand, row, col, p.k);
+         }
+      }
+   }
+#pragma unroll
    for(int u = 0; u < 8; u++) {
-      const int lrow = u * 16 + (threadIdx.x >> 4);
-      const int64_t row = r0 + lrow;
-      float v[8] = {};
-      uint32_t r[8] = {};
-      if(row < p.rows && col < p.k) {
-         load_row8(x, p.ld, row, col, p.k, v);
-         if constexpr(RAND) load_rand8(p.rand, row, col, p.k, r);
-      }
-#pragma unroll
-      for(int i = 0; i < 4; i++) {
-         const int at = lrow * 64 + ((lane * 4 + i) ^ ((lrow >> 5) << 4));
-         tile[at] = Pair<T>{(T)v[2 * i], (T)v[2 * i + 1]};
-         if constexpr(RAND) rtile[at] = Pair<uint8_t>{(uint8_t)r[2 * i], (uint8_t)r[2 * i + 1]};
-      }
+      const int lrow = u * 16 + first, at = lrow * 64 + ((lane * 4) ^ ((lrow >> 5) << 4));
+      struct alignas(16) Whole { T e[8]; };
+      *reinterpret_cast<Whole*>(&tile[at]) = __builtin_bit_cast(Whole, v[u]);
+      if constexpr(RAND) *reinterpret_cast<u32x2*>(&rtile[at]) = r[u];
       if(p.codes) {
-         uint32_t top = 0;
-#pragma unroll
-         for(int i = 0; i < 8; i++) top = umax(top, magnitude(v[i]));
-         top = umax(top, dpp<kQuadSwap1>(top));
-         top = umax(top, dpp<kQuadSwap2>(top));
-         const uint32_t s = scale_byte(top, fit);
-         uint32_t word = s | (dpp<kRowLeft4>(s) << 8);
-         word |= dpp<kRowLeft8>(word) << 16;
-         uint32_t c;
-         if constexpr(RAND) c = encode8_random(v, s, r);
-         else               c = encode8(v, s);
+         const int64_t row = r0 + lrow;
+         uint32_t c, word;
+         encode_row8<T, RAND>(v[u], r[u], fit, &c, &word);
          if(row < p.rows) {
             *reinterpret_cast<uint32_t*>(p.codes + row * (kp / 2) + col / 2) = c;
             if(lane == 0) *reinterpret_cast<uint32_t*>(p.scales + row * (kp / kBlock) + col / kBlock) = word;
@@ -146,12 +167,15 @@ quantize_both(QuantizeParams p, int64_t kp, int64_t rowsp)
    __syncthreads();
    const int blk = threadIdx.x & 3, pair = threadIdx.x >> 2;
    const int base = blk * 32 * 64 + (pair ^ (blk << 4));
+   Pair<T> t[32];
+   Pair<uint8_t> b[32];
    uint32_t top[2] = {0, 0};
 #pragma unroll
    for(int i = 0; i < 32; i++) {
-      const Pair<T> t = tile[base + i * 64];
-      top[0] = umax(top[0], magnitude(to_float(t.a)));
-      top[1] = umax(top[1], magnitude(to_float(t.b)));
+      t[i] = tile[base + i * 64];
+      if constexpr(RAND) b[i] = rtile[base + i * 64];
+      top[0] = umax(top[0], magnitude(to_float(t[i].a)));
+      top[1] = umax(top[1], magnitude(to_float(t[i].b)));
    }
 #pragma unroll
    for(int h = 0; h < 2; h++) {
@@ -161,16 +185,14 @@ quantize_both(QuantizeParams p, int64_t kp, int64_t rowsp)
       u32x4 c;
 #pragma unroll
       for(int q = 0; q < 4; q++) {
-         float v[8];
-         uint32_t r[8];
+         float w[8];
+         u32x2 rr = {0, 0};
 #pragma unroll
          for(int i = 0; i < 8; i++) {
-            const int at = base + (q * 8 + i) * 64;
-            v[i] = to_float(h ? tile[at].b : tile[at].a);
-            if constexpr(RAND) r[i] = h ? rtile[at].b : rtile[at].a;
+            w[i] = to_float(h ? t[q * 8 + i].b : t[q * 8 + i].a);
+            if constexpr(RAND) rr[i / 4] |= (uint32_t)(h ? b[q * 8 + i].b : b[q * 8 + i].a) << (8 * (i % 4));
          }
-         if constexpr(RAND) c[q] = encode8_random(v, s, r);
-         else               c[q] = encode8(v, s);
+         c[q] = encode<T, RAND>(w, s, rr);
       }
       const int64_t tcol = c0 + pair * 2 + h;
       if(tcol < p.k) {

@@ -5,6 +5,8 @@
 #include "mx4_device.hpp"
 #include "mx4_internal.hpp"
 
+#include <type_traits>
+
 namespace fufft {
 namespace mx4 {
 
@@ -120,102 +122,149 @@ read_channels(CacheParams c, T* out, int64_t length, int64_t cp)
 }
 
 // out[b][channel] = sum over j < min(len_b, taps) of taps[j][channel] times the
-// value of token len_b - 1 - j.  8 channels a lane; a workgroup has L = 1 << lr
-// lanes to a token and 256 / L runs of TAPS taps at a time, for SEQS sequences
-// that share the taps it holds.  It covers taps [y * chunk, (y + 1) * chunk); the
-// sums of its runs are joined in LDS, those of the chunks by join_splits, both in
-// a fixed order.
-template<class T, int SEQS, int TAPS>
-__global__ void __launch_bounds__(kLanes)
-cache_conv(CacheParams c, const T* taps, int64_t tap_count, int64_t chunk, int64_t cp, int lr, float* sums)
+// value of token len_b - 1 - j.  The bytes bound it: 17/32 a token and channel, and the taps,
+// which weigh most where few sequences share them.
+//
+// A wavefront has one token at a time of each of SEQS sequences, CH channels a lane, so that
+// pages and rows are scalar work, and reads TAPS taps and their tokens of every
+// sequence before it uses them.  A workgroup covers one slice of 64 CH channels and
+// one split, taps [split * chunk, ...), its wavefronts taking TAPS taps in turn; their sums are
+// joined in LDS, those of the splits by join_splits, both in a fixed order.  The
+// workgroups of all sequence groups that read the same taps follow each other on one XCD, whose
+// L2 then has them.
+template<int CH> struct Codes;
+template<> struct Codes<8> { typedef uint32_t type; };
+template<> struct Codes<4> { typedef uint16_t type; };
+
+template<int CH>
+__device__ inline void decode(uint32_t c, uint32_t s, float (&v)[CH])
 {
-   __shared__ float join[kLanes * 8];
-   const int lane = threadIdx.x & ((1 << lr) - 1), run = threadIdx.x >> lr, runs = kLanes >> lr;
-   const int64_t col = ((int64_t)blockIdx.x << (lr + 3)) + lane * 8;
-   const int64_t b0 = (int64_t)blockIdx.z * SEQS;
-   const int64_t j_begin = (int64_t)blockIdx.y * chunk;
-   int64_t n[SEQS], most = 0;
+   const float p = scale_operand(s);
+   const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, p, 0);
+   const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, p, 1);
+   v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1];
+   if constexpr(CH == 8) {
+      const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, p, 2);
+      const f32x2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, p, 3);
+      v[4] = d[0]; v[5] = d[1]; v[6] = e[0]; v[7] = e[1];
+   }
+}
+
+template<class T, int CH, int SEQS, int TAPS, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES)
+cache_conv(CacheParams c, const T* taps, uint32_t tap_count, uint32_t chunk, uint32_t cp, uint32_t slices, uint32_t parts,
+           uint32_t seq_groups, float* sums)
+{
+   typedef typename Codes<CH>::type Code;
+   struct __attribute__((packed, aligned(sizeof(T)))) Taps { T e[CH]; };
+   __shared__ float join[WAVES * 64 * CH];
+   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+   // ids 8 apart run on one XCD: part 8 i + (id % 8) for every group of sequences, then the next i
+   const uint32_t set = blockIdx.x / (8 * seq_groups), in = blockIdx.x % (8 * seq_groups);
+   const uint32_t part = set * 8 + in % 8;
+   if(part >= parts) return;
+   const uint32_t split = part / slices, col = part % slices * (64 * CH) + lane * CH;
+   const int64_t b0 = (int64_t)(in / 8) * SEQS;
+   // tokens and taps count in 32 bits, as lengths do.  Sequence g takes part in taps j < end[g].
+   uint32_t n[SEQS], end[SEQS], j_end = 0;
+   const uint32_t chunk_end = (split + 1) * chunk < tap_count ? (split + 1) * chunk : tap_count;
 #pragma unroll
    for(int g = 0; g < SEQS; g++) {
-      n[g] = b0 + g < c.batch ? sequence_length(c, b0 + g) : 0;
-      most = n[g] > most ? n[g] : most;
+      n[g] = b0 + g < c.batch && c.pages > 0 ? (uint32_t)sequence_length(c, b0 + g) : 0;
+      end[g] = n[g] < chunk_end ? n[g] : chunk_end;
+      j_end = end[g] > j_end ? end[g] : j_end;
    }
-   int64_t j_end = j_begin + chunk;
-   if(j_end > tap_count) j_end = tap_count;
-   if(j_end > most) j_end = most;
-   float acc[SEQS][8] = {};
-   if(col < c.channels) {
-      for(int64_t j0 = j_begin + run * TAPS; j0 < j_end; j0 += (int64_t)runs * TAPS) {
-         float h[TAPS][8];
+   const uint32_t pages = c.pages < 0x7fffffff ? (uint32_t)c.pages : 0x7fffffffu, page_mask = (1u << c.page_log) - 1;
+   float acc[SEQS][CH] = {};
+   // Every load of a step has an address that is good, so that all go out before the first
+   // is used: taps past the end are the last one, channels past the end the last one,
+   // a token that is none is row 0 (n > 0 somewhere, so there is a page and a table).
+   auto steps = [&](auto inside) {
+      constexpr bool INSIDE = decltype(inside)::value;
+      uint32_t ch[CH];
+#pragma unroll
+      for(int i = 0; i < CH; i++) ch[i] = col + i < c.channels ? col + i : (uint32_t)c.channels - 1;
+      const uint32_t code_at = (col < cp ? col : 0) / 2, scale_at = (col < cp ? col : 0) / kBlock;
+      for(uint32_t j0 = split * chunk + wave * TAPS; j0 < j_end; j0 += WAVES * TAPS) {
+         Taps h[TAPS];
 #pragma unroll
          for(int u = 0; u < TAPS; u++) {
+            const T* row = taps + (int64_t)(j0 + u < j_end ? j0 + u : j_end - 1) * c.channels;
+            if constexpr(INSIDE) {
+               h[u] = *reinterpret_cast<const Taps*>(row + col);
+            } else {
 #pragma unroll
-            for(int i = 0; i < 8; i++) h[u][i] = 0.0f;
-            if(j0 + u < j_end) {
-               const T* at = taps + (j0 + u) * c.channels + col;
-               if(col + 8 <= c.channels) {
-                  load8(at, h[u]);
-               } else {
-#pragma unroll
-                  for(int i = 0; i < 8; i++)
-                     if(col + i < c.channels) h[u][i] = to_float(at[i]);
-               }
+               for(int i = 0; i < CH; i++) h[u].e[i] = row[ch[i]];
             }
          }
+         uint32_t q[SEQS][TAPS], s[SEQS][TAPS];
+         bool there[SEQS][TAPS];
 #pragma unroll
          for(int g = 0; g < SEQS; g++) {
-            if(j0 >= n[g]) continue;
-            const int32_t* table = c.table + (b0 + g) * c.width;
-            uint32_t q[TAPS], s[TAPS];
-            bool there[TAPS];
+            const int32_t* table = c.table + (b0 + g < c.batch ? b0 + g : c.batch - 1) * c.width;
 #pragma unroll
             for(int u = 0; u < TAPS; u++) {
-               const int64_t t = n[g] - 1 - j0 - u;
-               const int64_t from = t >= 0 && j0 + u < j_end ? cache_row(c, table, t) : -1;
-               there[u] = from >= 0;
-               q[u] = s[u] = 0;
-               if(there[u]) {
-                  q[u] = *reinterpret_cast<const uint32_t*>(c.codes + from * (cp / 2) + col / 2);
-                  s[u] = c.scales[from * (cp / kBlock) + col / kBlock];
-               }
-            }
-#pragma unroll
-            for(int u = 0; u < TAPS; u++) {
-               if(!there[u]) continue;       // a tap that meets no token may be anything
-               float v[8];
-               decode8(q[u], s[u], v);
-#pragma unroll
-               for(int i = 0; i < 8; i++) acc[g][i] = fmaf(h[u][i], v[i], acc[g][i]);
+               const int32_t left = (int32_t)(n[g] - 1 - j0 - u);
+               const uint32_t t = left > 0 ? left : 0, pg = (uint32_t)table[t >> c.page_log];
+               there[g][u] = j0 + u < end[g] && pg < pages;
+               const uint64_t row = ((uint64_t)(pg < pages ? pg : 0) << c.page_log) + (t & page_mask);
+               const uint64_t from = row * (cp / 2);
+               q[g][u] = *reinterpret_cast<const Code*>(c.codes + from + code_at);
+               s[g][u] = (c.scales + (from >> 4))[scale_at];
             }
          }
+#pragma unroll
+         for(int g = 0; g < SEQS; g++)
+#pragma unroll
+            for(int u = 0; u < TAPS; u++) {
+               if(!there[g][u]) continue;       // a tap that meets no token may be anything
+               float v[CH];
+               decode<CH>(q[g][u], s[g][u], v);
+#pragma unroll
+               for(int i = 0; i < CH; i++) acc[g][i] = fmaf(to_float(h[u].e[i]), v[i], acc[g][i]);
+            }
       }
-   }
+   };
+   if(col - lane * CH + 64 * CH <= c.channels) steps(std::true_type());
+   else                                        steps(std::false_type());
 #pragma unroll
    for(int g = 0; g < SEQS; g++) {
       if(b0 + g >= c.batch) break;
       if(g) __syncthreads();
 #pragma unroll
-      for(int i = 0; i < 8; i++) join[i * kLanes + threadIdx.x] = acc[g][i];
+      for(int i = 0; i < CH; i++) join[(wave * CH + i) * 64 + lane] = acc[g][i];
       __syncthreads();
-      float* to = sums + ((int64_t)blockIdx.y * c.batch + b0 + g) * c.channels;
-      for(int k = threadIdx.x; k < 8 << lr; k += kLanes) {
-         const int64_t ch = ((int64_t)blockIdx.x << (lr + 3)) + k;
+      float* to = sums + ((int64_t)split * c.batch + b0 + g) * c.channels;
+      for(int k = threadIdx.x; k < 64 * CH; k += 64 * WAVES) {
+         const int64_t ch = (int64_t)(col - lane * CH) + k;
          float a = 0.0f;
-         for(int r = 0; r < runs; r++) a += join[(k & 7) * kLanes + (r << lr) + (k >> 3)];
+#pragma unroll
+         for(int w = 0; w < WAVES; w++) a += join[(w * CH + k % CH) * 64 + k / CH];
          if(ch < c.channels) to[ch] = a;
       }
    }
 }
 
+// The splits' sums, 8 lanes a result, each taking every eighth.
 template<class T>
 __global__ void __launch_bounds__(kLanes)
-join_splits(const float* sums, T* out, int64_t count, int64_t splits)
+join_splits(const float* sums, T* out, int64_t count, int splits)
 {
-   const int64_t i = (int64_t)blockIdx.x * kLanes + threadIdx.x;
-   if(i >= count) return;
+   __shared__ float part[8][32];
+   const int lane = threadIdx.x & 31, k0 = threadIdx.x >> 5;
+   const int64_t i = (int64_t)blockIdx.x * 32 + lane;
    float a = 0.0f;
-   for(int64_t k = 0; k < splits; k++) a += sums[k * count + i];
-   out[i] = (T)a;
+   if(i < count) {
+#pragma unroll 8
+      for(int k = k0; k < splits; k += 8) a += sums[k * count + i];
+   }
+   part[k0][lane] = a;
+   __syncthreads();
+   if(k0 == 0 && i < count) {
+#pragma unroll
+      for(int k = 1; k < 8; k++) a += part[k][lane];
+      out[i] = (T)a;
+   }
 }
 
 template<class T>
@@ -239,37 +288,44 @@ hipError_t read_typed(const CacheParams& c, T* out, int64_t length, bool channel
    return hipGetLastError();
 }
 
-template<class T, int SEQS, int TAPS>
+template<class T, int CH, int SEQS, int TAPS, int WAVES>
 hipError_t conv_shape(const CacheParams& c, const T* taps, int64_t tap_count, float* direct, float* work,
-                      int64_t splits, int64_t* used, hipStream_t s)
+                      int64_t splits, int* used, hipStream_t s)
 {
-   const int64_t cp = padded(c.channels);
-   int lr = 4;
-   while(lr < 6 && ((int64_t)8 << lr) < cp) lr++;
-   const int64_t gx = (cp / 8 + (1 << lr) - 1) >> lr, gz = (c.batch + SEQS - 1) / SEQS;
-   const int64_t step = (int64_t)(kLanes >> lr) * TAPS;
-   int64_t want = (2048 + gx * gz - 1) / (gx * gz);
+   const int64_t cp = padded(c.channels), slices = (cp + 64 * CH - 1) / (64 * CH);
+   if(cp > 0x7fffffff) return hipErrorInvalidValue;
+   const int64_t seq_groups = (c.batch + SEQS - 1) / SEQS, step = WAVES * TAPS;
+   // two workgroups a CU, each with one step at least
+   int64_t want = (512 + slices * seq_groups - 1) / (slices * seq_groups);
    const int64_t most = (tap_count + step - 1) / step;
    want = want < most ? want : most;
    want = want < splits ? want : splits;
    if(want < 1) want = 1;
    int64_t chunk = ((tap_count + want - 1) / want + step - 1) / step * step;
    if(chunk < step) chunk = step;
-   const int64_t gy = tap_count > 0 ? (tap_count + chunk - 1) / chunk : 1;
-   if(gx > 0x7fffffff || gy > 65535 || gz > 65535) return hipErrorInvalidValue;
-   float* sums = gy == 1 && direct ? direct : work;
-   cache_conv<T, SEQS, TAPS><<<dim3((unsigned)gx, (unsigned)gy, (unsigned)gz), kLanes, 0, s>>>(
-      c, taps, tap_count, chunk, cp, lr, sums);
-   *used = sums == direct ? 0 : gy;
+   const int64_t parts = slices * (tap_count > 0 ? (tap_count + chunk - 1) / chunk : 1);
+   const int64_t grid = (parts + 7) / 8 * 8 * seq_groups;
+   if(grid > 0x7fffffff || parts / slices > 0x7fffffff) return hipErrorInvalidValue;
+   const int count = (int)(parts / slices);
+   float* sums = count == 1 && direct ? direct : work;
+   cache_conv<T, CH, SEQS, TAPS, WAVES><<<(unsigned)grid, 64 * WAVES, 0, s>>>(
+      c, taps, (uint32_t)tap_count, (uint32_t)chunk, (uint32_t)cp, (uint32_t)slices, (uint32_t)parts, (uint32_t)seq_groups, sums);
+   *used = sums == direct ? 0 : count;
    return hipGetLastError();
 }
 
 template<class T>
 hipError_t conv_typed(const CacheParams& c, const T* taps, int64_t tap_count, float* direct, float* work,
-                      int64_t splits, int64_t* used, hipStream_t s)
+                      int64_t splits, int* used, hipStream_t s)
 {
-   if(c.batch == 1) return conv_shape<T, 1, 4>(c, taps, tap_count, direct, work, splits, used, s);
-   return conv_shape<T, 2, 4>(c, taps, tap_count, direct, work, splits, used, s);
+   // One sequence: the taps' bytes are most of the work, and many wavefronts with 4 channels a
+   // lane find room (1 x 65536 x 1024, bf16 taps: 33 us of a floor of 33).  More: what
+   // scalar work a token costs counts, so 8 channels, and registers for four sequences with
+   // 2 taps (24 x 8000 x 4096, fp32 taps: 4 x 2 taps 126 us, 4 x 4 148, 2 x 4 170; 3 x 30000 x
+   // 768 58, 54, 45).
+   if(c.batch == 1) return conv_shape<T, 4, 1, 8, 16>(c, taps, tap_count, direct, work, splits, used, s);
+   if(c.batch <= 3) return conv_shape<T, 8, 2, 4, 8>(c, taps, tap_count, direct, work, splits, used, s);
+   return conv_shape<T, 8, 4, 2, 8>(c, taps, tap_count, direct, work, splits, used, s);
 }
 
 }  // namespace
@@ -289,12 +345,13 @@ hipError_t launch_cache_conv(const CacheParams& c, const void* taps, int tap_typ
                              int out_type, float* work, int64_t splits, hipStream_t s)
 {
    if(c.batch <= 0 || c.channels <= 0) return hipSuccess;
-   // no token is beyond the page table
-   const int64_t most = c.width << c.page_log;
+   // no token is beyond the page table, nor beyond a 32-bit length
+   int64_t most = c.width << c.page_log;
+   if(most > 0x7fffffff) most = 0x7fffffff;
    if(tap_count > most) tap_count = most;
    // fp32 results that one workgroup sums need no workspace and no join
    float* direct = out_type == T_F32 ? static_cast<float*>(out) : nullptr;
-   int64_t used = 0;
+   int used = 0;
    hipError_t e;
    switch(tap_type) {
       case T_F32:  e = conv_typed(c, static_cast<const float*>(taps), tap_count, direct, work, splits, &used, s); break;
@@ -302,7 +359,7 @@ hipError_t launch_cache_conv(const CacheParams& c, const void* taps, int tap_typ
       default:     e = conv_typed(c, static_cast<const f16*>(taps), tap_count, direct, work, splits, &used, s); break;
    }
    if(e != hipSuccess || used == 0) return e;
-   const int64_t count = c.batch * c.channels, groups = (count + kLanes - 1) / kLanes;
+   const int64_t count = c.batch * c.channels, groups = (count + 31) / 32;
    if(groups > 0x7fffffff) return hipErrorInvalidValue;
    const dim3 g((unsigned)groups);
    switch(out_type) {

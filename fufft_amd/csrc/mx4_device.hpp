@@ -103,13 +103,42 @@ __device__ inline uint32_t encode_random(float v, float inverse, uint32_t r)
    c = c > 7u ? 7u : c;
    return c | ((__float_as_uint(v) >> 28) & 8u);
 }
-__device__ inline uint32_t encode8_random(const float (&v)[8], uint32_t s, const uint32_t (&r)[8])
+// The same for values of 16-bit types by the conversion to the nearest, in half the
+// instructions.  With p the power of two below a (1 at least, 4 at most, so that a step
+// is p / 2), c = a + p ((r + 1/2) / 512 - 1/4 + 2^-22) is half a step below a plus that
+// share of a step, so the nearest code to c is the one to take, but where c falls
+// below the power of two under a, past which the steps are finer: c is at least that.
+// The 2^-22 p decides ties upwards; a has 11 bits, so c is exact and nothing else lies
+// that near a tie.  (r, K: the share is exact in fp32 too.)
+__device__ inline float dithered(float v, float inverse, float r)
+{
+   const float a = __uint_as_float(magnitude(v)) * inverse;
+   const float below = __uint_as_float(__float_as_uint(a) & 0x7f800000u);
+   const float p = __builtin_amdgcn_fmed3f(below, 1.0f, 4.0f);
+   const float share = fmaf(r, 1.0f / 512.0f, 1.0f / 1024.0f - 0.25f + 0x1p-22f);
+   const float c = fmaxf(fmaf(p, share, a), below);
+   return __uint_as_float((__float_as_uint(v) & 0x80000000u) | __float_as_uint(c));
+}
+
+// eight values with their random bytes, two words of four; 16 bits: the values are of a 16-bit type
+template<bool BITS16>
+__device__ inline uint32_t encode8_random(const float (&v)[8], uint32_t s, u32x2 r)
 {
    if(s == 255u) return 0u;
    const float inverse = __uint_as_float((254u - s) << 23);   // 2^(127 - s); s <= 253 here
    uint32_t c = 0;
+   if constexpr(BITS16) {
+      float d[8];
 #pragma unroll
-   for(int i = 0; i < 8; i++) c |= encode_random(v[i], inverse, r[i]) << (4 * i);
+      for(int i = 0; i < 8; i++) d[i] = dithered(v[i], inverse, (float)((r[i / 4] >> (8 * (i % 4))) & 255u));
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, d[0], d[1], 1.0f, 0);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, d[2], d[3], 1.0f, 1);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, d[4], d[5], 1.0f, 2);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, d[6], d[7], 1.0f, 3);
+   } else {
+#pragma unroll
+      for(int i = 0; i < 8; i++) c |= encode_random(v[i], inverse, (r[i / 4] >> (8 * (i % 4))) & 255u) << (4 * i);
+   }
    return c;
 }
 
