@@ -158,6 +158,7 @@ if torch is not None:
     }
     # element types of the mx4 calls (FUFFT_F32, FUFFT_BF16, FUFFT_F16)
     _ELEMENT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    _BYTE = torch.uint8
     # the reads every launch makes, without torch.cuda's Python layer (which
     # initialises the GPU on first use: a tensor that is on one has done that)
     _TENSOR = torch.Tensor
@@ -736,9 +737,17 @@ def _name(table: dict, key, name: str) -> int:
     return table[key]
 
 
+# These calls are short (a few rows take the GPU 2 to 4 us), so their arguments are read as
+# _ptrs reads its own: the case that passes in the cheapest reads of each property, any
+# other through the checks that say what is wrong.  (48 rows of 4096 made 4-bit, host time a
+# call: 7.3 us with _ptrs and a check of x's device by name, 5.5 so, 3.2 of them the launch.)
+
 def _matrix(x, name: str):
     """(type, leading dimension, rows, columns) of a 2D tensor of elements, checked but for
     its device (the last check, _on_gpu)."""
+    if type(x) is _TENSOR and x.dtype in _ELEMENT and x.dim() == 2 and x.is_contiguous():
+        rows, k = x.shape
+        return _ELEMENT[x.dtype], k, rows, k
     if torch is None or not isinstance(x, torch.Tensor):
         raise TypeError(f"{name}: expected a torch tensor in GPU memory, got {type(x).__name__}")
     kind = _ELEMENT.get(x.dtype)
@@ -757,17 +766,39 @@ def _matrix(x, name: str):
 
 
 def _on_gpu(*pairs) -> None:
+    """Every tensor (None: an argument that is not given) is on the current GPU."""
+    gpu = None
     for x, name in pairs:
+        if x is None:
+            continue
+        if x.is_cuda:
+            if gpu is None:
+                gpu = _current_device()
+            if x.get_device() == gpu:
+                continue
         _check_device(x, name)
 
 
+def _array(x, name: str, nbytes: int, kind: str) -> int:
+    """The address of a contiguous array of at least nbytes, checked but for its device."""
+    if not (type(x) is _TENSOR and x.dtype in _DT[kind] and x.is_contiguous() and x.nbytes >= nbytes):
+        _check_shape(x, name, nbytes, kind)
+    return x.data_ptr()
+
+
 def _blocks(codes, scales, name: str, rows: int, k: int):
-    kp = mx4_padded(k)
-    return (codes, name, rows * (kp // 2), "bytes"), (scales, name + "_scales", rows * (kp // MX4_BLOCK), "bytes")
+    """The addresses of `rows` rows of k values in blocks, checked but for their device."""
+    groups = (k + 127) // 128
+    if not (type(codes) is _TENSOR and type(scales) is _TENSOR and codes.dtype is _BYTE and scales.dtype is _BYTE
+            and codes.is_contiguous() and scales.is_contiguous() and codes.nbytes >= rows * groups * 64
+            and scales.nbytes >= rows * groups * 4):
+        _check_shape(codes, name, rows * groups * 64, "bytes")
+        _check_shape(scales, name + "_scales", rows * groups * 4, "bytes")
+    return codes.data_ptr(), scales.data_ptr()
 
 
 def _bias(bias, n: int):
-    return None if bias is None else (bias, "bias", 4 * n, "real")
+    return None if bias is None else _array(bias, "bias", 4 * n, "real")
 
 
 def mx4_quantize(x, codes=None, scales=None, codes_t=None, scales_t=None, *, rand=None, rule: str = "fit",
@@ -778,23 +809,26 @@ def mx4_quantize(x, codes=None, scales=None, codes_t=None, scales_t=None, *, ran
     down at random; None rounds to the nearest.  rule: "fit" (nothing saturates) or "floor"."""
     rule = _name(MX4_RULE, rule, "rule")
     kind, ld, rows, k = _matrix(x, "x")
-    along, across = codes is not None or scales is not None, codes_t is not None or scales_t is not None
-    if not (along or across):
+    pc = ps = qc = qs = pr = None
+    if codes is not None or scales is not None:
+        pc, ps = _blocks(codes, scales, "codes", rows, k)
+    elif codes_t is None and scales_t is None:
         raise ValueError("mx4_quantize: neither blocks along rows nor along columns are asked for")
-    none = (None, None)
-    pc, ps, qc, qs, pr = _ptrs(*(_blocks(codes, scales, "codes", rows, k) if along else none),
-                               *(_blocks(codes_t, scales_t, "codes_t", k, rows) if across else none),
-                               None if rand is None else (rand, "rand", rows * k, "bytes"))
-    _on_gpu((x, "x"))
-    check(lib.fufft_mx4_quantize(x.data_ptr(), kind, ld, rows, k, rule, pr, pc, ps, qc, qs,
-                                 _stream(stream)), "fufft_mx4_quantize")
+    if codes_t is not None or scales_t is not None:
+        qc, qs = _blocks(codes_t, scales_t, "codes_t", k, rows)
+    if rand is not None:
+        pr = _array(rand, "rand", rows * k, "bytes")
+    _on_gpu((x, "x"), (codes, "codes"), (scales, "codes_scales"), (codes_t, "codes_t"), (scales_t, "codes_t_scales"),
+            (rand, "rand"))
+    check(lib.fufft_mx4_quantize(x.data_ptr(), kind, ld, rows, k, rule, pr, pc, ps, qc, qs, _stream(stream)),
+          "fufft_mx4_quantize")
 
 
 def mx4_dequantize(codes, scales, out, stream=None) -> None:
     """The values that blocks along rows stand for, into out (rows, k)."""
     kind, ld, rows, k = _matrix(out, "out")
-    pc, ps = _ptrs(*_blocks(codes, scales, "codes", rows, k))
-    _on_gpu((out, "out"))
+    pc, ps = _blocks(codes, scales, "codes", rows, k)
+    _on_gpu((out, "out"), (codes, "codes"), (scales, "codes_scales"))
     check(lib.fufft_mx4_dequantize(pc, ps, out.data_ptr(), kind, ld, rows, k, _stream(stream)),
           "fufft_mx4_dequantize")
 
@@ -804,8 +838,10 @@ def mx4_matmul(a, a_scales, b, b_scales, out, k: int, bias=None, stream=None) ->
     For y = x w^T the gradients are dx = mx4_matmul(dy, w's columns) and dw = mx4_matmul(dy's
     columns, x's columns), all from mx4_quantize."""
     kind, ld, m, n = _matrix(out, "out")
-    pa, pas, pb, pbs, pbias = _ptrs(*_blocks(a, a_scales, "a", m, k), *_blocks(b, b_scales, "b", n, k), _bias(bias, n))
-    _on_gpu((out, "out"))
+    pa, pas = _blocks(a, a_scales, "a", m, k)
+    pb, pbs = _blocks(b, b_scales, "b", n, k)
+    pbias = _bias(bias, n)
+    _on_gpu((out, "out"), (a, "a"), (a_scales, "a_scales"), (b, "b"), (b_scales, "b_scales"), (bias, "bias"))
     check(lib.fufft_mx4_matmul(pa, pas, pb, pbs, pbias, out.data_ptr(), kind, ld, m, n, k, _stream(stream)),
           "fufft_mx4_matmul")
 
@@ -817,8 +853,9 @@ def mx4_linear(x, w, w_scales, out, bias=None, stream=None) -> None:
     kind, ld, rows, n = _matrix(out, "out")
     if rows != m:
         raise ValueError(f"out: {rows} rows, x has {m}")
-    pw, pws, pbias = _ptrs(*_blocks(w, w_scales, "w", n, k), _bias(bias, n))
-    _on_gpu((x, "x"), (out, "out"))
+    pw, pws = _blocks(w, w_scales, "w", n, k)
+    pbias = _bias(bias, n)
+    _on_gpu((x, "x"), (w, "w"), (w_scales, "w_scales"), (out, "out"), (bias, "bias"))
     check(lib.fufft_mx4_linear(x.data_ptr(), x_kind, ldx, pw, pws, pbias, out.data_ptr(), kind, ld, m, n, k,
                                _stream(stream)), "fufft_mx4_linear")
 
@@ -831,22 +868,23 @@ def _cache(codes, scales, channels: int):
             raise TypeError(f"{name}: expected a torch tensor in GPU memory, got {type(x).__name__}")
         if x.dim() != 3 or x.shape[2] != last:
             raise ValueError(f"{name}: expected (pages, page, {last}), got {tuple(x.shape)}")
-    if codes.shape[:2] != scales.shape[:2]:
+    pages, page, _ = codes.shape
+    if scales.shape[0] != pages or scales.shape[1] != page:
         raise ValueError(f"codes and scales: {tuple(codes.shape[:2])} and {tuple(scales.shape[:2])} pages and tokens")
-    pages, page = codes.shape[:2]
     if page < 1 or page > 65536 or page & (page - 1):
         raise ValueError(f"codes: {page} tokens a page, not a power of two up to 65536")
     return pages, page
 
 
 def _table(table, lens):
+    """(batch, width, address of the page table, address of the lengths)."""
     if torch is None or not isinstance(table, torch.Tensor) or not isinstance(lens, torch.Tensor):
         raise TypeError("pages and lens: expected torch tensors in GPU memory")
     if table.dim() != 2 or lens.dim() != 1 or table.shape[0] != lens.shape[0]:
         raise ValueError(f"pages and lens: expected (batch, width) and (batch), got {tuple(table.shape)} and "
                          f"{tuple(lens.shape)}")
     batch, width = table.shape
-    return batch, width, (table, "pages", 4 * batch * width, "words"), (lens, "lens", 4 * batch, "words")
+    return (batch, width, _array(table, "pages", 4 * batch * width, "words"), _array(lens, "lens", 4 * batch, "words"))
 
 
 def mx4_cache_write(x, slots, codes, scales, stream=None) -> None:
@@ -854,8 +892,9 @@ def mx4_cache_write(x, slots, codes, scales, stream=None) -> None:
     different) of a cache; a slot outside it, such as -1, is skipped."""
     kind, ld, rows, channels = _matrix(x, "x")
     pages, page = _cache(codes, scales, channels)
-    pl, pc, ps = _ptrs((slots, "slots", 8 * rows, "slots"), *_blocks(codes, scales, "codes", pages * page, channels))
-    _on_gpu((x, "x"))
+    pl = _array(slots, "slots", 8 * rows, "slots")
+    pc, ps = _blocks(codes, scales, "codes", pages * page, channels)
+    _on_gpu((x, "x"), (slots, "slots"), (codes, "codes"), (scales, "scales"))
     check(lib.fufft_mx4_cache_write(x.data_ptr(), kind, ld, pl, rows, channels, pc, ps, pages * page,
                                     _stream(stream)), "fufft_mx4_cache_write")
 
@@ -869,15 +908,19 @@ def mx4_cache_read(codes, scales, pages, lens, out, order: str = "tokens", strea
         raise TypeError(f"out: expected a torch tensor in GPU memory, got {type(out).__name__}")
     if out.dtype not in _ELEMENT:
         raise ValueError(f"out: dtype {out.dtype} is not one of {', '.join(str(d) for d in _ELEMENT)}")
-    batch, width, st, sl = _table(pages, lens)
-    if out.dim() != 3 or out.shape[0] != batch:
-        raise ValueError(f"out: expected three dimensions with {batch} sequences, got {tuple(out.shape)}")
+    if out.dim() != 3:
+        raise ValueError(f"out: expected three dimensions, got {tuple(out.shape)}")
     if not out.is_contiguous():
         raise ValueError("out: tensor is not contiguous")
-    channels, length = (out.shape[1], out.shape[2]) if turned else (out.shape[2], out.shape[1])
+    sequences, length, channels = out.shape
+    if turned:
+        length, channels = channels, length
     count, page = _cache(codes, scales, channels)
-    pc, ps, pt, pn = _ptrs(*_blocks(codes, scales, "codes", count * page, channels), st, sl)
-    _on_gpu((out, "out"))
+    batch, width, pt, pn = _table(pages, lens)
+    if sequences != batch:
+        raise ValueError(f"out: {sequences} sequences, pages and lens have {batch} sequences")
+    pc, ps = _blocks(codes, scales, "codes", count * page, channels)
+    _on_gpu((out, "out"), (codes, "codes"), (scales, "scales"), (pages, "pages"), (lens, "lens"))
     check(lib.fufft_mx4_cache_read(pc, ps, count, page, channels, pt, width, pn, batch, length, out.data_ptr(),
                                    _ELEMENT[out.dtype], turned, _stream(stream)), "fufft_mx4_cache_read")
 
@@ -892,16 +935,16 @@ def mx4_cache_conv(codes, scales, pages, lens, taps, out, work=None, stream=None
         raise ValueError(f"out: {out_channels} channels, taps have {channels}")
     if (tap_count > 1 and t_ld != channels) or (batch > 1 and ld != channels):
         raise ValueError("taps and out: tensor is not contiguous")
-    rows, width, st, sl = _table(pages, lens)
-    if rows != batch:
-        raise ValueError(f"out: {batch} sequences, pages have {rows}")
     count, page = _cache(codes, scales, channels)
     splits = 0 if work is None or batch * channels == 0 else work.numel() // (batch * channels)
     if kind != 0 and splits == 0 and batch * channels > 0:
         raise ValueError("work: results in 16 bits need a workspace of one split at least")
-    pc, ps, pt, pn, pw = _ptrs(*_blocks(codes, scales, "codes", count * page, channels), st, sl,
-                               None if splits == 0 else (work, "work", 4 * splits * batch * channels, "real"))
-    _on_gpu((taps, "taps"), (out, "out"))
+    pw = None if splits == 0 else _array(work, "work", 4 * splits * batch * channels, "real")
+    rows, width, pt, pn = _table(pages, lens)
+    if rows != batch:
+        raise ValueError(f"out: {batch} sequences, pages have {rows}")
+    pc, ps = _blocks(codes, scales, "codes", count * page, channels)
+    _on_gpu((taps, "taps"), (out, "out"), (codes, "codes"), (scales, "scales"), (pages, "pages"), (lens, "lens"),
+            (work if splits else None, "work"))
     check(lib.fufft_mx4_cache_conv(pc, ps, count, page, channels, pt, width, pn, batch, taps.data_ptr(), t_kind,
-                                   tap_count, out.data_ptr(), kind, pw, splits, _stream(stream)),
-          "fufft_mx4_cache_conv")
+                                   tap_count, out.data_ptr(), kind, pw, splits, _stream(stream)), "fufft_mx4_cache_conv")

@@ -81,16 +81,31 @@ quantize_rows(QuantizeParams p, int64_t kp, int lr)
    Eight<T> v[ROWS];
    u32x2 r[ROWS];
    int64_t to[ROWS];
+   // a workgroup whose rows and columns are all there has its loads in straight code
+   const bool whole = row0 - (threadIdx.x >> lr) + per * ROWS <= p.rows && col - lane * 8 + (8 << lr) <= p.k;
+   if(whole) {
 #pragma unroll
-   for(int u = 0; u < ROWS; u++) {
-      const int64_t row = row0 + u * per;
-      const bool in = row < p.rows && col < kp;
-      to[u] = in ? (p.slots ? p.slots[row] : row) : -1;
-      v[u] = {};
-      r[u] = u32x2{0, 0};
-      if(in && col < p.k) {
-         v[u] = load_row8(x, p.ld, row, col, p.k);
-         if constexpr(RAND) r[u] = load_rand8(p.rand, row, col, p.k);
+      for(int u = 0; u < ROWS; u++) {
+         const int64_t row = row0 + u * per;
+         v[u] = *reinterpret_cast<const Eight<T>*>(x + row * p.ld + col);
+         if constexpr(RAND) {
+            const Bytes8 t = *reinterpret_cast<const Bytes8*>(p.rand + row * p.k + col);
+            r[u] = u32x2{t.e[0], t.e[1]};
+         }
+         to[u] = p.slots ? p.slots[row] : row;
+      }
+   } else {
+#pragma unroll
+      for(int u = 0; u < ROWS; u++) {
+         const int64_t row = row0 + u * per;
+         const bool in = row < p.rows && col < kp;
+         to[u] = in ? (p.slots ? p.slots[row] : row) : -1;
+         v[u] = {};
+         r[u] = u32x2{0, 0};
+         if(in && col < p.k) {
+            v[u] = load_row8(x, p.ld, row, col, p.k);
+            if constexpr(RAND) r[u] = load_rand8(p.rand, row, col, p.k);
+         }
       }
    }
 #pragma unroll
