@@ -217,6 +217,93 @@ inline int apply2d(const void* spec, const void* filt, void* out, int64_t h, int
    return fufft_apply2d_f32(spec, spec_stride, filt, filt_stride, out, h, w, batch, Mid::id, layout, stream);
 }
 
+// ---- microscaled 4-bit blocks (no reference counterpart; formats in fufft.h) ------------------
+namespace mx4 {
+
+enum class Type : int { F32 = FUFFT_F32, BF16 = FUFFT_BF16, F16 = FUFFT_F16 };
+enum class Rule : int { Fit = FUFFT_MX4_FIT, Floor = FUFFT_MX4_FLOOR };
+enum class Order : int { Tokens = FUFFT_MX4_TOKENS, Channels = FUFFT_MX4_CHANNELS };
+
+inline int64_t padded(int64_t k) { return fufft_mx4_padded(k); }
+// bytes of the codes and of the scales of `rows` rows of k values
+inline std::size_t code_bytes(int64_t rows, int64_t k) { return (std::size_t)(rows * (padded(k) / 2)); }
+inline std::size_t scale_bytes(int64_t rows, int64_t k) { return (std::size_t)(rows * (padded(k) / FUFFT_MX4_BLOCK)); }
+
+// rows of values in blocks: an operand of the products, an output of quantize
+struct Blocks {
+   void*    codes  = nullptr;
+   uint8_t* scales = nullptr;
+};
+// rows x k elements, `ld` elements from row to row (0: k, without gaps)
+struct Matrix {
+   const void* data;
+   Type        type;
+   int64_t     rows, k, ld = 0;
+   int64_t     stride() const { return ld ? ld : k; }
+};
+struct MutableMatrix {
+   void*   data;
+   Type    type;
+   int64_t rows, k, ld = 0;
+   int64_t stride() const { return ld ? ld : k; }
+};
+
+inline int quantize(const Matrix& x, Blocks along, Blocks across = {}, void* stream = nullptr, Rule rule = Rule::Fit,
+                    const uint8_t* rand = nullptr)
+{
+   return fufft_mx4_quantize(x.data, (int)x.type, x.stride(), x.rows, x.k, (int)rule, rand, along.codes, along.scales,
+                             across.codes, across.scales, stream);
+}
+inline int dequantize(Blocks b, const MutableMatrix& out, void* stream = nullptr)
+{
+   return fufft_mx4_dequantize(b.codes, b.scales, out.data, (int)out.type, out.stride(), out.rows, out.k, stream);
+}
+// out (m x n) = a b^T + bias, a m rows and b n rows of k values
+inline int matmul(Blocks a, Blocks b, const MutableMatrix& out, int64_t k, void* stream = nullptr,
+                  const float* bias = nullptr)
+{
+   return fufft_mx4_matmul(a.codes, a.scales, b.codes, b.scales, bias, out.data, (int)out.type, out.stride(), out.rows,
+                           out.k, k, stream);
+}
+inline int linear(const Matrix& x, Blocks w, const MutableMatrix& out, void* stream = nullptr,
+                  const float* bias = nullptr)
+{
+   if(x.rows != out.rows) return FUFFT_ERR_INVALID;
+   return fufft_mx4_linear(x.data, (int)x.type, x.stride(), w.codes, w.scales, bias, out.data, (int)out.type,
+                           out.stride(), out.rows, out.k, x.k, stream);
+}
+
+// a paged cache and the sequences in it
+struct Cache {
+   Blocks         blocks;
+   int64_t        pages, page, channels;
+   const int32_t* table;        // batch x width
+   int64_t        width;
+   const int32_t* lens;         // batch
+   int64_t        batch;
+};
+inline int write(const Cache& c, const Matrix& x, const int64_t* slots, void* stream = nullptr)
+{
+   if(x.k != c.channels) return FUFFT_ERR_INVALID;
+   return fufft_mx4_cache_write(x.data, (int)x.type, x.stride(), slots, x.rows, c.channels, c.blocks.codes,
+                                c.blocks.scales, c.pages * c.page, stream);
+}
+inline int read(const Cache& c, void* out, Type type, int64_t length, void* stream = nullptr,
+                Order order = Order::Tokens)
+{
+   return fufft_mx4_cache_read(c.blocks.codes, c.blocks.scales, c.pages, c.page, c.channels, c.table, c.width, c.lens,
+                               c.batch, length, out, (int)type, (int)order, stream);
+}
+// taps: tap_count x channels; work: splits x batch x channels floats, or none for fp32 results
+inline int conv(const Cache& c, const void* taps, Type tap_type, int64_t tap_count, void* out, Type type,
+                void* stream = nullptr, float* work = nullptr, int64_t splits = 0)
+{
+   return fufft_mx4_cache_conv(c.blocks.codes, c.blocks.scales, c.pages, c.page, c.channels, c.table, c.width, c.lens,
+                               c.batch, taps, (int)tap_type, tap_count, out, (int)type, work, splits, stream);
+}
+
+}  // namespace mx4
+
 // ---- the reference's launch surface, by name --------------------------------------------
 // A caller of the reference instantiates a kernel template whose parameters
 // spell out the plan and launches it, e.g. (bench_fufft.cu:216-221)

@@ -16,7 +16,7 @@ def scale_of(top, rule):
     if top == 0:
         return 0
     if rule == "fit":
-        e = -127
+        e = max(-127, int(np.floor(np.log2(top))) - 5)      # below every power that holds top
         while top > 6 * 2.0 ** e:
             e += 1
     else:

@@ -170,7 +170,10 @@ def random_blocks(rng, rows, k, spread=6):
 
 MATMULS = [(1, 1, 1), (1, 17, 32), (2, 5, 127), (16, 16, 128), (17, 33, 129), (33, 40, 384), (64, 64, 256),
            (65, 100, 1000), (5, 1000, 4096), (130, 257, 520), (128, 128, 2048), (256, 256, 512), (300, 513, 2176),
-           (129, 640, 1100), (513, 300, 96), (1000, 999, 200), (1, 4096, 640), (2048, 2048, 256)]
+           (129, 640, 1100), (513, 300, 96), (1000, 999, 200), (1, 4096, 640), (2048, 2048, 256),
+           # each kernel and tile, with K ending in half a slab and beyond the scales of one fetch
+           (7, 5000, 300), (20, 1000, 4200), (32, 4090, 2176), (64, 4090, 2100), (700, 1000, 2500), (2048, 2000, 4700),
+           (4096, 4096, 300), (4090, 3900, 2176)]
 
 
 @pytest.mark.parametrize("m,n,k", MATMULS)
@@ -271,7 +274,8 @@ def test_layer_gradients(dev, rng, kind, m, n, k):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 300, 1000), (2, 64, 128), (7, 33, 4100), (15, 16, 129), (16, 100, 256),
-                                   (17, 129, 640), (33, 50, 96), (64, 64, 1024), (65, 70, 300), (200, 48, 257)])
+                                   (17, 129, 640), (33, 50, 96), (64, 64, 1024), (65, 70, 300), (200, 48, 257),
+                                   (1, 4200, 700), (20, 4200, 300), (40, 4200, 1100)])
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("out", TYPES)
 def test_linear(dev, rng, m, n, k, kind, out):

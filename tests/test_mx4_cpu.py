@@ -1,5 +1,9 @@
 """CPU tests of the microscaled 4-bit calls: what the C ABI and the Python binding refuse
 before anything is launched, and the 64-bit form that the GPU tests compare with."""
+import shutil
+import subprocess
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -199,3 +203,15 @@ def test_reference_definition(rule):
                 near = min(R.GRID, key=lambda g: abs(abs(v[i]) - g * p)) * p
                 assert abs(abs(back[r, 32 * b + i]) - near) == 0 or \
                     abs(abs(abs(v[i]) - near) - abs(abs(v[i]) - abs(back[r, 32 * b + i]))) < 1e-12 * p
+
+
+def test_cpp_header(tmp_path):
+    """The 4-bit part of include/fufft/fufft.hpp: built with g++ and run without a GPU."""
+    if shutil.which("g++") is None:
+        pytest.skip("g++ not available")
+    root = Path(__file__).resolve().parent.parent
+    exe, lib = tmp_path / "mx4_hpp_check", root / "fufft_amd"
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Wextra", "-Werror", f"-I{root / 'include'}",
+                    str(root / "tests" / "cpp" / "mx4_hpp_check.cpp"), f"-L{lib}", "-lfufft_amd", f"-Wl,-rpath,{lib}",
+                    "-o", str(exe)], check=True)
+    assert subprocess.run([str(exe)], timeout=60).returncode == 0
