@@ -136,6 +136,11 @@ def _load() -> C.CDLL:
 
 
 lib = _load()
+if torch is not None:
+    if not _LIB_PATH.with_name("_binding.so").exists():
+        raise FileNotFoundError(f"{_LIB_PATH.with_name('_binding.so')} is missing: build it with "
+                                "`python fufft_amd/build.py`")
+    from . import _binding  # noqa: E402
 
 
 def check(status: int, where: str) -> None:
@@ -158,7 +163,6 @@ if torch is not None:
     }
     # element types of the mx4 calls (FUFFT_F32, FUFFT_BF16, FUFFT_F16)
     _ELEMENT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    _BYTE = torch.uint8
     # the reads every launch makes, without torch.cuda's Python layer (which
     # initialises the GPU on first use: a tensor that is on one has done that)
     _TENSOR = torch.Tensor
@@ -737,17 +741,21 @@ def _name(table: dict, key, name: str) -> int:
     return table[key]
 
 
-# These calls are short (a few rows take the GPU 2 to 4 us), so their arguments are read as
-# _ptrs reads its own: the case that passes in the cheapest reads of each property, any
-# other through the checks that say what is wrong.  (48 rows of 4096 made 4-bit, host time a
-# call: 7.3 us with _ptrs and a check of x's device by name, 5.5 so, 3.2 of them the launch.)
+# Each call goes to the native binding first, which checks every argument and launches.  What it
+# does not take (it answers None) goes through the checks here, which say what is wrong; a
+# tensor subclass, which it does not take either, passes them and is launched from here.
+
+def _native(x) -> bool:
+    return type(x) is _TENSOR and x.is_cuda
+
+
+def _handle(stream, gpu: int) -> int:
+    return _current_raw_stream(gpu) if stream is None else _stream(stream)
+
 
 def _matrix(x, name: str):
     """(type, leading dimension, rows, columns) of a 2D tensor of elements, checked but for
     its device (the last check, _on_gpu)."""
-    if type(x) is _TENSOR and x.dtype in _ELEMENT and x.dim() == 2 and x.is_contiguous():
-        rows, k = x.shape
-        return _ELEMENT[x.dtype], k, rows, k
     if torch is None or not isinstance(x, torch.Tensor):
         raise TypeError(f"{name}: expected a torch tensor in GPU memory, got {type(x).__name__}")
     kind = _ELEMENT.get(x.dtype)
@@ -767,34 +775,21 @@ def _matrix(x, name: str):
 
 def _on_gpu(*pairs) -> None:
     """Every tensor (None: an argument that is not given) is on the current GPU."""
-    gpu = None
     for x, name in pairs:
-        if x is None:
-            continue
-        if x.is_cuda:
-            if gpu is None:
-                gpu = _current_device()
-            if x.get_device() == gpu:
-                continue
-        _check_device(x, name)
+        if x is not None:
+            _check_device(x, name)
 
 
 def _array(x, name: str, nbytes: int, kind: str) -> int:
     """The address of a contiguous array of at least nbytes, checked but for its device."""
-    if not (type(x) is _TENSOR and x.dtype in _DT[kind] and x.is_contiguous() and x.nbytes >= nbytes):
-        _check_shape(x, name, nbytes, kind)
+    _check_shape(x, name, nbytes, kind)
     return x.data_ptr()
 
 
 def _blocks(codes, scales, name: str, rows: int, k: int):
     """The addresses of `rows` rows of k values in blocks, checked but for their device."""
     groups = (k + 127) // 128
-    if not (type(codes) is _TENSOR and type(scales) is _TENSOR and codes.dtype is _BYTE and scales.dtype is _BYTE
-            and codes.is_contiguous() and scales.is_contiguous() and codes.nbytes >= rows * groups * 64
-            and scales.nbytes >= rows * groups * 4):
-        _check_shape(codes, name, rows * groups * 64, "bytes")
-        _check_shape(scales, name + "_scales", rows * groups * 4, "bytes")
-    return codes.data_ptr(), scales.data_ptr()
+    return (_array(codes, name, rows * groups * 64, "bytes"), _array(scales, name + "_scales", rows * groups * 4, "bytes"))
 
 
 def _bias(bias, n: int):
@@ -808,6 +803,11 @@ def mx4_quantize(x, codes=None, scales=None, codes_t=None, scales_t=None, *, ran
     not wanted is None.  rand: a uint8 for each value of x, contiguous, for rounding up or
     down at random; None rounds to the nearest.  rule: "fit" (nothing saturates) or "floor"."""
     rule = _name(MX4_RULE, rule, "rule")
+    if _native(x):
+        gpu = _current_device()
+        status = _binding.quantize(x, codes, scales, codes_t, scales_t, rand, rule, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_mx4_quantize")
     kind, ld, rows, k = _matrix(x, "x")
     pc = ps = qc = qs = pr = None
     if codes is not None or scales is not None:
@@ -826,6 +826,11 @@ def mx4_quantize(x, codes=None, scales=None, codes_t=None, scales_t=None, *, ran
 
 def mx4_dequantize(codes, scales, out, stream=None) -> None:
     """The values that blocks along rows stand for, into out (rows, k)."""
+    if _native(out):
+        gpu = _current_device()
+        status = _binding.dequantize(codes, scales, out, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_mx4_dequantize")
     kind, ld, rows, k = _matrix(out, "out")
     pc, ps = _blocks(codes, scales, "codes", rows, k)
     _on_gpu((out, "out"), (codes, "codes"), (scales, "codes_scales"))
@@ -837,6 +842,11 @@ def mx4_matmul(a, a_scales, b, b_scales, out, k: int, bias=None, stream=None) ->
     """out (m, n) = a b^T + bias: a is m rows of k values in blocks, b n rows, bias fp32.
     For y = x w^T the gradients are dx = mx4_matmul(dy, w's columns) and dw = mx4_matmul(dy's
     columns, x's columns), all from mx4_quantize."""
+    if _native(out):
+        gpu = _current_device()
+        status = _binding.matmul(a, a_scales, b, b_scales, out, k, bias, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_mx4_matmul")
     kind, ld, m, n = _matrix(out, "out")
     pa, pas = _blocks(a, a_scales, "a", m, k)
     pb, pbs = _blocks(b, b_scales, "b", n, k)
@@ -849,6 +859,11 @@ def mx4_matmul(a, a_scales, b, b_scales, out, k: int, bias=None, stream=None) ->
 def mx4_linear(x, w, w_scales, out, bias=None, stream=None) -> None:
     """out (m, n) = x w^T + bias with x (m, k) as it is and w n rows of k values in blocks:
     the form for single tokens."""
+    if _native(x):
+        gpu = _current_device()
+        status = _binding.linear(x, w, w_scales, out, bias, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_mx4_linear")
     x_kind, ldx, m, k = _matrix(x, "x")
     kind, ld, rows, n = _matrix(out, "out")
     if rows != m:
@@ -890,6 +905,11 @@ def _table(table, lens):
 def mx4_cache_write(x, slots, codes, scales, stream=None) -> None:
     """Rows of x (tokens, channels) into the slots (int64, page * page_size + offset, all
     different) of a cache; a slot outside it, such as -1, is skipped."""
+    if _native(x):
+        gpu = _current_device()
+        status = _binding.cache_write(x, slots, codes, scales, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_mx4_cache_write")
     kind, ld, rows, channels = _matrix(x, "x")
     pages, page = _cache(codes, scales, channels)
     pl = _array(slots, "slots", 8 * rows, "slots")
@@ -904,6 +924,11 @@ def mx4_cache_read(codes, scales, pages, lens, out, order: str = "tokens", strea
     from its length on: out (batch, length, channels), or with order "channels" (batch,
     channels, length), the signals that the convolutions take."""
     turned = _name(MX4_ORDER, order, "order")
+    if _native(out):
+        gpu = _current_device()
+        status = _binding.cache_read(codes, scales, pages, lens, out, turned, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_mx4_cache_read")
     if torch is None or not isinstance(out, torch.Tensor):
         raise TypeError(f"out: expected a torch tensor in GPU memory, got {type(out).__name__}")
     if out.dtype not in _ELEMENT:
@@ -929,6 +954,11 @@ def mx4_cache_conv(codes, scales, pages, lens, taps, out, work=None, stream=None
     """out (batch, channels) = the causal convolution with taps (count, channels) at every
     sequence's last token, read from the cache.  work: fp32 (splits, batch, channels); the
     taps are split over at most that many workgroups.  None is allowed for fp32 results."""
+    if _native(out):
+        gpu = _current_device()
+        status = _binding.cache_conv(codes, scales, pages, lens, taps, out, work, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_mx4_cache_conv")
     t_kind, t_ld, tap_count, channels = _matrix(taps, "taps")
     kind, ld, batch, out_channels = _matrix(out, "out")
     if out_channels != channels:

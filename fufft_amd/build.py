@@ -1,4 +1,5 @@
-"""Build the gfx950 library (fufft_amd/libfufft_amd.so) and the CPU oracle.
+"""Build the gfx950 library (fufft_amd/libfufft_amd.so), the native part of the
+Python binding (fufft_amd/_binding.so) and the CPU oracle.
 
 Everything is compiled in-tree so the shared objects travel with the source
 tree to the GPU box.  hipcc cross-compiles for gfx950 without a GPU.
@@ -64,6 +65,27 @@ def build_library(jobs: int = 8) -> Path:
     return LIB
 
 
+def build_binding() -> Path:
+    """The native part of the Python binding (fufft_amd/_binding.so): host code only, against
+    the installed torch and linked to the library beside it."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    out = PKG / "_binding.so"
+    tmp = out.with_suffix(".so.tmp")
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"]]
+    lib = Path(torch.__file__).resolve().parent / "lib"
+    _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          *[a for i in includes for a in ("-isystem", i)], str(CSRC / "binding.cpp"),
+          f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", f"-L{PKG}", "-lfufft_amd", "-Wl,-rpath,$ORIGIN",
+          "-o", str(tmp)])
+    os.replace(tmp, out)
+    return out
+
+
 def build_cpp_checks() -> Path:
     """The C++ caller test (tests/cpp/abi_gpu_check.cpp): host code only,
     linked against this library and the HIP runtime; run on a GPU by
@@ -89,6 +111,7 @@ def build_oracle() -> None:
 def build(jobs: int = 8) -> None:
     build_oracle()
     build_library(jobs)
+    build_binding()
     if shutil.which("g++"):
         build_cpp_checks()
 

@@ -362,3 +362,46 @@ def test_calls_on_another_stream_and_captured(dev, rng):
         torch.cuda.synchronize()
         assert torch.equal(out, got[0]) and torch.equal(lin, got[1])
         torch.randn(1000, device=dev).sum().item()
+
+
+def test_refusals_on_the_gpu(dev):
+    """What the native binding does not take, the checks in Python name: a short array, another
+    type, rows that overlap, a tensor of the host; a tensor subclass and a parameter pass."""
+    import torch
+    import fufft_amd as ff
+    x, (c, s) = torch.randn(6, 300, device=dev), ff.mx4_empty(6, 300)
+    out = torch.empty(6, 6, device=dev)
+    cache, lens = (torch.zeros(4, 16, 192, dtype=torch.uint8, device=dev), torch.zeros(4, 16, 12, dtype=torch.uint8, device=dev)), \
+        torch.zeros(2, dtype=torch.int32, device=dev)
+    table = torch.zeros(2, 2, dtype=torch.int32, device=dev)
+    for call, message in (
+            (lambda: ff.mx4_quantize(x, c[:5].contiguous(), s), "codes: holds"),
+            (lambda: ff.mx4_quantize(x, c, s, rand=torch.zeros(6, 299, dtype=torch.uint8, device=dev)), "rand: holds"),
+            (lambda: ff.mx4_quantize(x.double(), c, s), "x: dtype"),
+            (lambda: ff.mx4_quantize(x[:1].expand(6, 300), c, s), "rows overlap"),
+            (lambda: ff.mx4_quantize(x, c.cpu(), s), "codes: tensor is on cpu"),
+            (lambda: ff.mx4_quantize(x), "neither"),
+            (lambda: ff.mx4_dequantize(c, s[:, :8].contiguous(), x), "codes_scales: holds"),
+            (lambda: ff.mx4_matmul(c, s, c, s, torch.empty(6, 7, device=dev), 300), "b: holds"),
+            (lambda: ff.mx4_matmul(c, s, c, s, out, 300, bias=torch.zeros(6, device=dev).half()), "bias: dtype"),
+            (lambda: ff.mx4_linear(x, c, s, out[:5]), "out: 5 rows"),
+            (lambda: ff.mx4_cache_write(x, torch.zeros(6, dtype=torch.int32, device=dev), *cache), "slots: dtype"),
+            (lambda: ff.mx4_cache_read(*cache, table.long(), lens, torch.empty(2, 9, 300, device=dev)), "pages: dtype"),
+            (lambda: ff.mx4_cache_conv(*cache, table, lens, x, torch.empty(2, 300, device=dev).half()), "workspace"),
+            (lambda: ff.mx4_cache_conv(*cache, table, lens, x, torch.empty(3, 300, device=dev)), "3 sequences")):
+        with pytest.raises(ValueError, match=message):
+            call()
+    for bad in (c.view(torch.int8), s):                       # refused by the library itself: x's own bytes as codes
+        with pytest.raises((ff.FufftError, ValueError)):
+            ff.mx4_quantize(x, x.view(torch.uint8).view(-1), s) if bad is s else ff.mx4_quantize(x, bad, s)
+    ff.mx4_quantize(x, c, s)
+    want = c.clone()
+
+    class Sub(torch.Tensor):
+        pass
+
+    for t in (torch.nn.Parameter(x), x.as_subclass(Sub)):
+        c.zero_()
+        ff.mx4_quantize(t, c, s)
+        torch.cuda.synchronize()
+        assert torch.equal(c, want)
