@@ -119,6 +119,22 @@ quantize_rows(QuantizeParams p, int64_t kp, int lr)
    }
 }
 
+// eight 16-bit elements without the first n (1 .. 7), zeros behind
+template<class T>
+__device__ inline Eight<T> drop_first(const Eight<T>& v, int n)
+{
+   struct Halves { uint64_t lo, hi; } h = __builtin_bit_cast(Halves, v);
+   const int bits = 16 * n;
+   if(bits >= 64) {
+      h.lo = h.hi >> (bits - 64);
+      h.hi = 0;
+   } else {
+      h.lo = (h.lo >> bits) | (h.hi << (64 - bits));
+      h.hi >>= bits;
+   }
+   return __builtin_bit_cast(Eight<T>, h);
+}
+
 // Blocks along columns, and along rows too where p.codes is given, from one
 // reading: a workgroup takes 128 rows x 128 columns, a lane 8 values of 8 rows.  The
 // values (and random bytes) wait in LDS in their own type, and each lane takes two
@@ -142,22 +158,34 @@ quantize_both(QuantizeParams p, int64_t kp, int64_t rowsp)
    const int64_t col = c0 + lane * 8;
    Eight<T> v[8];
    u32x2 r[8];
-   if(p.k % 8 == 0 || c0 + 128 <= p.k) {
+   if(p.k % 8 == 0 || c0 + 128 <= p.k || (sizeof(T) == 2 && p.k >= 8)) {
       // whole pieces of eight: all loads ahead, beyond the matrix from its last row or piece
-      // (777 x 520, fp16 with random bytes: 13.6 us with a branch around each piece, 8.4 so)
-      const int64_t c = col < p.k ? col : p.k - 8;
+      // (777 x 520, fp16 with random bytes: 13.6 us with a branch around each piece, 8.4 so).
+      // A piece that the last column cuts is the row's last eight values, the earlier
+      // ones shifted out.
+      const int64_t c = col + 8 <= p.k ? col : p.k - 8;
+      const int drop = col < p.k ? (int)(col - c) : 0;
 #pragma unroll
       for(int u = 0; u < 8; u++) {
          const int64_t row = r0 + u * 16 + first, at = row < p.rows ? row : p.rows - 1;
          v[u] = *reinterpret_cast<const Eight<T>*>(x + at * p.ld + c);
+         r[u] = u32x2{0, 0};
          if constexpr(RAND) {
             const Bytes8 t = *reinterpret_cast<const Bytes8*>(p.rand + at * p.k + c);
             r[u] = u32x2{t.e[0], t.e[1]};
          }
       }
 #pragma unroll
-      for(int u = 0; u < 8; u++)
+      for(int u = 0; u < 8; u++) {
+         if constexpr(sizeof(T) == 2) {
+            if(drop) {
+               v[u] = drop_first(v[u], drop);
+               const uint64_t b = (((uint64_t)r[u][1] << 32) | r[u][0]) >> (8 * drop);
+               r[u] = u32x2{(uint32_t)b, (uint32_t)(b >> 32)};
+            }
+         }
          if(r0 + u * 16 + first >= p.rows || col >= p.k) v[u] = {};
+      }
    } else {
 #pragma unroll
       for(int u = 0; u < 8; u++) {

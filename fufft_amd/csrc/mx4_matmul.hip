@@ -266,15 +266,36 @@ linear_rows(MatmulParams p, int groups, int waves)
                group(i, v);
             }
          } else {
+            // the last run: whole groups as above, then what is left of x in pieces of eight, beyond
+            // its end the last piece again, made zero; single values where K cuts one
 #pragma unroll
             for(int i = 0; i < kRun; i++) {
                const int64_t k = (first + i) * 128;
                if(k >= p.k) break;
                Block v[MT];
+               if(k + 128 <= p.k) {
 #pragma unroll
-               for(int a = 0; a < MT; a++)
+                  for(int a = 0; a < MT; a++) v[a] = *reinterpret_cast<const Block*>(x[a] + k);
+               } else {
+                  struct __attribute__((packed, aligned(sizeof(T)))) Eight { T e[8]; };
 #pragma unroll
-                  for(int e = 0; e < 32; e++) v[a].e[e / 8][e % 8] = k + k0 + e < p.k ? x[a][k + e] : (T)0.0f;
+                  for(int t = 0; t < 4; t++) {
+                     const int64_t at = k + k0 + t * 8;      // in the row; x[a] starts at k0
+#pragma unroll
+                     for(int a = 0; a < MT; a++) {
+                        const T* const row = x[a] - k0;
+                        Eight e;
+                        if(p.k % 8 == 0) {
+                           e = *reinterpret_cast<const Eight*>(row + (at < p.k ? at : p.k - 8));
+                        } else {
+#pragma unroll
+                           for(int j = 0; j < 8; j++) e.e[j] = row[at + j < p.k ? at + j : p.k - 1];
+                        }
+#pragma unroll
+                        for(int j = 0; j < 8; j++) v[a].e[t][j] = at + j < p.k ? e.e[j] : (T)0.0f;
+                     }
+                  }
+               }
                group(i, v);
             }
          }
@@ -591,8 +612,7 @@ hipError_t linear_typed(const MatmulParams& p, hipStream_t s)
    // 32 rows of w a workgroup share x's loads; 16 where 32 would leave CUs without one
    const bool wide = p.n > 16 * 256;
    if(p.m <= 16) return wide ? linear_shape<T, O, 1, 2, 2>(p, s) : linear_shape<T, O, 1, 1, 2>(p, s);
-   if(p.m <= 32) return wide ? linear_shape<T, O, 2, 2, 1>(p, s) : linear_shape<T, O, 2, 1, 1>(p, s);
-   return wide ? linear_shape<T, O, 4, 2, 1>(p, s) : linear_shape<T, O, 4, 1, 1>(p, s);
+   return wide ? linear_shape<T, O, 2, 2, 1>(p, s) : linear_shape<T, O, 2, 1, 1>(p, s);
 }
 
 template<class T>

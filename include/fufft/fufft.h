@@ -537,8 +537,8 @@ int fufft_mx4_matmul(const void* a, const uint8_t* a_scales, const void* b,
                      const uint8_t* b_scales, const float* bias, void* out, int type, int64_t ld,
                      int64_t m, int64_t n, int64_t k, void* stream);
 /* out[i][j] = bias[j] + sum over k of x[i][k] w[j][k] with x (x_type, leading
- * dimension ldx) as it is: the form for single tokens, which reads w once for up
- * to 64 rows.  (Many rows run faster quantized, through fufft_mx4_matmul.) */
+ * dimension ldx) as it is: the form for single tokens, which reads w once for every
+ * 32 rows.  (Many rows run faster quantized, through fufft_mx4_matmul.) */
 int fufft_mx4_linear(const void* x, int x_type, int64_t ldx, const void* w,
                      const uint8_t* w_scales, const float* bias, void* out, int type, int64_t ld,
                      int64_t m, int64_t n, int64_t k, void* stream);
