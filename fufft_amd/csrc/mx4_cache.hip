@@ -78,7 +78,8 @@ read_tokens(CacheParams c, T* out, int64_t length, int64_t cp, int lr)
 
 // out[b][channel][t], zeros from each sequence's length on: tiles of 64 tokens x
 // 128 channels turned in LDS, so that codes are read along channels and signals
-// written along tokens.
+// written along tokens.  4 x 8192 tokens x 2048 channels in fp32: 63 to 72 us, 268 MB written at
+// 3.7 to 4.3 TB/s.
 template<class T>
 __global__ void __launch_bounds__(kLanes)
 read_channels(CacheParams c, T* out, int64_t length, int64_t cp)

@@ -609,7 +609,10 @@ hipError_t linear_shape(const MatmulParams& p, hipStream_t s)
 template<class T, class O>
 hipError_t linear_typed(const MatmulParams& p, hipStream_t s)
 {
-   // 32 rows of w a workgroup share x's loads; 16 where 32 would leave CUs without one
+   // 32 rows of w a workgroup share x's loads; 16 where 32 would leave CUs without one (us, 16 / 32
+   // rows: 1 x 8192 x 8192 11.6 / 10.8, 13 x 5000 x 2056 5.4 / 4.7, 16 x 16384 x 16384 84 / 58, but 1 x
+   // 4096 x 4096 4.1 / 5.7).  Beyond 32 rows of x, more workgroups: 64 rows in one took as long (64 x
+   // 8192 x 8192 41 / 43, 64 x 4096 x 4096 19.9 / 19.4) and 48 x 208 x 113 8.5 / 5.8.
    const bool wide = p.n > 16 * 256;
    if(p.m <= 16) return wide ? linear_shape<T, O, 1, 2, 2>(p, s) : linear_shape<T, O, 1, 1, 2>(p, s);
    return wide ? linear_shape<T, O, 2, 2, 1>(p, s) : linear_shape<T, O, 2, 1, 1>(p, s);
