@@ -41,7 +41,7 @@ __device__ inline u32x2 load_rand8(const uint8_t* rand, int64_t row, int64_t col
 }
 
 template<class T, bool RAND>
-__device__ inline uint32_t encode(const float (&v)[8], uint32_t s, u32x2 r)
+__device__ inline uint32_t encode(const float (&v)[8], uint32_t s, const uint32_t (&r)[8])
 {
    if constexpr(RAND) return encode8_random<sizeof(T) == 2>(v, s, r);
    else               return encode8(v, s);
@@ -64,7 +64,10 @@ __device__ inline void encode_row8(const Eight<T>& x, u32x2 r, bool fit, uint32_
    const uint32_t s = scale_byte(top, fit);
    *word = s | (dpp<kRowLeft4>(s) << 8);
    *word |= dpp<kRowLeft8>(*word) << 16;
-   *codes = encode<T, RAND>(v, s, r);
+   uint32_t b[8];
+#pragma unroll
+   for(int i = 0; i < 8; i++) b[i] = (r[i / 4] >> (8 * (i % 4))) & 255u;
+   *codes = encode<T, RAND>(v, s, b);
 }
 
 // Blocks along rows: 16 lanes a group of 128 values.  A workgroup has 2^lr lanes to a
@@ -149,7 +152,7 @@ __global__ void __launch_bounds__(kLanes)
 quantize_both(QuantizeParams p, int64_t kp, int64_t rowsp)
 {
    __shared__ alignas(16) Pair<T> tile[128 * 64];
-   __shared__ alignas(16) Pair<uint8_t> rtile[RAND ? 128 * 64 : 8];
+   __shared__ alignas(16) uint16_t rtile[RAND ? 128 * 64 : 8];
    const T* x = static_cast<const T*>(p.x);
    const int64_t c0 = (int64_t)blockIdx.x * 128;
    const int64_t r0 = ((int64_t)blockIdx.y + (int64_t)blockIdx.z * gridDim.y) * 128;
@@ -222,7 +225,7 @@ quantize_both(QuantizeParams p, int64_t kp, int64_t rowsp)
    const int blk = threadIdx.x & 3, pair = threadIdx.x >> 2;
    const int base = blk * 32 * 64 + (pair ^ (blk << 4));
    Pair<T> t[32];
-   Pair<uint8_t> b[32];
+   uint32_t b[RAND ? 32 : 1] = {};                    // the random bytes of both columns
    uint32_t top[2] = {0, 0};
 #pragma unroll
    for(int i = 0; i < 32; i++) {
@@ -240,11 +243,11 @@ quantize_both(QuantizeParams p, int64_t kp, int64_t rowsp)
 #pragma unroll
       for(int q = 0; q < 4; q++) {
          float w[8];
-         u32x2 rr = {0, 0};
+         uint32_t rr[8];
 #pragma unroll
          for(int i = 0; i < 8; i++) {
             w[i] = to_float(h ? t[q * 8 + i].b : t[q * 8 + i].a);
-            if constexpr(RAND) rr[i / 4] |= (uint32_t)(h ? b[q * 8 + i].b : b[q * 8 + i].a) << (8 * (i % 4));
+            rr[i] = (b[RAND ? q * 8 + i : 0] >> (8 * h)) & 255u;
          }
          c[q] = encode<T, RAND>(w, s, rr);
       }

@@ -120,9 +120,9 @@ __device__ inline float dithered(float v, float inverse, float r)
    return __uint_as_float((__float_as_uint(v) & 0x80000000u) | __float_as_uint(c));
 }
 
-// eight values with their random bytes, two words of four; 16 bits: the values are of a 16-bit type
+// eight values with their random bytes; 16 bits: the values are of a 16-bit type
 template<bool BITS16>
-__device__ inline uint32_t encode8_random(const float (&v)[8], uint32_t s, u32x2 r)
+__device__ inline uint32_t encode8_random(const float (&v)[8], uint32_t s, const uint32_t (&r)[8])
 {
    if(s == 255u) return 0u;
    const float inverse = __uint_as_float((254u - s) << 23);   // 2^(127 - s); s <= 253 here
@@ -130,14 +130,14 @@ __device__ inline uint32_t encode8_random(const float (&v)[8], uint32_t s, u32x2
    if constexpr(BITS16) {
       float d[8];
 #pragma unroll
-      for(int i = 0; i < 8; i++) d[i] = dithered(v[i], inverse, (float)((r[i / 4] >> (8 * (i % 4))) & 255u));
+      for(int i = 0; i < 8; i++) d[i] = dithered(v[i], inverse, (float)r[i]);
       c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, d[0], d[1], 1.0f, 0);
       c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, d[2], d[3], 1.0f, 1);
       c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, d[4], d[5], 1.0f, 2);
       c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, d[6], d[7], 1.0f, 3);
    } else {
 #pragma unroll
-      for(int i = 0; i < 8; i++) c |= encode_random(v[i], inverse, (r[i / 4] >> (8 * (i % 4))) & 255u) << (4 * i);
+      for(int i = 0; i < 8; i++) c |= encode_random(v[i], inverse, r[i]) << (4 * i);
    }
    return c;
 }

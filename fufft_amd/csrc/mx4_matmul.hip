@@ -199,7 +199,9 @@ __device__ inline bf16x8 decode8_bf16(uint32_t c, float p)
 }
 
 // The block that a lane reads holds its 8 values of each of four products, so
-// product t takes values 8 t .. 8 t + 7 of the four blocks of a group.
+// product t takes values 8 t .. 8 t + 7 of the four blocks of a group.  (Blocks turned among
+// a row's four lanes, so that those read 64 bytes of x in a row: 1 x 8192 x 8192 10.9 / 11.1 us,
+// 64 x 8192 x 8192 in bf16 43 / 42, in fp32 89 / 75.)
 template<class T, class O, int MT, int NT, int DEPTH>
 __global__ void __launch_bounds__(64 * most_waves(MT * NT))
 linear_rows(MatmulParams p, int groups, int waves)
