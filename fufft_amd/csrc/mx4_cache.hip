@@ -151,6 +151,18 @@ __device__ inline void decode(uint32_t c, uint32_t s, float (&v)[CH])
    }
 }
 
+// a row's CH taps without the first `drop` of them, which are another lane's
+template<class T, int CH>
+__device__ inline void drop_first(T (&e)[CH], int drop)
+{
+#pragma unroll
+   for(int by = CH / 2; by > 0; by /= 2) {
+      const bool go = (drop & by) != 0;
+#pragma unroll
+      for(int i = 0; i < CH; i++) e[i] = go ? (i + by < CH ? e[i + by] : (T)0.0f) : e[i];
+   }
+}
+
 template<class T, int CH, int SEQS, int TAPS, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES)
 cache_conv(CacheParams c, const T* taps, uint32_t tap_count, uint32_t chunk, uint32_t cp, uint32_t slices, uint32_t parts,
@@ -178,24 +190,27 @@ cache_conv(CacheParams c, const T* taps, uint32_t tap_count, uint32_t chunk, uin
    const uint32_t pages = c.pages < 0x7fffffff ? (uint32_t)c.pages : 0x7fffffffu, page_mask = (1u << c.page_log) - 1;
    float acc[SEQS][CH] = {};
    // Every load of a step has an address that is good, so that all go out before the first
-   // is used: taps past the end are the last one, channels past the end the last one,
+   // is used: taps past the end are the last one, channels past the end the last ones,
    // a token that is none is row 0 (n > 0 somewhere, so there is a page and a table).
-   auto steps = [&](auto inside) {
-      constexpr bool INSIDE = decltype(inside)::value;
-      uint32_t ch[CH];
-#pragma unroll
-      for(int i = 0; i < CH; i++) ch[i] = col + i < c.channels ? col + i : (uint32_t)c.channels - 1;
+   // A lane that the last channel cuts (CUT) reads the row's last CH taps and drops the
+   // first; fewer channels than that (FEW) are read one by one.  The three are code of their own:
+   // a branch at each load would end in a wait for it (51 x 4144 x 2044, fp32 taps: 250 us, 85 so).
+   enum { INSIDE, CUT, FEW };
+   auto steps = [&](auto mode) {
+      constexpr int MODE = decltype(mode)::value;
+      const uint32_t channels = (uint32_t)c.channels, at = MODE == CUT && col + CH > channels ? channels - CH : col;
+      const int drop = MODE == CUT && col < channels ? (int)(col - at) : 0;
       const uint32_t code_at = (col < cp ? col : 0) / 2, scale_at = (col < cp ? col : 0) / kBlock;
       for(uint32_t j0 = split * chunk + wave * TAPS; j0 < j_end; j0 += WAVES * TAPS) {
          Taps h[TAPS];
 #pragma unroll
          for(int u = 0; u < TAPS; u++) {
             const T* row = taps + (int64_t)(j0 + u < j_end ? j0 + u : j_end - 1) * c.channels;
-            if constexpr(INSIDE) {
-               h[u] = *reinterpret_cast<const Taps*>(row + col);
+            if constexpr(MODE != FEW) {
+               h[u] = *reinterpret_cast<const Taps*>(row + at);
             } else {
 #pragma unroll
-               for(int i = 0; i < CH; i++) h[u].e[i] = row[ch[i]];
+               for(int i = 0; i < CH; i++) h[u].e[i] = row[i < (int)channels ? i : (int)channels - 1];
             }
          }
          uint32_t q[SEQS][TAPS], s[SEQS][TAPS];
@@ -214,6 +229,10 @@ cache_conv(CacheParams c, const T* taps, uint32_t tap_count, uint32_t chunk, uin
                s[g][u] = (c.scales + (from >> 4))[scale_at];
             }
          }
+         if constexpr(MODE == CUT) {
+#pragma unroll
+            for(int u = 0; u < TAPS; u++) drop_first<T, CH>(h[u].e, drop);
+         }
 #pragma unroll
          for(int g = 0; g < SEQS; g++)
 #pragma unroll
@@ -226,8 +245,9 @@ cache_conv(CacheParams c, const T* taps, uint32_t tap_count, uint32_t chunk, uin
             }
       }
    };
-   if(col - lane * CH + 64 * CH <= c.channels) steps(std::true_type());
-   else                                        steps(std::false_type());
+   if(col - lane * CH + 64 * CH <= c.channels) steps(std::integral_constant<int, INSIDE>());
+   else if(c.channels >= CH)                   steps(std::integral_constant<int, CUT>());
+   else                                        steps(std::integral_constant<int, FEW>());
 #pragma unroll
    for(int g = 0; g < SEQS; g++) {
       if(b0 + g >= c.batch) break;
