@@ -163,7 +163,7 @@ __device__ inline void drop_first(T (&e)[CH], int drop)
    }
 }
 
-template<class T, int CH, int SEQS, int TAPS, int WAVES>
+template<class T, int CH, int SEQS, int TAPS, int WAVES, bool FEW>
 __global__ void __launch_bounds__(64 * WAVES)
 cache_conv(CacheParams c, const T* taps, uint32_t tap_count, uint32_t chunk, uint32_t cp, uint32_t slices, uint32_t parts,
            uint32_t seq_groups, float* sums)
@@ -192,25 +192,24 @@ cache_conv(CacheParams c, const T* taps, uint32_t tap_count, uint32_t chunk, uin
    // Every load of a step has an address that is good, so that all go out before the first
    // is used: taps past the end are the last one, channels past the end the last ones,
    // a token that is none is row 0 (n > 0 somewhere, so there is a page and a table).
-   // A lane that the last channel cuts (CUT) reads the row's last CH taps and drops the
-   // first; fewer channels than that (FEW) are read one by one.  The three are code of their own:
-   // a branch at each load would end in a wait for it (51 x 4144 x 2044, fp32 taps: 250 us, 85 so).
-   enum { INSIDE, CUT, FEW };
-   auto steps = [&](auto mode) {
-      constexpr int MODE = decltype(mode)::value;
-      const uint32_t channels = (uint32_t)c.channels, at = MODE == CUT && col + CH > channels ? channels - CH : col;
-      const int drop = MODE == CUT && col < channels ? (int)(col - at) : 0;
+   // A lane that the last channel cuts reads the row's last CH taps and drops the first; a
+   // kernel for fewer channels than that (FEW) reads them one by one.  Each is code of its own: a
+   // branch at each load would end in a wait for it (51 x 4144 x 2044, fp32 taps: 250 us, 85 so).
+   auto steps = [&](auto cut) {
+      constexpr bool CUT = decltype(cut)::value;
+      const uint32_t channels = (uint32_t)c.channels, at = CUT && col + CH > channels ? channels - CH : col;
+      const int drop = CUT && col < channels ? (int)(col - at) : 0;
       const uint32_t code_at = (col < cp ? col : 0) / 2, scale_at = (col < cp ? col : 0) / kBlock;
       for(uint32_t j0 = split * chunk + wave * TAPS; j0 < j_end; j0 += WAVES * TAPS) {
          Taps h[TAPS];
 #pragma unroll
          for(int u = 0; u < TAPS; u++) {
             const T* row = taps + (int64_t)(j0 + u < j_end ? j0 + u : j_end - 1) * c.channels;
-            if constexpr(MODE != FEW) {
-               h[u] = *reinterpret_cast<const Taps*>(row + at);
-            } else {
+            if constexpr(FEW) {
 #pragma unroll
-               for(int i = 0; i < CH; i++) h[u].e[i] = row[i < (int)channels ? i : (int)channels - 1];
+               for(int i = 0; i < CH; i++) h[u].e[i] = row[col + i < channels ? col + i : channels - 1];
+            } else {
+               h[u] = *reinterpret_cast<const Taps*>(row + at);
             }
          }
          uint32_t q[SEQS][TAPS], s[SEQS][TAPS];
@@ -229,7 +228,7 @@ cache_conv(CacheParams c, const T* taps, uint32_t tap_count, uint32_t chunk, uin
                s[g][u] = (c.scales + (from >> 4))[scale_at];
             }
          }
-         if constexpr(MODE == CUT) {
+         if constexpr(CUT) {
 #pragma unroll
             for(int u = 0; u < TAPS; u++) drop_first<T, CH>(h[u].e, drop);
          }
@@ -245,9 +244,8 @@ cache_conv(CacheParams c, const T* taps, uint32_t tap_count, uint32_t chunk, uin
             }
       }
    };
-   if(col - lane * CH + 64 * CH <= c.channels) steps(std::integral_constant<int, INSIDE>());
-   else if(c.channels >= CH)                   steps(std::integral_constant<int, CUT>());
-   else                                        steps(std::integral_constant<int, FEW>());
+   if(FEW || col - lane * CH + 64 * CH <= c.channels) steps(std::false_type());
+   else if constexpr(!FEW)                            steps(std::true_type());
 #pragma unroll
    for(int g = 0; g < SEQS; g++) {
       if(b0 + g >= c.batch) break;
@@ -309,7 +307,7 @@ hipError_t read_typed(const CacheParams& c, T* out, int64_t length, bool channel
    return hipGetLastError();
 }
 
-template<class T, int CH, int SEQS, int TAPS, int WAVES>
+template<class T, int CH, int SEQS, int TAPS, int WAVES, bool FEW = false>
 hipError_t conv_shape(const CacheParams& c, const T* taps, int64_t tap_count, float* direct, float* work,
                       int64_t splits, int* used, hipStream_t s)
 {
@@ -329,7 +327,7 @@ hipError_t conv_shape(const CacheParams& c, const T* taps, int64_t tap_count, fl
    if(grid > 0x7fffffff || parts / slices > 0x7fffffff) return hipErrorInvalidValue;
    const int count = (int)(parts / slices);
    float* sums = count == 1 && direct ? direct : work;
-   cache_conv<T, CH, SEQS, TAPS, WAVES><<<(unsigned)grid, 64 * WAVES, 0, s>>>(
+   cache_conv<T, CH, SEQS, TAPS, WAVES, FEW><<<(unsigned)grid, 64 * WAVES, 0, s>>>(
       c, taps, (uint32_t)tap_count, (uint32_t)chunk, (uint32_t)cp, (uint32_t)slices, (uint32_t)parts, (uint32_t)seq_groups, sums);
    *used = sums == direct ? 0 : count;
    return hipGetLastError();
@@ -346,6 +344,9 @@ hipError_t conv_typed(const CacheParams& c, const T* taps, int64_t tap_count, fl
    // More: what scalar work a token costs counts, so 8 channels, and registers for four
    // sequences with 2 taps (24 x 8000 x 4096, fp32 taps: 4 x 2 taps 126 us, 4 x 4 148, 2 x 4 170;
    // 2 x 4000 x 4096 two at a time 21, one 22.5).
+   // Fewer channels than a lane may hold have a kernel of their own, as a third loop in each
+   // kernel would spill scalars.
+   if(c.channels < 8) return conv_shape<T, 4, 1, 8, 16, true>(c, taps, tap_count, direct, work, splits, used, s);
    const int64_t lanes = c.batch * ((padded(c.channels) + 255) / 256);
    if(c.batch == 1 || lanes <= 16) return conv_shape<T, 4, 1, 8, 16>(c, taps, tap_count, direct, work, splits, used, s);
    if(c.batch <= 3) return conv_shape<T, 8, 2, 4, 8>(c, taps, tap_count, direct, work, splits, used, s);
