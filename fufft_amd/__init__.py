@@ -715,8 +715,10 @@ def bfp_dequantize(q: np.ndarray, e: np.ndarray, block: int = BFP_BLOCK) -> np.n
 
 # ---- microscaled 4-bit blocks (mx4) ------------------------------------------------------
 # Blocks of 32 values share a scale byte; a row's codes are uint8 (mx4_padded(k) // 2 of them),
-# its scales uint8 (mx4_padded(k) // 32).  Matrices of ordinary elements (fp32, bf16, fp16) are
-# 2D tensors whose rows may be apart (x.stride(0) >= columns) and whose elements are adjacent.
+# its scales uint8 (mx4_padded(k) // 32).  Codes and scales with rows of their own (two dimensions
+# or more) have rows of that length, or the call is refused; flat ones are rows of it, one after the other.
+# Matrices of ordinary elements (fp32, bf16, fp16) are 2D tensors whose rows may be apart
+# (x.stride(0) >= columns) and whose elements are adjacent.
 
 MX4_BLOCK = 32
 MX4_RULE = {"fit": 0, "floor": 1}
@@ -786,10 +788,19 @@ def _array(x, name: str, nbytes: int, kind: str) -> int:
     return x.data_ptr()
 
 
+def _rows(x, name: str, rows: int, width: int) -> int:
+    """The address of `rows` rows of `width` bytes, checked but for their device.  A tensor with rows of
+    another length, made for other sizes, would be read at the wrong places."""
+    p = _array(x, name, rows * width, "bytes")
+    if x.dim() > 1 and rows * width > 0 and x.shape[-1] != width:
+        raise ValueError(f"{name}: has rows of {x.shape[-1]} bytes, the call's have {width}")
+    return p
+
+
 def _blocks(codes, scales, name: str, rows: int, k: int):
     """The addresses of `rows` rows of k values in blocks, checked but for their device."""
     groups = (k + 127) // 128
-    return (_array(codes, name, rows * groups * 64, "bytes"), _array(scales, name + "_scales", rows * groups * 4, "bytes"))
+    return _rows(codes, name, rows, groups * 64), _rows(scales, name + "_scales", rows, groups * 4)
 
 
 def _bias(bias, n: int):
@@ -817,7 +828,7 @@ def mx4_quantize(x, codes=None, scales=None, codes_t=None, scales_t=None, *, ran
     if codes_t is not None or scales_t is not None:
         qc, qs = _blocks(codes_t, scales_t, "codes_t", k, rows)
     if rand is not None:
-        pr = _array(rand, "rand", rows * k, "bytes")
+        pr = _rows(rand, "rand", rows, k)
     _on_gpu((x, "x"), (codes, "codes"), (scales, "codes_scales"), (codes_t, "codes_t"), (scales_t, "codes_t_scales"),
             (rand, "rand"))
     check(lib.fufft_mx4_quantize(x.data_ptr(), kind, ld, rows, k, rule, pr, pc, ps, qc, qs, _stream(stream)),

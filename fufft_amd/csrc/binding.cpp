@@ -64,6 +64,15 @@ Matrix matrix(PyObject* o, int64_t gpu)
    return m;
 }
 
+// `rows` rows of `width` bytes: a flat array, or one whose own rows have that length
+void* rows_of(PyObject* o, int64_t rows, int64_t width, int64_t gpu)
+{
+   void* const p = array(o, at::kByte, rows * width, gpu);
+   const at::Tensor& t = THPVariable_Unpack(o);
+   if(t.dim() > 1 && rows * width > 0 && t.size(t.dim() - 1) != width) throw Refused();
+   return p;
+}
+
 struct Blocks {
    void*    codes;
    uint8_t* scales;
@@ -71,8 +80,7 @@ struct Blocks {
 Blocks blocks(PyObject* codes, PyObject* scales, int64_t rows, int64_t k, int64_t gpu)
 {
    const int64_t groups = (k + 127) / 128;
-   return {array(codes, at::kByte, rows * groups * 64, gpu),
-           static_cast<uint8_t*>(array(scales, at::kByte, rows * groups * 4, gpu))};
+   return {rows_of(codes, rows, groups * 64, gpu), static_cast<uint8_t*>(rows_of(scales, rows, groups * 4, gpu))};
 }
 
 // codes (pages, page, bytes of a row) and scales of the same pages
@@ -156,7 +164,7 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n)
       const Blocks q = along ? blocks(a[1], a[2], x.rows, x.k, gpu) : Blocks{nullptr, nullptr};
       const Blocks t = across ? blocks(a[3], a[4], x.k, x.rows, gpu) : Blocks{nullptr, nullptr};
       const uint8_t* const rand =
-         a[5] == Py_None ? nullptr : static_cast<const uint8_t*>(array(a[5], at::kByte, x.rows * x.k, gpu));
+         a[5] == Py_None ? nullptr : static_cast<const uint8_t*>(rows_of(a[5], x.rows, x.k, gpu));
       const int rule = (int)integer(a[6]);
       return status_of([&] {
          return fufft_mx4_quantize(x.p, x.type, x.ld, x.rows, x.k, rule, rand, q.codes, q.scales, t.codes, t.scales, stream);
