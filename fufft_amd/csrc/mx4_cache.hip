@@ -30,16 +30,17 @@ __device__ inline int64_t sequence_length(const CacheParams& c, int64_t b)
    return n < 0 ? 0 : n < most ? n : most;
 }
 
-// out[b][t][channel], zeros from each sequence's length on: 8 channels a lane.
+// out[b][t][channel], zeros from each sequence's length on: 8 channels a lane, the tokens of
+// this launch from `first` on.
 template<class T, int ROWS>
 __global__ void __launch_bounds__(kLanes)
-read_tokens(CacheParams c, T* out, int64_t length, int64_t cp, int lr)
+read_tokens(CacheParams c, T* out, int64_t first, int64_t length, int64_t cp, int lr)
 {
    const int lane = threadIdx.x & ((1 << lr) - 1);
    const int64_t col = ((int64_t)blockIdx.x << (lr + 3)) + lane * 8;
    if(col >= c.channels) return;
    const int per = kLanes >> lr;
-   const int64_t t0 = (int64_t)blockIdx.y * (per * ROWS) + (threadIdx.x >> lr);
+   const int64_t t0 = first + (int64_t)blockIdx.y * (per * ROWS) + (threadIdx.x >> lr);
    for(int64_t b = blockIdx.z; b < c.batch; b += gridDim.z) {
       const int64_t n = sequence_length(c, b);
       const int32_t* table = c.table + b * c.width;
@@ -76,16 +77,16 @@ read_tokens(CacheParams c, T* out, int64_t length, int64_t cp, int lr)
    }
 }
 
-// out[b][channel][t], zeros from each sequence's length on: tiles of 64 tokens x
-// 128 channels turned in LDS, so that codes are read along channels and signals
+// out[b][channel][t], zeros from each sequence's length on, from token `first` on: tiles of 64 tokens
+// x 128 channels turned in LDS, so that codes are read along channels and signals
 // written along tokens.  4 x 8192 tokens x 2048 channels in fp32: 63 to 72 us, 268 MB written at
 // 3.7 to 4.3 TB/s.
 template<class T>
 __global__ void __launch_bounds__(kLanes)
-read_channels(CacheParams c, T* out, int64_t length, int64_t cp)
+read_channels(CacheParams c, T* out, int64_t first, int64_t length, int64_t cp)
 {
    __shared__ float tile[128 * 65];
-   const int64_t c0 = (int64_t)blockIdx.x * 128, t0 = (int64_t)blockIdx.y * 64;
+   const int64_t c0 = (int64_t)blockIdx.x * 128, t0 = first + (int64_t)blockIdx.y * 64;
    const int lane = threadIdx.x & 15;
    for(int64_t b = blockIdx.z; b < c.batch; b += gridDim.z) {
       const int64_t n = sequence_length(c, b);
@@ -286,25 +287,28 @@ join_splits(const float* sums, T* out, int64_t count, int splits)
    }
 }
 
+// A launch for every 65535 tiles of tokens, a grid's end in y: beyond them a text is long enough that
+// a launch more costs nothing (a loop in the kernel costs the others: 4 x 8192 x 2048 to bf16 rows 34 -> 35 us).
 template<class T>
 hipError_t read_typed(const CacheParams& c, T* out, int64_t length, bool channels_first, hipStream_t s)
 {
+   constexpr int ROWS = 4;
    const int64_t cp = padded(c.channels);
    const unsigned gz = (unsigned)(c.batch < 65535 ? c.batch : 65535);
-   if(channels_first) {
-      const int64_t gy = (length + 63) / 64;
-      if(gy > 65535 || cp / 128 > 0x7fffffff) return hipErrorInvalidValue;
-      read_channels<T><<<dim3((unsigned)(cp / 128), (unsigned)gy, gz), kLanes, 0, s>>>(c, out, length, cp);
-   } else {
-      constexpr int ROWS = 4;
-      int lr = 4;
-      while(lr < 8 && ((int64_t)8 << lr) < cp) lr++;
-      const int64_t per = (kLanes >> lr) * ROWS, gy = (length + per - 1) / per;
-      const int64_t gx = (cp / 8 + (1 << lr) - 1) >> lr;
-      if(gy > 65535 || gx > 0x7fffffff) return hipErrorInvalidValue;
-      read_tokens<T, ROWS><<<dim3((unsigned)gx, (unsigned)gy, gz), kLanes, 0, s>>>(c, out, length, cp, lr);
+   int lr = 4;
+   while(lr < 8 && ((int64_t)8 << lr) < cp) lr++;
+   const int64_t per = channels_first ? 64 : (kLanes >> lr) * ROWS;
+   const int64_t gx = channels_first ? cp / 128 : (cp / 8 + (1 << lr) - 1) >> lr;
+   if(gx > 0x7fffffff) return hipErrorInvalidValue;
+   for(int64_t first = 0; first < length; first += 65535 * per) {
+      const int64_t tiles = (length - first + per - 1) / per;
+      const dim3 g((unsigned)gx, (unsigned)(tiles < 65535 ? tiles : 65535), gz);
+      if(channels_first) read_channels<T><<<g, kLanes, 0, s>>>(c, out, first, length, cp);
+      else               read_tokens<T, ROWS><<<g, kLanes, 0, s>>>(c, out, first, length, cp, lr);
+      const hipError_t e = hipGetLastError();
+      if(e != hipSuccess) return e;
    }
-   return hipGetLastError();
+   return hipSuccess;
 }
 
 template<class T, int CH, int SEQS, int TAPS, int WAVES, bool FEW = false>

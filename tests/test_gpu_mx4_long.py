@@ -1,0 +1,45 @@
+"""GPU tests of the 4-bit calls on long texts, many rows and many sequences: more tiles than one
+dimension of a grid takes."""
+import numpy as np
+import pytest
+
+import mx4_reference as R
+from test_gpu_mx4 import signal, to_dev, torch_type
+
+pytestmark = pytest.mark.gpu
+
+
+def small_cache(rng, dev, pages, page, channels):
+    """A cache of few pages on the GPU, and the values of its slots."""
+    c, s = R.quantize(signal(rng, pages * page, channels))
+    values = R.values(c, s, channels)
+    dc, ds = to_dev(dev, c.reshape(pages, page, -1), s.reshape(pages, page, -1))
+    return dc, ds, values
+
+
+# tokens order: 4 tokens a workgroup above 1024 channels, 64 below 129, so 65535 workgroups are 262140 and
+# 4194240 tokens; channels order: 64 always
+@pytest.mark.parametrize("order,channels,length,kind", [("tokens", 2048, 300001, "bf16"), ("tokens", 1030, 262141, "f16"),
+                                                        ("tokens", 5, 4194300, "f32"), ("channels", 3, 4194305, "f32"),
+                                                        ("channels", 130, 4194300, "bf16")])
+def test_read_long_texts(dev, rng, order, channels, length, kind):
+    """Every token of a long text, a short one and one that ends beyond the last whole round, each a row of
+    one of the few pages that the page tables repeat."""
+    import torch
+    import fufft_amd as ff
+    print(f"case cache read {length} x {channels} {kind}, {order}", flush=True)
+    page, pages = 64, 11
+    codes, scales, values = small_cache(rng, dev, pages, page, channels)
+    rows = torch.from_numpy(values).to(torch_type(kind)).to(dev)
+    width = -(-length // page)
+    table = torch.from_numpy(rng.integers(0, pages, (3, width)).astype(np.int32)).to(dev)
+    lens = torch.tensor([length, 70, length - 3], dtype=torch.int32, device=dev)
+    shape = (length, channels) if order == "tokens" else (channels, length)
+    out = torch.full((3, *shape), 7.0, dtype=torch_type(kind), device=dev)
+    ff.mx4_cache_read(codes, scales, table, lens, out, order=order)
+    torch.cuda.synchronize()
+    t = torch.arange(length, device=dev)
+    for b in range(3):
+        want = rows[table[b].long()[t // page] * page + t % page]
+        want[int(lens[b]):] = 0
+        assert torch.equal(out[b] if order == "tokens" else out[b].t(), want)
