@@ -595,17 +595,27 @@ hipError_t matmul_typed(const MatmulParams& p, hipStream_t s)
    return tiles_shape<O, 64, 64, 2, 2>(p, s);
 }
 
+// A launch for every 65535 tiles of rows, a grid's end in y.
 template<class T, class O, int MT, int NT, int DEPTH>
 hipError_t linear_shape(const MatmulParams& p, hipStream_t s)
 {
    const int64_t groups = padded(p.k) / kGroup;
    if(groups > 0x3fffffff) return hipErrorInvalidValue;
    const int waves = wavefronts((groups + kRun - 1) / kRun, most_waves(MT * NT));
-   const int64_t gx = (p.n + 16 * NT - 1) / (16 * NT), gy = (p.m + 16 * MT - 1) / (16 * MT);
-   if(gx > 0x7fffffff || gy > 65535) return hipErrorInvalidValue;
-   linear_rows<T, O, MT, NT, DEPTH><<<dim3((unsigned)gx, (unsigned)gy), waves * 64, (size_t)waves * MT * NT * 1024,
-                                      s>>>(p, (int)groups, waves);
-   return hipGetLastError();
+   const int64_t gx = (p.n + 16 * NT - 1) / (16 * NT), most = 65535 * 16 * MT;
+   if(gx > 0x7fffffff) return hipErrorInvalidValue;
+   for(int64_t first = 0; first < p.m; first += most) {
+      MatmulParams q = p;
+      q.m = p.m - first < most ? p.m - first : most;
+      q.x = static_cast<const T*>(p.x) + first * p.ldx;
+      q.out = static_cast<O*>(p.out) + first * p.ld;
+      const unsigned gy = (unsigned)((q.m + 16 * MT - 1) / (16 * MT));
+      linear_rows<T, O, MT, NT, DEPTH><<<dim3((unsigned)gx, gy), waves * 64, (size_t)waves * MT * NT * 1024, s>>>(
+         q, (int)groups, waves);
+      const hipError_t e = hipGetLastError();
+      if(e != hipSuccess) return e;
+   }
+   return hipSuccess;
 }
 
 template<class T, class O>

@@ -43,3 +43,24 @@ def test_read_long_texts(dev, rng, order, channels, length, kind):
         want = rows[table[b].long()[t // page] * page + t % page]
         want[int(lens[b]):] = 0
         assert torch.equal(out[b] if order == "tokens" else out[b].t(), want)
+
+
+@pytest.mark.parametrize("n,k,kind,out", [(3, 40, "bf16", "f32"), (5, 130, "f32", "bf16")])
+def test_linear_many_rows(dev, rng, n, k, kind, out):
+    """More rows than 65535 tiles of 32 hold, in rows apart: each the product of its own x.  Integers and
+    halves, whose sums are exact; the last rows are other rows' values, so they differ from the first."""
+    import torch
+    import fufft_amd as ff
+    m = 65535 * 32 + 77
+    print(f"case linear {m}x{n}x{k} {kind} -> {out}", flush=True)
+    x = torch.randint(-3, 4, (m, k + 3), device=dev).to(torch_type(kind))[:, :k]
+    q = rng.integers(0, 4, (n, R.padded(k))).astype(np.uint8)                # 0, .5, 1, 1.5
+    q[:, k:] = 0
+    codes, scales = q[:, 0::2] + 16 * q[:, 1::2], np.full((n, R.padded(k) // 32), 127, np.uint8)
+    w = torch.from_numpy(R.values(codes, scales, k)).float().to(dev)
+    o = torch.full((m + 1, n + 1), 7.0, dtype=torch_type(out), device=dev)
+    ff.mx4_linear(x, *to_dev(dev, codes, scales), o[:m, :n])
+    torch.cuda.synchronize()
+    want = (x.double() @ w.double().t().contiguous()).float()
+    assert torch.equal(o[:m, :n], want.to(o.dtype))
+    assert bool((o[m] == 7).all()) and bool((o[:, n] == 7).all())
