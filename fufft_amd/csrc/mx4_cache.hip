@@ -327,14 +327,26 @@ hipError_t conv_shape(const CacheParams& c, const T* taps, int64_t tap_count, fl
    int64_t chunk = ((tap_count + want - 1) / want + step - 1) / step * step;
    if(chunk < step) chunk = step;
    const int64_t parts = slices * (tap_count > 0 ? (tap_count + chunk - 1) / chunk : 1);
-   const int64_t grid = (parts + 7) / 8 * 8 * seq_groups;
-   if(grid > 0x7fffffff || parts / slices > 0x7fffffff) return hipErrorInvalidValue;
+   const int64_t sets = (parts + 7) / 8 * 8, most_groups = kMostLanes / (64 * WAVES) / sets;
+   if(most_groups < 1 || parts / slices > 0x7fffffff) return hipErrorInvalidValue;
    const int count = (int)(parts / slices);
    float* sums = count == 1 && direct ? direct : work;
-   cache_conv<T, CH, SEQS, TAPS, WAVES, FEW><<<(unsigned)grid, 64 * WAVES, 0, s>>>(
-      c, taps, (uint32_t)tap_count, (uint32_t)chunk, (uint32_t)cp, (uint32_t)slices, (uint32_t)parts, (uint32_t)seq_groups, sums);
+   // one launch, but for so many sequences that its lanes would pass 32 bits: these have one split, so
+   // the sums of each launch's sequences lie together
+   for(int64_t first = 0; first < seq_groups; first += most_groups) {
+      const int64_t groups = seq_groups - first < most_groups ? seq_groups - first : most_groups, b0 = first * SEQS;
+      CacheParams q = c;
+      q.table += b0 * c.width;
+      q.lens += b0;
+      if(groups < seq_groups) q.batch = c.batch - b0 < groups * SEQS ? c.batch - b0 : groups * SEQS;
+      cache_conv<T, CH, SEQS, TAPS, WAVES, FEW><<<(unsigned)(sets * groups), 64 * WAVES, 0, s>>>(
+         q, taps, (uint32_t)tap_count, (uint32_t)chunk, (uint32_t)cp, (uint32_t)slices, (uint32_t)parts, (uint32_t)groups,
+         sums + b0 * c.channels);
+      const hipError_t e = hipGetLastError();
+      if(e != hipSuccess) return e;
+   }
    *used = sums == direct ? 0 : count;
-   return hipGetLastError();
+   return hipSuccess;
 }
 
 template<class T>
@@ -355,6 +367,20 @@ hipError_t conv_typed(const CacheParams& c, const T* taps, int64_t tap_count, fl
    if(c.batch == 1 || lanes <= 16) return conv_shape<T, 4, 1, 8, 16>(c, taps, tap_count, direct, work, splits, used, s);
    if(c.batch <= 3) return conv_shape<T, 8, 2, 4, 8>(c, taps, tap_count, direct, work, splits, used, s);
    return conv_shape<T, 8, 4, 2, 8>(c, taps, tap_count, direct, work, splits, used, s);
+}
+
+template<class T>
+hipError_t join_typed(const float* sums, T* out, int64_t count, int splits, hipStream_t s)
+{
+   // one launch, but for so many results that its lanes would pass 32 bits: these have one split
+   constexpr int64_t most = kMostLanes / kLanes * 32;
+   for(int64_t first = 0; first < count; first += most) {
+      const int64_t n = count - first < most ? count - first : most;
+      join_splits<T><<<(unsigned)((n + 31) / 32), kLanes, 0, s>>>(sums + first, out + first, n, splits);
+      const hipError_t e = hipGetLastError();
+      if(e != hipSuccess) return e;
+   }
+   return hipSuccess;
 }
 
 }  // namespace
@@ -388,15 +414,11 @@ hipError_t launch_cache_conv(const CacheParams& c, const void* taps, int tap_typ
       default:     e = conv_typed(c, static_cast<const f16*>(taps), tap_count, direct, work, splits, &used, s); break;
    }
    if(e != hipSuccess || used == 0) return e;
-   const int64_t count = c.batch * c.channels, groups = (count + 31) / 32;
-   if(groups > 0x7fffffff) return hipErrorInvalidValue;
-   const dim3 g((unsigned)groups);
    switch(out_type) {
-      case T_F32:  join_splits<float><<<g, kLanes, 0, s>>>(work, static_cast<float*>(out), count, used); break;
-      case T_BF16: join_splits<bf16><<<g, kLanes, 0, s>>>(work, static_cast<bf16*>(out), count, used); break;
-      default:     join_splits<f16><<<g, kLanes, 0, s>>>(work, static_cast<f16*>(out), count, used); break;
+      case T_F32:  return join_typed(work, static_cast<float*>(out), c.batch * c.channels, used, s);
+      case T_BF16: return join_typed(work, static_cast<bf16*>(out), c.batch * c.channels, used, s);
+      default:     return join_typed(work, static_cast<f16*>(out), c.batch * c.channels, used, s);
    }
-   return hipGetLastError();
 }
 
 }  // namespace mx4

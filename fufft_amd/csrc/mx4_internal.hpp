@@ -13,6 +13,10 @@ enum { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
 inline int64_t type_bytes(int type) { return type == T_F32 ? 4 : 2; }
 inline int64_t padded(int64_t k) { return (k + 127) / 128 * 128; }
 
+// Lanes that one launch may have in x: the runtime counts them in 32 bits, and starts a grid
+// of more without an error but with the count's low bits.
+constexpr int64_t kMostLanes = 0xffffffff;
+
 struct QuantizeParams {
    const void*    x;         // rows x k, leading dimension ld (elements)
    const uint8_t* rand;      // a byte per value, rows x k, or NULL: nearest

@@ -64,3 +64,32 @@ def test_linear_many_rows(dev, rng, n, k, kind, out):
     want = (x.double() @ w.double().t().contiguous()).float()
     assert torch.equal(o[:m, :n], want.to(o.dtype))
     assert bool((o[m] == 7).all()) and bool((o[:, n] == 7).all())
+
+
+# workgroups of 1024 lanes, 8 for a sequence, up to 7 channels; of 512, 2 for a sequence, above; the join
+# has 8 lanes a result: each beyond 2^32 lanes in one launch
+@pytest.mark.parametrize("batch,channels,kind", [(524300, 3, "f32"), (4194310, 9, "bf16"), (131100, 4100, "bf16")])
+def test_conv_many_sequences(dev, rng, batch, channels, kind):
+    """Sequences of 0 to 2 tokens; values and taps whose sums are exact in the results' type."""
+    import torch
+    import fufft_amd as ff
+    print(f"case cache conv {batch} x {channels} -> {kind}", flush=True)
+    page, pages = 2, 5
+    q = rng.integers(0, 16, (pages * page, R.padded(channels))).astype(np.uint8)
+    q[:, channels:] = 0
+    codes, scales = q[:, 0::2] + 16 * q[:, 1::2], np.full((pages * page, R.padded(channels) // 32), 127, np.uint8)
+    values = torch.from_numpy(R.values(codes, scales, channels)).float().to(dev)
+    dc, ds = to_dev(dev, codes.reshape(pages, page, -1), scales.reshape(pages, page, -1))
+    table = torch.randint(0, pages, (batch, 1), device=dev, dtype=torch.int32)
+    lens = torch.randint(0, 3, (batch,), device=dev, dtype=torch.int32)
+    taps = torch.randint(-2, 3, (2, channels), device=dev).float()
+    out = torch.full((batch + 1, channels), 7.0, dtype=torch_type(kind), device=dev)
+    work = None if kind == "f32" else torch.empty(1, batch, channels, device=dev)
+    ff.mx4_cache_conv(dc, ds, table, lens, taps, out[:batch], work=work)
+    torch.cuda.synchronize()
+    # every (page, length) has one result
+    first, second = values[0::2], values[1::2]
+    each = torch.stack((torch.zeros_like(first), taps[0] * first, taps[0] * second + taps[1] * first)).to(out.dtype)
+    for i in torch.arange(batch, device=dev).split(1 << 16):
+        assert torch.equal(out[i], each[lens[i].long(), table[i, 0].long()] + 0.0)
+    assert bool((out[batch] == 7).all())
