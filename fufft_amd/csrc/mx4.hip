@@ -310,7 +310,7 @@ int lanes_log(int64_t kp)
 bool make_grid(int64_t gx, int64_t tiles, dim3* g)
 {
    const int64_t gy = tiles < 65535 ? tiles : 65535, gz = (tiles + gy - 1) / gy;
-   if(gx > 0x7fffffff || gz > 65535) return false;
+   if(!grid_ok(gx, kLanes) || gz > 65535) return false;
    *g = dim3((unsigned)gx, (unsigned)gy, (unsigned)gz);
    return true;
 }
@@ -322,13 +322,13 @@ hipError_t quantize_typed(const QuantizeParams& p, hipStream_t s)
    dim3 g;
    if(p.codes_t) {
       const int64_t rowsp = padded(p.rows);
-      if(!make_grid(kp / 128, rowsp / 128, &g)) return hipErrorInvalidValue;
+      if(!make_grid(kp / 128, rowsp / 128, &g)) return kTooLarge;
       quantize_both<T, RAND><<<g, kLanes, 0, s>>>(p, kp, rowsp);
    } else {
       constexpr int ROWS = 4;
       const int lr = lanes_log(kp);
       const int64_t per = (kLanes >> lr) * ROWS;
-      if(!make_grid((kp / 8 + (1 << lr) - 1) >> lr, (p.rows + per - 1) / per, &g)) return hipErrorInvalidValue;
+      if(!make_grid((kp / 8 + (1 << lr) - 1) >> lr, (p.rows + per - 1) / per, &g)) return kTooLarge;
       quantize_rows<T, RAND, ROWS><<<g, kLanes, 0, s>>>(p, kp, lr);
    }
    return hipGetLastError();
@@ -342,7 +342,7 @@ hipError_t dequantize_typed(const DequantizeParams& p, hipStream_t s)
    const int lr = lanes_log(kp);
    const int64_t per = (kLanes >> lr) * ROWS;
    dim3 g;
-   if(!make_grid((kp / 8 + (1 << lr) - 1) >> lr, (p.rows + per - 1) / per, &g)) return hipErrorInvalidValue;
+   if(!make_grid((kp / 8 + (1 << lr) - 1) >> lr, (p.rows + per - 1) / per, &g)) return kTooLarge;
    dequantize_rows<T, ROWS><<<g, kLanes, 0, s>>>(p, kp, lr);
    return hipGetLastError();
 }

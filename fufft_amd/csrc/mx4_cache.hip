@@ -299,7 +299,7 @@ hipError_t read_typed(const CacheParams& c, T* out, int64_t length, bool channel
    while(lr < 8 && ((int64_t)8 << lr) < cp) lr++;
    const int64_t per = channels_first ? 64 : (kLanes >> lr) * ROWS;
    const int64_t gx = channels_first ? cp / 128 : (cp / 8 + (1 << lr) - 1) >> lr;
-   if(gx > 0x7fffffff) return hipErrorInvalidValue;
+   if(!grid_ok(gx, kLanes)) return kTooLarge;
    for(int64_t first = 0; first < length; first += 65535 * per) {
       const int64_t tiles = (length - first + per - 1) / per;
       const dim3 g((unsigned)gx, (unsigned)(tiles < 65535 ? tiles : 65535), gz);
@@ -316,7 +316,7 @@ hipError_t conv_shape(const CacheParams& c, const T* taps, int64_t tap_count, fl
                       int64_t splits, int* used, hipStream_t s)
 {
    const int64_t cp = padded(c.channels), slices = (cp + 64 * CH - 1) / (64 * CH);
-   if(cp > 0x7fffffff) return hipErrorInvalidValue;
+   if(cp > 0x7fffffff) return kTooLarge;
    const int64_t seq_groups = (c.batch + SEQS - 1) / SEQS, step = WAVES * TAPS;
    // two workgroups a CU, each with one step at least
    int64_t want = (512 + slices * seq_groups - 1) / (slices * seq_groups);
@@ -328,7 +328,7 @@ hipError_t conv_shape(const CacheParams& c, const T* taps, int64_t tap_count, fl
    if(chunk < step) chunk = step;
    const int64_t parts = slices * (tap_count > 0 ? (tap_count + chunk - 1) / chunk : 1);
    const int64_t sets = (parts + 7) / 8 * 8, most_groups = kMostLanes / (64 * WAVES) / sets;
-   if(most_groups < 1 || parts / slices > 0x7fffffff) return hipErrorInvalidValue;
+   if(most_groups < 1 || parts / slices > 0x7fffffff) return kTooLarge;
    const int count = (int)(parts / slices);
    float* sums = count == 1 && direct ? direct : work;
    // one launch, but for so many sequences that its lanes would pass 32 bits: these have one split, so

@@ -57,7 +57,10 @@ bool matrix_ok(int type, int64_t ld, int64_t rows, int64_t k)
 Span codes_of(const void* p, int64_t rows, int64_t k) { return {p, rows * (padded(k) / 2)}; }
 Span scales_of(const void* p, int64_t rows, int64_t k) { return {p, rows * (padded(k) / 32)}; }
 
-int status_of(hipError_t e) { return e == hipSuccess ? FUFFT_OK : FUFFT_ERR_HIP; }
+int status_of(hipError_t e)
+{
+   return e == hipSuccess ? FUFFT_OK : e == kTooLarge ? FUFFT_ERR_UNSUPPORTED : FUFFT_ERR_HIP;
+}
 
 #define FUFFT_MX4_CHECK(expr)                       \
    do {                                             \

@@ -16,6 +16,10 @@ inline int64_t padded(int64_t k) { return (k + 127) / 128 * 128; }
 // Lanes that one launch may have in x: the runtime counts them in 32 bits, and starts a grid
 // of more without an error but with the count's low bits.
 constexpr int64_t kMostLanes = 0xffffffff;
+inline bool grid_ok(int64_t blocks, int64_t lanes) { return blocks <= kMostLanes / lanes; }
+
+// what the launches below return for sizes that they cannot hold, before anything is launched
+constexpr hipError_t kTooLarge = hipErrorNotSupported;
 
 struct QuantizeParams {
    const void*    x;         // rows x k, leading dimension ld (elements)

@@ -532,7 +532,7 @@ hipError_t tiles_shape(const MatmulParams& p, hipStream_t s)
 {
    constexpr size_t bytes = (size_t)(BM + BN) * (2 * 128 + 64);
    const int64_t groups = padded(p.k) / kGroup, tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
-   if(tm * tn > 0x7fffffff) return hipErrorInvalidValue;
+   if(!grid_ok(tm * tn, 64 * WM * WN)) return kTooLarge;
    static std::atomic<uint64_t> mask{0};
    const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(&matmul_tiles<O, BM, BN, WM, WN>), bytes, mask);
    if(e != hipSuccess) return e;
@@ -553,10 +553,10 @@ template<class O, int MT, int NT, int DEPTH>
 hipError_t rows_shape(const MatmulParams& p, hipStream_t s)
 {
    const int64_t groups = padded(p.k) / kGroup;
-   if(groups > 0x3fffffff) return hipErrorInvalidValue;
+   if(groups > 0x3fffffff) return kTooLarge;
    const int waves = wavefronts((groups + kRun - 1) / kRun, most_waves(MT * NT));
    const int64_t gx = (p.n + 16 * NT - 1) / (16 * NT), gy = (p.m + 16 * MT - 1) / (16 * MT);
-   if(gx > 0x7fffffff || gy > 65535) return hipErrorInvalidValue;
+   if(!grid_ok(gx, waves * 64) || gy > 65535) return kTooLarge;
    matmul_rows<O, MT, NT, DEPTH><<<dim3((unsigned)gx, (unsigned)gy), waves * 64, (size_t)waves * MT * NT * 1024, s>>>(
       p, (int)groups, waves);
    return hipGetLastError();
@@ -600,10 +600,10 @@ template<class T, class O, int MT, int NT, int DEPTH>
 hipError_t linear_shape(const MatmulParams& p, hipStream_t s)
 {
    const int64_t groups = padded(p.k) / kGroup;
-   if(groups > 0x3fffffff) return hipErrorInvalidValue;
+   if(groups > 0x3fffffff) return kTooLarge;
    const int waves = wavefronts((groups + kRun - 1) / kRun, most_waves(MT * NT));
    const int64_t gx = (p.n + 16 * NT - 1) / (16 * NT), most = 65535 * 16 * MT;
-   if(gx > 0x7fffffff) return hipErrorInvalidValue;
+   if(!grid_ok(gx, waves * 64)) return kTooLarge;
    for(int64_t first = 0; first < p.m; first += most) {
       MatmulParams q = p;
       q.m = p.m - first < most ? p.m - first : most;

@@ -497,7 +497,11 @@ int fufft_apply2d_f32(const void* spec, int64_t spec_stride, const void* filt,
  * leading dimension ld (elements, >= k), only need their element's alignment.
  * Element types: FUFFT_F32, FUFFT_BF16, FUFFT_F16.  Sums are fp32, rounded once
  * to the output's type.  Sizes of zero are allowed and pointers to nothing may
- * then be NULL.  Inputs and outputs of a call share no byte. */
+ * then be NULL.  Inputs and outputs of a call share no byte.
+ *
+ * Rows of up to 2^31 - 128 values, and products of fewer than 2^28 rows of each
+ * 4-bit operand and 2^38 results, are always taken; beyond them, sizes that no
+ * launch can hold are FUFFT_ERR_UNSUPPORTED. */
 #define FUFFT_F32   0
 #define FUFFT_BF16  1
 #define FUFFT_F16   2
