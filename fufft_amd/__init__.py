@@ -2,7 +2,8 @@
 
 The compute path is the in-tree HIP library ``libfufft_amd.so`` (built by
 ``fufft_amd.build``).  There is no fallback: if the library is missing, import
-fails loudly.  Device buffers are torch tensors on ``cuda`` (ROCm); every
+fails loudly.  (``_binding.so`` beside it is a shorter way from Python to some of
+its calls, not a second implementation.)  Device buffers are torch tensors on ``cuda`` (ROCm); every
 launch wrapper checks their dtype, contiguity, size and device before the
 call (``_ptrs``), and launches on torch's current stream unless given one.
 
@@ -13,6 +14,8 @@ the library's dependency to that same copy).
 from __future__ import annotations
 
 import ctypes as C
+import re
+import warnings
 from pathlib import Path
 
 import numpy as np
@@ -135,12 +138,26 @@ def _load() -> C.CDLL:
     return L
 
 
+def _load_binding():
+    """The native way to the 4-bit calls (_binding.so), or None: without it they go through ctypes, to the
+    same kernels at 2 us more of the host's time.  One built for another torch or another
+    library is left alone, with a warning."""
+    path = _LIB_PATH.with_name("_binding.so")
+    if torch is None or not path.exists():
+        return None
+    try:
+        from . import _binding as b
+        if not re.match(re.escape(b.TORCH) + r"(?!\d)", torch.__version__) or b.ABI != ABI_VERSION:
+            raise ImportError(f"built for torch {b.TORCH} and ABI version {b.ABI}, this is torch {torch.__version__} "
+                              f"and ABI version {ABI_VERSION}")
+    except (ImportError, AttributeError) as e:
+        warnings.warn(f"{path} is not used ({e}): rebuild it with `python fufft_amd/build.py`", RuntimeWarning)
+        return None
+    return b
+
+
 lib = _load()
-if torch is not None:
-    if not _LIB_PATH.with_name("_binding.so").exists():
-        raise FileNotFoundError(f"{_LIB_PATH.with_name('_binding.so')} is missing: build it with "
-                                "`python fufft_amd/build.py`")
-    from . import _binding  # noqa: E402
+_binding = _load_binding()
 
 
 def check(status: int, where: str) -> None:
@@ -743,12 +760,12 @@ def _name(table: dict, key, name: str) -> int:
     return table[key]
 
 
-# Each call goes to the native binding first, which checks every argument and launches.  What it
-# does not take (it answers None) goes through the checks here, which say what is wrong; a
+# Each call goes to the native binding first, where it is there: it checks every argument and launches.
+# What it does not take (it answers None) goes through the checks here, which say what is wrong; a
 # tensor subclass, which it does not take either, passes them and is launched from here.
 
 def _native(x) -> bool:
-    return type(x) is _TENSOR and x.is_cuda
+    return _binding is not None and type(x) is _TENSOR and x.is_cuda
 
 
 def _handle(stream, gpu: int) -> int:

@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 #include "../../include/fufft/fufft.h"
 
@@ -292,4 +293,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", "The 4-bit calls, check
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__binding(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__binding(void)
+{
+   PyObject* const m = PyModule_Create(&module);
+   // what it was built for: tensors are read through inline code, and the calls through the header
+   if(m && (PyModule_AddStringConstant(m, "TORCH", TORCH_VERSION) || PyModule_AddIntConstant(m, "ABI", FUFFT_ABI_VERSION))) {
+      Py_DECREF(m);
+      return nullptr;
+   }
+   return m;
+}
