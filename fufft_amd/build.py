@@ -65,14 +65,21 @@ def build_library(jobs: int = 8) -> Path:
     return LIB
 
 
-def build_binding() -> Path:
+def build_binding() -> Path | None:
     """The native part of the Python binding (fufft_amd/_binding.so): host code only, against
-    the installed torch and linked to the library beside it."""
+    the installed torch and linked to the library beside it.  Without torch, Python's headers or
+    g++ there is none (a C or C++ caller needs none, and the package does without it)."""
     import sysconfig
 
-    import torch
-    from torch.utils import cpp_extension
-
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError:
+        print("torch is not installed: fufft_amd/_binding.so is not built", file=sys.stderr)
+        return None
+    if not shutil.which("g++") or not (Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
+        print("g++ or Python's headers are not installed: fufft_amd/_binding.so is not built", file=sys.stderr)
+        return None
     out = PKG / "_binding.so"
     tmp = out.with_suffix(".so.tmp")
     includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"]]
