@@ -54,6 +54,17 @@ bool matrix_ok(int type, int64_t ld, int64_t rows, int64_t k)
 {
    return type_ok(type) && size_ok(rows) && size_ok(k) && size_ok(ld) && (rows <= 1 || ld >= k) && volume_ok(rows, ld, 4);
 }
+// Two matrices of `rows` rows that share no byte: far from each other, or columns of one array, the rows
+// of each in the gaps of the other's.
+bool matrices_apart(const Span& a, int64_t pitch_a, int64_t width_a, const Span& b, int64_t pitch_b, int64_t width_b,
+                    int64_t rows)
+{
+   if(disjoint(a, b)) return true;
+   if(rows <= 1 || pitch_a != pitch_b) return false;
+   const int64_t by = static_cast<const char*>(b.p) - static_cast<const char*>(a.p);
+   const int64_t from = (by % pitch_a + pitch_a) % pitch_a;     // b's first byte in a row of a
+   return from >= width_a && from + width_b <= pitch_a;
+}
 Span codes_of(const void* p, int64_t rows, int64_t k) { return {p, rows * (padded(k) / 2)}; }
 Span scales_of(const void* p, int64_t rows, int64_t k) { return {p, rows * (padded(k) / 32)}; }
 
@@ -166,12 +177,14 @@ int fufft_mx4_linear(const void* x, int x_type, int64_t ldx, const void* w, cons
    if(m == 0 || n == 0) return FUFFT_OK;
    const Span so = matrix(out, type, ld, m, n), sbias{bias, bias ? n * 4 : 0}, sx = matrix(x, x_type, ldx, m, k);
    const Span sw = codes_of(w, n, k), sws = scales_of(w_scales, n, k);
+   const int64_t xb = type_bytes(x_type), ob = type_bytes(type);
    FUFFT_MX4_CHECK(span_status(so, (uintptr_t)type_bytes(type)));
    FUFFT_MX4_CHECK(span_status(sx, (uintptr_t)type_bytes(x_type)));
    FUFFT_MX4_CHECK(span_status(sw, 16));
    FUFFT_MX4_CHECK(span_status(sws, 4));
    FUFFT_MX4_CHECK(span_status(sbias, 4));
-   if(!apart(so, {sx, sw, sws, sbias})) return FUFFT_ERR_INVALID;
+   if(!apart(so, {sw, sws, sbias}) || !matrices_apart(sx, ldx * xb, k * xb, so, ld * ob, n * ob, m))
+      return FUFFT_ERR_INVALID;
    MatmulParams p{};
    p.x = x;
    p.w = static_cast<const uint8_t*>(w);
