@@ -981,7 +981,8 @@ def mx4_cache_read(codes, scales, pages, lens, out, order: str = "tokens", strea
 def mx4_cache_conv(codes, scales, pages, lens, taps, out, work=None, stream=None) -> None:
     """out (batch, channels) = the causal convolution with taps (count, channels) at every
     sequence's last token, read from the cache.  work: fp32 (splits, batch, channels); the
-    taps are split over at most that many workgroups.  None is allowed for fp32 results."""
+    taps are split over at most that many workgroups (about 256 / (batch * ceil(channels / 256))
+    are as many as help).  None is allowed for fp32 results."""
     if _native(out):
         gpu = _current_device()
         status = _binding.cache_conv(codes, scales, pages, lens, taps, out, work, _handle(stream, gpu), gpu)
