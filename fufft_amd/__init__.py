@@ -14,6 +14,7 @@ the library's dependency to that same copy).
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import re
 import warnings
 from pathlib import Path
@@ -876,6 +877,7 @@ def mx4_matmul(a, a_scales, b, b_scales, out, k: int, bias=None, stream=None) ->
         if status is not None:
             return check(status, "fufft_mx4_matmul")
     kind, ld, m, n = _matrix(out, "out")
+    k = operator.index(k)
     pa, pas = _blocks(a, a_scales, "a", m, k)
     pb, pbs = _blocks(b, b_scales, "b", n, k)
     pbias = _bias(bias, n)

@@ -36,3 +36,23 @@ def test_same_without_the_binding(dev, monkeypatch):
     monkeypatch.setattr(ff, "_binding", None)
     for got, ref in zip(every_call(torch, ff, dev), want):
         assert torch.equal(got, ref)
+
+
+def test_any_integer_as_k(dev, monkeypatch):
+    """numpy's and a 0-dimensional array's too, with the binding and without; a number that is none is refused."""
+    import numpy as np
+    import torch
+    import fufft_amd as ff
+    q, out = ff.mx4_empty(4, 200), torch.empty(4, 4, device=dev)
+    ff.mx4_quantize(torch.randn(4, 200, device=dev), *q)
+    ff.mx4_matmul(*q, *q, out, 200)
+    for binding in (ff._binding, None):
+        monkeypatch.setattr(ff, "_binding", binding)
+        for k in (np.int64(200), np.array(200)):
+            got = torch.empty(4, 4, device=dev)
+            ff.mx4_matmul(*q, *q, got, k)
+            torch.cuda.synchronize()
+            assert torch.equal(got, out)
+        for k in (200.0, "200", None):
+            with pytest.raises(TypeError):
+                ff.mx4_matmul(*q, *q, out, k)
