@@ -355,7 +355,7 @@ hipError_t conv_typed(const CacheParams& c, const T* taps, int64_t tap_count, fl
 {
    // Few sequences, or few channels: the wait for memory and the taps' bytes are the work, and
    // many wavefronts of one sequence, 4 channels a lane, serve them best (1 x 65536 x 1024, bf16
-   // taps: 33 us of a floor of 33; one sequence a group / two or four: 3 x 38104 x 62 20 / 38 us, 7 x 9546
+   // taps: 32 us, 5.3 TB/s; one sequence a group / two or four: 3 x 38104 x 62 20 / 38 us, 7 x 9546
    // x 46 12 / 21, 3 x 30000 x 768 28 / 45, but 8 x 4000 x 1000 23 / 19, 40 x 2000 x 100 21 / 15).
    // More: what scalar work a token costs counts, so 8 channels, and registers for four
    // sequences with 2 taps (24 x 8000 x 4096, fp32 taps: 4 x 2 taps 126 us, 4 x 4 148, 2 x 4 170;
