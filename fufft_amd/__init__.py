@@ -125,6 +125,13 @@ def _load() -> C.CDLL:
         "fufft_mx4_cache_write": ([vp, i32, i64, vp, i64, i64, vp, vp, i64, vp], i32),
         "fufft_mx4_cache_read": ([vp, vp, i64, i64, i64, vp, i64, vp, i64, i64, vp, i32, i32, vp], i32),
         "fufft_mx4_cache_conv": ([vp, vp, i64, i64, i64, vp, i64, vp, i64, vp, i32, i64, vp, i32, vp, i64, vp], i32),
+        "fufft_i8_padded": ([i64], i64),
+        "fufft_i8_quantize": ([vp, i32, i64, i64, i64, vp, vp, vp], i32),
+        "fufft_i8_dequantize": ([vp, vp, vp, i32, i64, i64, i64, vp], i32),
+        "fufft_i8_matmul": ([vp, vp, vp, vp, vp, vp, i32, i64, i64, i64, i64, vp], i32),
+        "fufft_rms_norm": ([vp, i32, i64, vp, i64, vp, i64, i32, vp, C.c_float, vp, i64, vp, vp, i64, i64, vp], i32),
+        "fufft_rms_norm_grad": ([vp, i32, i64, vp, i64, vp, i64, i32, vp, C.c_float, vp, i32, i64, vp, vp, i64, i64, i64,
+                                 vp], i32),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name, None)
@@ -178,6 +185,7 @@ if torch is not None:
         "words": (torch.int32,),
         "bytes": (torch.uint8,),
         "slots": (torch.int64,),
+        "codes": (torch.int8,),
     }
     # element types of the mx4 calls (FUFFT_F32, FUFFT_BF16, FUFFT_F16)
     _ELEMENT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -1009,3 +1017,116 @@ def mx4_cache_conv(codes, scales, pages, lens, taps, out, work=None, stream=None
             (work if splits else None, "work"))
     check(lib.fufft_mx4_cache_conv(pc, ps, count, page, channels, pt, width, pn, batch, taps.data_ptr(), t_kind,
                                    tap_count, out.data_ptr(), kind, pw, splits, _stream(stream)), "fufft_mx4_cache_conv")
+
+
+# ---- norms and 8-bit rows (i8) ----------------------------------------------------------
+# A row of k values in 8 bits is i8_padded(k) signed bytes and one fp32 scale: codes are int8
+# (rows, i8_padded(k)), or flat, scales fp32 (rows).
+
+def i8_padded(k: int) -> int:
+    """Bytes of a row of k values with its padding: the next multiple of 128."""
+    return (k + 127) // 128 * 128
+
+
+def i8_empty(rows: int, k: int, device="cuda"):
+    """Uninitialised (codes, scales) for `rows` rows of k values."""
+    return (torch.empty(rows, i8_padded(k), dtype=torch.int8, device=device),
+            torch.empty(rows, dtype=torch.float32, device=device))
+
+
+def _eight(codes, scales, name: str, rows: int, k: int):
+    """The addresses of `rows` 8-bit rows of k values, checked but for their device."""
+    width = i8_padded(k)
+    p = _array(codes, name, rows * width, "codes")
+    if codes.dim() > 1 and rows * width > 0 and codes.shape[-1] != width:
+        raise ValueError(f"{name}: has rows of {codes.shape[-1]} bytes, the call's have {width}")
+    return p, _array(scales, "scales" if name == "codes" else name + "_scales", 4 * rows, "real")
+
+
+def i8_quantize(x, codes, scales, stream=None) -> None:
+    """x (rows, k) as 8-bit rows: each row's scale is its largest magnitude over 127, its bytes
+    the nearest multiples."""
+    kind, ld, rows, k = _matrix(x, "x")
+    pc, ps = _eight(codes, scales, "codes", rows, k)
+    _on_gpu((x, "x"), (codes, "codes"), (scales, "scales"))
+    check(lib.fufft_i8_quantize(x.data_ptr(), kind, ld, rows, k, pc, ps, _stream(stream)), "fufft_i8_quantize")
+
+
+def i8_dequantize(codes, scales, out, stream=None) -> None:
+    """The values that 8-bit rows stand for, into out (rows, k)."""
+    kind, ld, rows, k = _matrix(out, "out")
+    pc, ps = _eight(codes, scales, "codes", rows, k)
+    _on_gpu((out, "out"), (codes, "codes"), (scales, "scales"))
+    check(lib.fufft_i8_dequantize(pc, ps, out.data_ptr(), kind, ld, rows, k, _stream(stream)), "fufft_i8_dequantize")
+
+
+def i8_matmul(a, a_scales, b, b_scales, out, k: int, bias=None, stream=None) -> None:
+    """out (m, n) = a b^T + bias: a is m 8-bit rows of k values (tokens), b n (channels), bias
+    fp32.  The integer sum is exact; k goes up to 131071."""
+    kind, ld, m, n = _matrix(out, "out")
+    k = operator.index(k)
+    pa, pas = _eight(a, a_scales, "a", m, k)
+    pb, pbs = _eight(b, b_scales, "b", n, k)
+    pbias = _bias(bias, n)
+    _on_gpu((out, "out"), (a, "a"), (a_scales, "a_scales"), (b, "b"), (b_scales, "b_scales"), (bias, "bias"))
+    check(lib.fufft_i8_matmul(pa, pas, pb, pbs, pbias, out.data_ptr(), kind, ld, m, n, k, _stream(stream)),
+          "fufft_i8_matmul")
+
+
+def _like(x, name: str, rows: int, k: int, kinds):
+    """(address, leading dimension, type) of a matrix of rows x k in one of the types, or zeros for None."""
+    if x is None:
+        return None, 0, None
+    kind, ld, r, c = _matrix(x, name)
+    if (r, c) != (rows, k):
+        raise ValueError(f"{name}: is {r} x {c}, the call's rows are {rows} x {k}")
+    if kind not in kinds:
+        raise ValueError(f"{name}: dtype {x.dtype} does not go with the call's")
+    return x.data_ptr(), ld, kind
+
+
+def rms_norm(x, weight=None, out=None, *, codes=None, scales=None, residual=None, total=None, eps: float = 1e-6,
+             stream=None) -> None:
+    """y = h weight / sqrt(mean(h^2) + eps) along rows, h = x + residual: into out (x's type),
+    as 8-bit rows into codes and scales, or both.  total takes h, in residual's type (x's or
+    fp32), and may be residual itself, or x; out may be x.  weight: fp32, None: ones."""
+    kind, ldx, rows, k = _matrix(x, "x")
+    pr, ldr, rk = _like(residual, "residual", rows, k, (kind, 0))
+    pt, ldt, tk = _like(total, "total", rows, k, (kind, 0) if rk is None else (rk,))
+    po, ldo, _ = _like(out, "out", rows, k, (kind,))
+    sum_kind = rk if rk is not None else tk if tk is not None else kind
+    pc = ps = None
+    if codes is not None or scales is not None:
+        pc, ps = _eight(codes, scales, "codes", rows, k)
+    elif out is None:
+        raise ValueError("rms_norm: neither out nor codes and scales are asked for")
+    pw = None if weight is None else _array(weight, "weight", 4 * k, "real")
+    _on_gpu((x, "x"), (weight, "weight"), (out, "out"), (codes, "codes"), (scales, "scales"), (residual, "residual"),
+            (total, "total"))
+    check(lib.fufft_rms_norm(x.data_ptr(), kind, ldx, pr, ldr, pt, ldt, sum_kind, pw, eps, po, ldo, pc, ps, rows, k,
+                             _stream(stream)), "fufft_rms_norm")
+
+
+def rms_norm_grad(dy, h, weight, dx, dweight=None, work=None, *, dtotal=None, eps: float = 1e-6, stream=None) -> None:
+    """Gradients of rms_norm's y: dx (that of x and of the residual), with dtotal, the gradient that
+    reaches h along the residual, added; dweight (fp32).  h is rms_norm's total, or x where there was
+    no residual.  dx is of dy's type or h's, and may be dy or dtotal.  work: fp32 (splits, k), needed
+    for dweight; 512 splits are as many as help."""
+    kind, ldy, rows, k = _matrix(dy, "dy")
+    ph, ldh, hk = _like(h, "h", rows, k, (kind, 0))
+    if ph is None:
+        raise TypeError("h: expected a torch tensor in GPU memory, got NoneType")
+    pt, ldt, _ = _like(dtotal, "dtotal", rows, k, (hk,))
+    px, ldx, xk = _like(dx, "dx", rows, k, (kind, hk))
+    if px is None and xk is None:
+        raise TypeError("dx: expected a torch tensor in GPU memory, got NoneType")
+    pw = None if weight is None else _array(weight, "weight", 4 * k, "real")
+    pd = None if dweight is None else _array(dweight, "dweight", 4 * k, "real")
+    splits = 0 if work is None or dweight is None or k == 0 else work.numel() // k
+    if dweight is not None and splits == 0 and k > 0:
+        raise ValueError("work: dweight needs a workspace of one split at least")
+    pk = None if splits == 0 else _array(work, "work", 4 * splits * k, "real")
+    _on_gpu((dy, "dy"), (h, "h"), (weight, "weight"), (dx, "dx"), (dweight, "dweight"), (work if splits else None, "work"),
+            (dtotal, "dtotal"))
+    check(lib.fufft_rms_norm_grad(dy.data_ptr(), kind, ldy, ph, ldh, pt, ldt, hk, pw, eps, dx.data_ptr(), xk, ldx, pd, pk,
+                                  splits, rows, k, _stream(stream)), "fufft_rms_norm_grad")

@@ -1,0 +1,644 @@
+// Root-mean-square norm with the residual's sum and 8-bit rows, its gradients, and the way
+// to 8-bit rows and back.
+//
+//   h = x + residual      r = 1 / sqrt(mean(h^2) + eps)      y = h r w
+//   8 bits: scale = max|y| / 127, code = the integer nearest to 127 y / max|y|, ties to even
+//   dx = r (w dy - n mean(w dy n)) + dtotal,   n = r h;      dw = sum over rows of dy n
+//
+// Rows are held in registers between reading and writing, a wavefront, 4 or 16 of them to a row,
+// so that each byte crosses memory once: every call here is bound by its bytes.
+#include "layer_internal.hpp"
+#include "mx4_device.hpp"
+
+namespace fufft {
+namespace layer {
+
+namespace {
+
+using mx4::bf16;
+using mx4::dpp;
+using mx4::f16;
+using mx4::load8;
+using mx4::magnitude;
+using mx4::store8;
+using mx4::u32x2;
+using mx4::umax;
+
+// eight consecutive elements as they are in memory, at the element's alignment
+template<class T> struct __attribute__((packed, aligned(sizeof(T)))) Eight { T e[8]; };
+
+// of a row of k elements from `col` on, zeros beyond its end
+template<class T>
+__device__ inline Eight<T> fetch8(const T* row, int64_t col, int64_t k)
+{
+   if(col + 8 <= k) return *reinterpret_cast<const Eight<T>*>(row + col);
+   Eight<T> v;
+#pragma unroll
+   for(int i = 0; i < 8; i++) v.e[i] = col + i < k ? row[col + i] : (T)0.0f;
+   return v;
+}
+template<class T>
+__device__ inline void put8(T* row, int64_t col, int64_t k, const float (&v)[8])
+{
+   if(col + 8 <= k) {
+      store8<T>(row + col, v);
+   } else {
+#pragma unroll
+      for(int i = 0; i < 8; i++)
+         if(col + i < k) row[col + i] = (T)v[i];
+   }
+}
+
+// ---- sums and maxima over the lanes of a row ----------------------------------------
+
+constexpr int kHalfMirror = 0x141, kMirror = 0x140;     // within 8 and 16 lanes
+
+__device__ inline float lane_value(float v, int lane)
+{
+   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+// the sum over the 64 lanes, the same in all of them: within rows of 16 by DPP, then the four rows
+__device__ inline float wave_sum(float v)
+{
+   v += __uint_as_float(dpp<mx4::kQuadSwap1>(__float_as_uint(v)));
+   v += __uint_as_float(dpp<mx4::kQuadSwap2>(__float_as_uint(v)));
+   v += __uint_as_float(dpp<kHalfMirror>(__float_as_uint(v)));
+   v += __uint_as_float(dpp<kMirror>(__float_as_uint(v)));
+   return (lane_value(v, 0) + lane_value(v, 16)) + (lane_value(v, 32) + lane_value(v, 48));
+}
+__device__ inline uint32_t wave_max(uint32_t v)
+{
+   v = umax(v, dpp<mx4::kQuadSwap1>(v));
+   v = umax(v, dpp<mx4::kQuadSwap2>(v));
+   v = umax(v, dpp<kHalfMirror>(v));
+   v = umax(v, dpp<kMirror>(v));
+   const uint32_t a = umax(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
+   return umax(a, umax(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+
+// Over LANES lanes; `turn` counts a row's uses of the exchange, which has two sides so that
+// one barrier a use is enough.
+template<int LANES>
+__device__ inline float row_sum(float v, uint32_t (&side)[2][16], int& turn)
+{
+   v = wave_sum(v);
+   if constexpr(LANES == 64) return v;
+   uint32_t* const at = side[turn++ & 1];
+   if((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = __float_as_uint(v);
+   __syncthreads();
+   float s = 0.0f;
+#pragma unroll
+   for(int w = 0; w < LANES / 64; w++) s += __uint_as_float(at[w]);
+   return s;
+}
+template<int LANES>
+__device__ inline uint32_t row_max(uint32_t v, uint32_t (&side)[2][16], int& turn)
+{
+   v = wave_max(v);
+   if constexpr(LANES == 64) return v;
+   uint32_t* const at = side[turn++ & 1];
+   if((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
+   __syncthreads();
+   uint32_t m = 0;
+#pragma unroll
+   for(int w = 0; w < LANES / 64; w++) m = umax(m, at[w]);
+   return m;
+}
+
+// Factors of a row: n = h * c * r.  c is 1 but where squares of h leave fp32's range, upwards, or
+// downwards with an eps that does not hide it: the sum is then taken again of h * c.
+struct Factors {
+   float c, r;
+};
+__device__ inline float squares(const float (&h)[8], float c)
+{
+   float ss = 0.0f;
+#pragma unroll
+   for(int i = 0; i < 8; i++) ss += (h[i] * c) * (h[i] * c);
+   return ss;
+}
+// part(c): the lane's share of the sum of (h c)^2
+template<int LANES, class F>
+__device__ inline Factors factors_from(F part, int64_t k, float eps, uint32_t (&side)[2][16], int& turn)
+{
+   float c = 1.0f, ss = row_sum<LANES>(part(c), side, turn);
+   const bool large = !(ss < __builtin_inff()), small = ss < 0x1p-60f && eps < 0x1p-60f;
+   if(large || small) {                 // the same in all lanes of the row
+      c = large ? 0x1p-80f : 0x1p+80f;
+      ss = row_sum<LANES>(part(c), side, turn);
+   }
+   return {c, 1.0f / sqrtf(ss / (float)k + (eps * c) * c)};
+}
+template<int LANES, int V>
+__device__ inline Factors factors_of(const float (&h)[V][8], int64_t k, float eps, uint32_t (&side)[2][16], int& turn)
+{
+   return factors_from<LANES>([&](float c) {
+      float ss = 0.0f;
+#pragma unroll
+      for(int v = 0; v < V; v++) ss += squares(h[v], c);
+      return ss;
+   }, k, eps, side, turn);
+}
+
+// ---- eight bits ---------------------------------------------------------------------------
+
+// What makes codes of a row's values: y * up * inv is 127 y / max|y| to within 2^-22 of
+// itself.  up lifts rows whose reciprocal would overflow.
+struct Step {
+   float  up, inv;
+   double top;        // max|y| * up
+};
+__device__ inline Step step_of(uint32_t top_bits)
+{
+   const float top = __uint_as_float(top_bits), up = top < 0x1p-100f ? 0x1p+100f : 1.0f;
+   return {up, top_bits ? 127.0f / (top * up) : 0.0f, (double)(top * up)};
+}
+// Eight codes.  Where the product is so near to half-way between two integers that its own
+// error could decide, the exact comparison does: 254 |y| against (2 m + 1) max|y|, which
+// fp64 holds.  (Half of a row's largest magnitude is half-way: 16-bit rows meet it.)
+__device__ inline u32x2 codes8(const float (&y)[8], const Step& s)
+{
+   int   n[8];
+   float q[8];
+   bool  near = false;
+#pragma unroll
+   for(int i = 0; i < 8; i++) {
+      q[i] = y[i] * s.up * s.inv;
+      const float whole = rintf(q[i]);
+      n[i] = (int)whole;
+      near |= fabsf(q[i] - whole) > 0.49997f;
+   }
+   if(near) {
+#pragma unroll
+      for(int i = 0; i < 8; i++) {
+         const float a = fabsf(q[i]), low = floorf(a);
+         if(fabsf(a - low - 0.5f) < 0.00004f) {
+            const int    m = (int)low;
+            const double twice = 254.0 * (double)fabsf(y[i] * s.up), half = (double)(2 * m + 1) * s.top;
+            const int    c = twice > half || (twice == half && (m & 1)) ? m + 1 : m;
+            n[i] = q[i] < 0.0f ? -c : c;
+         }
+      }
+   }
+   u32x2 w = {0, 0};
+#pragma unroll
+   for(int i = 0; i < 8; i++) w[i / 4] |= ((uint32_t)n[i] & 255u) << (8 * (i % 4));
+   return w;
+}
+
+// ---- the norm, and rows to 8 bits (NORM false: y = x) -----------------------------------
+//
+// LANES lanes have a row, V vectors of 8 elements each; a workgroup of 256 has 4 rows at 64.
+template<class X, class S, int LANES, int V, bool NORM>
+__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES)
+norm_rows(NormParams p, int64_t kp)
+{
+   __shared__ uint32_t side[2][16];
+   constexpr int PER = LANES < 256 ? 256 / LANES : 1;
+   const int lane = threadIdx.x % LANES;
+   const int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
+   if(row >= p.rows) return;                     // whole wavefronts; with more lanes a row, never
+   const X* const x = static_cast<const X*>(p.x) + row * p.ldx;
+   int turn = 0;
+   float h[V][8];
+   {
+      Eight<X> a[V];
+#pragma unroll
+      for(int v = 0; v < V; v++) a[v] = fetch8<X>(x, (int64_t)(v * LANES + lane) * 8, p.k);
+      if(NORM && p.residual) {
+         const S* const res = static_cast<const S*>(p.residual) + row * p.ldr;
+         Eight<S> b[V];
+#pragma unroll
+         for(int v = 0; v < V; v++) b[v] = fetch8<S>(res, (int64_t)(v * LANES + lane) * 8, p.k);
+#pragma unroll
+         for(int v = 0; v < V; v++)
+#pragma unroll
+            for(int i = 0; i < 8; i++) h[v][i] = (float)a[v].e[i] + (float)b[v].e[i];
+      } else {
+#pragma unroll
+         for(int v = 0; v < V; v++)
+#pragma unroll
+            for(int i = 0; i < 8; i++) h[v][i] = (float)a[v].e[i];
+      }
+   }
+   if constexpr(NORM) {
+      const Factors f = factors_of<LANES, V>(h, p.k, p.eps, side, turn);
+      S* const total = p.total ? static_cast<S*>(p.total) + row * p.ldt : nullptr;
+      X* const out = p.out ? static_cast<X*>(p.out) + row * p.ldo : nullptr;
+#pragma unroll
+      for(int v = 0; v < V; v++) {
+         const int64_t col = (int64_t)(v * LANES + lane) * 8;
+         if(total) put8<S>(total, col, p.k, h[v]);
+         Eight<float> w;
+         if(p.weight) w = fetch8<float>(p.weight, col, p.k);
+#pragma unroll
+         for(int i = 0; i < 8; i++) {
+            h[v][i] = h[v][i] * f.c * f.r;
+            if(p.weight) h[v][i] *= w.e[i];
+         }
+         if(out) put8<X>(out, col, p.k, h[v]);
+      }
+      if(!p.codes) return;
+   }
+   uint32_t top = 0;
+#pragma unroll
+   for(int v = 0; v < V; v++)
+#pragma unroll
+      for(int i = 0; i < 8; i++) top = umax(top, magnitude(h[v][i]));      // values beyond the end are zeros
+   top = row_max<LANES>(top, side, turn);
+   const bool finite = top < 0x7f800000u;
+   if(lane == 0) p.scales[row] = finite ? __uint_as_float(top) / 127.0f : __builtin_nanf("");
+   const Step step = step_of(finite ? top : 0);
+   int8_t* const codes = p.codes + row * kp;
+#pragma unroll
+   for(int v = 0; v < V; v++) {
+      const int64_t col = (int64_t)(v * LANES + lane) * 8;
+      if(col >= kp) break;
+      u32x2 c = {0, 0};
+      if(finite) c = codes8(h[v], step);
+      *reinterpret_cast<u32x2*>(codes + col) = c;
+   }
+}
+
+// Rows too long for registers: 1024 lanes go over their row once for the sum of squares, once for the
+// largest magnitude where codes are asked for, once to write.  What a lane writes it has read itself, in
+// the same trip, so total may still be residual and out x.
+template<class X, class S, bool NORM>
+__global__ void __launch_bounds__(1024)
+norm_long(NormParams p, int64_t kp)
+{
+   __shared__ uint32_t side[2][16];
+   const int64_t row = blockIdx.x;
+   const X* const x = static_cast<const X*>(p.x) + row * p.ldx;
+   const S* const res = NORM && p.residual ? static_cast<const S*>(p.residual) + row * p.ldr : nullptr;
+   int turn = 0;
+   auto sums = [&](int64_t col, float (&h)[8]) {
+      const Eight<X> a = fetch8<X>(x, col, p.k);
+#pragma unroll
+      for(int i = 0; i < 8; i++) h[i] = (float)a.e[i];
+      if(res) {
+         const Eight<S> b = fetch8<S>(res, col, p.k);
+#pragma unroll
+         for(int i = 0; i < 8; i++) h[i] += (float)b.e[i];
+      }
+   };
+   Factors f{1.0f, 1.0f};
+   if constexpr(NORM)
+      f = factors_from<1024>([&](float c) {
+         float ss = 0.0f;
+         for(int64_t col = threadIdx.x * 8; col < p.k; col += 8192) {
+            float h[8];
+            sums(col, h);
+            ss += squares(h, c);
+         }
+         return ss;
+      }, p.k, p.eps, side, turn);
+   auto normed = [&](int64_t col, float (&h)[8]) {
+      if(!NORM) return;
+      Eight<float> w;
+      if(p.weight) w = fetch8<float>(p.weight, col, p.k);
+#pragma unroll
+      for(int i = 0; i < 8; i++) {
+         h[i] = h[i] * f.c * f.r;
+         if(p.weight) h[i] *= w.e[i];
+      }
+   };
+   uint32_t top = 0;
+   if(!NORM || p.codes) {
+      for(int64_t col = threadIdx.x * 8; col < p.k; col += 8192) {
+         float h[8];
+         sums(col, h);
+         normed(col, h);
+#pragma unroll
+         for(int i = 0; i < 8; i++) top = umax(top, magnitude(h[i]));
+      }
+      top = row_max<1024>(top, side, turn);
+   }
+   const bool finite = top < 0x7f800000u;
+   const Step step = step_of(finite ? top : 0);
+   if(p.codes && threadIdx.x == 0) p.scales[row] = finite ? __uint_as_float(top) / 127.0f : __builtin_nanf("");
+   for(int64_t col = threadIdx.x * 8; col < kp; col += 8192) {
+      float h[8];
+      sums(col, h);                                // zeros from k on
+      if(NORM && p.total) put8<S>(static_cast<S*>(p.total) + row * p.ldt, col, p.k, h);
+      normed(col, h);
+      if(NORM && p.out) put8<X>(static_cast<X*>(p.out) + row * p.ldo, col, p.k, h);
+      if(!p.codes) continue;
+      u32x2 c = {0, 0};
+      if(finite) c = codes8(h, step);
+      *reinterpret_cast<u32x2*>(p.codes + row * kp + col) = c;
+   }
+}
+
+// one lane, eight values; a row of lanes as long as a padded row
+template<class O>
+__global__ void __launch_bounds__(256)
+dequantize_rows(const int8_t* codes, const float* scales, O* out, int64_t ld, int64_t first, int64_t rows, int64_t k,
+                int64_t kp)
+{
+   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = kp / 8;
+   const int64_t row = first + i / per, col = i % per * 8;
+   if(row >= rows || col >= k) return;
+   const u32x2 c = *reinterpret_cast<const u32x2*>(codes + row * kp + col);
+   const float s = scales[row];
+   float v[8];
+#pragma unroll
+   for(int j = 0; j < 8; j++) v[j] = (float)(int8_t)(c[j / 4] >> (8 * (j % 4))) * s;
+   put8<O>(out + row * ld, col, k, v);
+}
+
+// ---- the norm's gradients ----------------------------------------------------------------
+//
+// Workgroup i of `groups` has rows i, i + groups, .. (times PER), and the sums of its rows'
+// part of dweight in registers; the next row's values are on their way while one is summed.
+template<class D, class S, class O, int LANES, int V>
+__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES)
+norm_grad_rows(NormGradParams p, int64_t groups)
+{
+   __shared__ uint32_t side[2][16];
+   constexpr int PER = LANES < 256 ? 256 / LANES : 1;
+   const int lane = threadIdx.x % LANES;
+   const int64_t step = groups * PER;
+   int turn = 0;
+   Eight<D> dy[V];
+   Eight<S> hh[V], dt[V];
+   auto fetch = [&](int64_t row) {
+#pragma unroll
+      for(int v = 0; v < V; v++) {
+         const int64_t col = (int64_t)(v * LANES + lane) * 8;
+         dy[v] = fetch8<D>(static_cast<const D*>(p.dy) + row * p.ldy, col, p.k);
+         hh[v] = fetch8<S>(static_cast<const S*>(p.h) + row * p.ldh, col, p.k);
+         if(p.dtotal) dt[v] = fetch8<S>(static_cast<const S*>(p.dtotal) + row * p.ldt, col, p.k);
+      }
+   };
+   float dw[V][8] = {};
+   int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
+   if(row < p.rows) fetch(row);
+   for(; row < p.rows; row += step) {
+      float g[V][8], h[V][8], through[V][8];
+#pragma unroll
+      for(int v = 0; v < V; v++)
+#pragma unroll
+         for(int i = 0; i < 8; i++) {
+            g[v][i] = (float)dy[v].e[i];
+            h[v][i] = (float)hh[v].e[i];
+            through[v][i] = p.dtotal ? (float)dt[v].e[i] : 0.0f;
+         }
+      if(row + step < p.rows) fetch(row + step);
+      const Factors f = factors_of<LANES, V>(h, p.k, p.eps, side, turn);
+      float mean = 0.0f;
+#pragma unroll
+      for(int v = 0; v < V; v++) {
+         const int64_t col = (int64_t)(v * LANES + lane) * 8;
+         Eight<float> w;
+         if(p.weight) w = fetch8<float>(p.weight, col, p.k);
+#pragma unroll
+         for(int i = 0; i < 8; i++) {
+            h[v][i] = h[v][i] * f.c * f.r;
+            dw[v][i] += g[v][i] * h[v][i];
+            if(p.weight) g[v][i] *= w.e[i];
+            mean += g[v][i] * h[v][i];
+         }
+      }
+      mean = row_sum<LANES>(mean, side, turn) / (float)p.k;
+      O* const dx = static_cast<O*>(p.dx) + row * p.ldx;
+#pragma unroll
+      for(int v = 0; v < V; v++) {
+         float o[8];
+#pragma unroll
+         for(int i = 0; i < 8; i++) o[i] = (g[v][i] - h[v][i] * mean) * f.r * f.c + through[v][i];
+         put8<O>(dx, (int64_t)(v * LANES + lane) * 8, p.k, o);
+      }
+   }
+   if(!p.dweight) return;
+   float* const work = p.work + (int64_t)blockIdx.x * p.k;
+   if constexpr(PER > 1) {
+      // the wavefronts' sums, in their order
+      __shared__ float join[PER][V * LANES * 8];
+#pragma unroll
+      for(int v = 0; v < V; v++)
+#pragma unroll
+         for(int i = 0; i < 8; i++) join[threadIdx.x / LANES][(v * 8 + i) * LANES + lane] = dw[v][i];
+      __syncthreads();
+      for(int i = threadIdx.x; i < V * 8 * LANES; i += 256) {
+         const int64_t col = (int64_t)(i / (8 * LANES) * LANES + i % LANES) * 8 + i / LANES % 8;
+         float s = 0.0f;
+#pragma unroll
+         for(int w = 0; w < PER; w++) s += join[w][i];
+         if(col < p.k) work[col] = s;
+      }
+   } else {
+#pragma unroll
+      for(int v = 0; v < V; v++) put8<float>(work, (int64_t)(v * LANES + lane) * 8, p.k, dw[v]);
+   }
+}
+
+// Rows too long for registers: three trips over a row by 1024 lanes; dweight's sums are in the workgroup's
+// row of the workspace, every element in the hands of one lane.
+template<class D, class S, class O>
+__global__ void __launch_bounds__(1024)
+norm_grad_long(NormGradParams p, int64_t groups)
+{
+   __shared__ uint32_t side[2][16];
+   int turn = 0;
+   float* const work = p.dweight ? p.work + (int64_t)blockIdx.x * p.k : nullptr;
+   for(int64_t row = blockIdx.x; row < p.rows; row += groups) {
+      const D* const dy = static_cast<const D*>(p.dy) + row * p.ldy;
+      const S* const hh = static_cast<const S*>(p.h) + row * p.ldh;
+      const Factors f = factors_from<1024>([&](float c) {
+         float ss = 0.0f;
+         for(int64_t col = threadIdx.x * 8; col < p.k; col += 8192) {
+            const Eight<S> a = fetch8<S>(hh, col, p.k);
+            float h[8];
+#pragma unroll
+            for(int i = 0; i < 8; i++) h[i] = (float)a.e[i];
+            ss += squares(h, c);
+         }
+         return ss;
+      }, p.k, p.eps, side, turn);
+      // n into h, w dy into g, dy into plain
+      auto values = [&](int64_t col, float (&h)[8], float (&g)[8], float (&plain)[8]) {
+         const Eight<S> a = fetch8<S>(hh, col, p.k);
+         const Eight<D> b = fetch8<D>(dy, col, p.k);
+         Eight<float> w;
+         if(p.weight) w = fetch8<float>(p.weight, col, p.k);
+#pragma unroll
+         for(int i = 0; i < 8; i++) {
+            h[i] = (float)a.e[i] * f.c * f.r;
+            plain[i] = (float)b.e[i];
+            g[i] = p.weight ? plain[i] * w.e[i] : plain[i];
+         }
+      };
+      float mean = 0.0f;
+      for(int64_t col = threadIdx.x * 8; col < p.k; col += 8192) {
+         float h[8], g[8], plain[8];
+         values(col, h, g, plain);
+#pragma unroll
+         for(int i = 0; i < 8; i++) mean += g[i] * h[i];
+      }
+      mean = row_sum<1024>(mean, side, turn) / (float)p.k;
+      const S* const dt = p.dtotal ? static_cast<const S*>(p.dtotal) + row * p.ldt : nullptr;
+      for(int64_t col = threadIdx.x * 8; col < p.k; col += 8192) {
+         float h[8], g[8], plain[8];
+         values(col, h, g, plain);
+         Eight<S> t;
+         if(dt) t = fetch8<S>(dt, col, p.k);
+         if(work) {
+            float sum[8];
+            const Eight<float> before = fetch8<float>(work, col, p.k);
+#pragma unroll
+            for(int i = 0; i < 8; i++) sum[i] = (row == blockIdx.x ? 0.0f : before.e[i]) + plain[i] * h[i];
+            put8<float>(work, col, p.k, sum);
+         }
+#pragma unroll
+         for(int i = 0; i < 8; i++) g[i] = (g[i] - h[i] * mean) * f.r * f.c + (dt ? (float)t.e[i] : 0.0f);
+         put8<O>(static_cast<O*>(p.dx) + row * p.ldx, col, p.k, g);
+      }
+   }
+}
+
+// dweight = the sum of `splits` rows of k: 32 columns a workgroup, 32 runs of rows, joined in order
+__global__ void __launch_bounds__(1024)
+join_weight(const float* work, float* dweight, int64_t splits, int64_t k)
+{
+   __shared__ float part[32][33];
+   const int c = threadIdx.x % 32, g = threadIdx.x / 32;
+   const int64_t col = (int64_t)blockIdx.x * 32 + c;
+   float s = 0.0f;
+   if(col < k)
+#pragma unroll 8
+      for(int64_t r = g; r < splits; r += 32) s += work[r * k + col];
+   part[g][c] = s;
+   __syncthreads();
+   if(g == 0 && col < k) {
+      s = 0.0f;
+#pragma unroll
+      for(int i = 0; i < 32; i++) s += part[i][c];
+      dweight[col] = s;
+   }
+}
+
+// ---- launches --------------------------------------------------------------------------------
+
+template<class X, class S, int LANES, int V, bool NORM>
+hipError_t norm_shape(const NormParams& p, hipStream_t s)
+{
+   constexpr int PER = LANES < 256 ? 256 / LANES : 1, BLOCK = LANES < 256 ? 256 : LANES;
+   const int64_t groups = (p.rows + PER - 1) / PER;
+   if(!grid_ok(groups, BLOCK)) return kTooLarge;
+   norm_rows<X, S, LANES, V, NORM><<<(unsigned)groups, BLOCK, 0, s>>>(p, padded(p.k));
+   return hipGetLastError();
+}
+
+// the lanes and vectors for a width
+template<class X, class S, bool NORM>
+hipError_t norm_typed(const NormParams& p, hipStream_t s)
+{
+   if(p.k <= 512)   return norm_shape<X, S, 64, 1, NORM>(p, s);
+   if(p.k <= 1024)  return norm_shape<X, S, 64, 2, NORM>(p, s);
+   if(p.k <= 2048)  return norm_shape<X, S, 256, 1, NORM>(p, s);
+   if(p.k <= 4096)  return norm_shape<X, S, 256, 2, NORM>(p, s);
+   if(p.k <= 8192)  return norm_shape<X, S, 256, 4, NORM>(p, s);
+   if(p.k <= 16384) return norm_shape<X, S, 1024, 2, NORM>(p, s);
+   if(p.k <= 32768) return norm_shape<X, S, 1024, 4, NORM>(p, s);
+   if(!grid_ok(p.rows, 1024)) return kTooLarge;
+   norm_long<X, S, NORM><<<(unsigned)p.rows, 1024, 0, s>>>(p, padded(p.k));
+   return hipGetLastError();
+}
+
+template<class O>
+hipError_t dequantize_typed(const int8_t* codes, const float* scales, void* out, int64_t ld, int64_t rows, int64_t k,
+                            hipStream_t s)
+{
+   const int64_t kp = padded(k), per = kp / 8;
+   const int64_t most = (int64_t)1 << 31;               // lanes of a launch, whole rows of them
+   const int64_t each = most / per > 0 ? most / per : 1;
+   if(!grid_ok((per + 255) / 256, 256)) return kTooLarge;
+   for(int64_t first = 0; first < rows; first += each) {
+      const int64_t n = rows - first < each ? rows - first : each;
+      dequantize_rows<O><<<(unsigned)((n * per + 255) / 256), 256, 0, s>>>(codes, scales, static_cast<O*>(out), ld, first,
+                                                                          first + n, k, kp);
+      const hipError_t e = hipGetLastError();
+      if(e != hipSuccess) return e;
+   }
+   return hipSuccess;
+}
+
+// LANES 0: the kernel of long rows
+template<class D, class S, class O, int LANES, int V>
+hipError_t grad_shape(const NormGradParams& p, hipStream_t s)
+{
+   constexpr int PER = LANES == 64 ? 4 : 1, BLOCK = LANES == 64 ? 256 : LANES;
+   int64_t groups = (p.rows + PER - 1) / PER;
+   if(p.dweight) groups = groups < p.splits ? groups : p.splits;
+   if(groups > 2048) groups = 2048;
+   if(groups > 0) {                                     // no rows: dweight is zero
+      if constexpr(LANES == 0) norm_grad_long<D, S, O><<<(unsigned)groups, 1024, 0, s>>>(p, groups);
+      else                     norm_grad_rows<D, S, O, LANES, V><<<(unsigned)groups, BLOCK, 0, s>>>(p, groups);
+      const hipError_t e = hipGetLastError();
+      if(e != hipSuccess) return e;
+   }
+   if(!p.dweight) return hipSuccess;
+   if(!grid_ok((p.k + 31) / 32, 1024)) return kTooLarge;
+   join_weight<<<(unsigned)((p.k + 31) / 32), 1024, 0, s>>>(p.work, p.dweight, groups, p.k);
+   return hipGetLastError();
+}
+
+template<class D, class S, class O>
+hipError_t grad_typed(const NormGradParams& p, hipStream_t s)
+{
+   if(p.k <= 512)   return grad_shape<D, S, O, 64, 1>(p, s);
+   if(p.k <= 1024)  return grad_shape<D, S, O, 64, 2>(p, s);
+   if(p.k <= 2048)  return grad_shape<D, S, O, 256, 1>(p, s);
+   if(p.k <= 4096)  return grad_shape<D, S, O, 256, 2>(p, s);
+   if(p.k <= 8192)  return grad_shape<D, S, O, 512, 2>(p, s);
+   return grad_shape<D, S, O, 0, 0>(p, s);
+}
+
+}  // namespace
+
+hipError_t launch_rms_norm(const NormParams& p, hipStream_t s)
+{
+   const bool wide = p.sum_type == T_F32;
+   switch(p.type) {
+      case T_F32:  return norm_typed<float, float, true>(p, s);
+      case T_BF16: return wide ? norm_typed<bf16, float, true>(p, s) : norm_typed<bf16, bf16, true>(p, s);
+      default:     return wide ? norm_typed<f16, float, true>(p, s) : norm_typed<f16, f16, true>(p, s);
+   }
+}
+
+hipError_t launch_i8_quantize(const NormParams& p, hipStream_t s)
+{
+   switch(p.type) {
+      case T_F32:  return norm_typed<float, float, false>(p, s);
+      case T_BF16: return norm_typed<bf16, bf16, false>(p, s);
+      default:     return norm_typed<f16, f16, false>(p, s);
+   }
+}
+
+hipError_t launch_i8_dequantize(const int8_t* codes, const float* scales, void* out, int type, int64_t ld, int64_t rows,
+                                int64_t k, hipStream_t s)
+{
+   switch(type) {
+      case T_F32:  return dequantize_typed<float>(codes, scales, out, ld, rows, k, s);
+      case T_BF16: return dequantize_typed<bf16>(codes, scales, out, ld, rows, k, s);
+      default:     return dequantize_typed<f16>(codes, scales, out, ld, rows, k, s);
+   }
+}
+
+hipError_t launch_rms_norm_grad(const NormGradParams& p, hipStream_t s)
+{
+   const bool wide = p.sum_type == T_F32, wide_out = p.dx_type == T_F32;
+   switch(p.type) {
+      case T_F32: return grad_typed<float, float, float>(p, s);
+      case T_BF16:
+         if(!wide) return grad_typed<bf16, bf16, bf16>(p, s);
+         return wide_out ? grad_typed<bf16, float, float>(p, s) : grad_typed<bf16, float, bf16>(p, s);
+      default:
+         if(!wide) return grad_typed<f16, f16, f16>(p, s);
+         return wide_out ? grad_typed<f16, float, float>(p, s) : grad_typed<f16, float, f16>(p, s);
+   }
+}
+
+}  // namespace layer
+}  // namespace fufft

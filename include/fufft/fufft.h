@@ -585,6 +585,61 @@ int fufft_mx4_cache_conv(const void* codes, const uint8_t* scales, int64_t pages
                          int64_t tap_count, void* out, int type, float* work, int64_t splits,
                          void* stream);
 
+/* ---- norms and 8-bit rows --------------------------------------------------------------
+ * What stands around a sequence mixer in a model.  No reference counterpart.
+ *
+ * Element types, leading dimensions, alignment and sizes of zero are as in the 4-bit
+ * calls above.  Every sum, state and statistic is fp32 (integer sums int32), rounded
+ * once to the output's type.  Outputs share no byte with another buffer of the call, but for
+ * those named below that may be one of its inputs, the same address and strides.
+ * Sizes that no launch can hold are FUFFT_ERR_UNSUPPORTED.
+ *
+ * 8-bit rows: a row of k values is fufft_i8_padded(k) signed bytes (k up to a multiple of
+ * 128; the padding holds zeros, and the quantizing calls write them) and one fp32 scale.
+ * A byte stands for itself times the scale, which is the row's largest magnitude over
+ * 127; the byte is the nearest, ties to even, exactly.  A row with an infinity or NaN
+ * has the scale NaN and zero bytes.  Bytes are 16-byte aligned, rows without gaps. */
+int64_t fufft_i8_padded(int64_t k);
+int fufft_i8_quantize(const void* x, int type, int64_t ld, int64_t rows, int64_t k, void* codes,
+                      float* scales, void* stream);
+int fufft_i8_dequantize(const void* codes, const float* scales, void* out, int type, int64_t ld,
+                        int64_t rows, int64_t k, void* stream);
+/* out[i][j] = bias[j] + a_scales[i] b_scales[j] * sum over k of a[i][k] b[j][k]: a is m 8-bit
+ * rows (tokens), b n (channels), bias fp32 or NULL, out m x n.  The integer sum is exact:
+ * k beyond 131071, where it could leave 32 bits, is FUFFT_ERR_UNSUPPORTED.  Few rows of a (single
+ * tokens) take kernels of their own, bound by b's bytes. */
+int fufft_i8_matmul(const void* a, const float* a_scales, const void* b, const float* b_scales,
+                    const float* bias, void* out, int type, int64_t ld, int64_t m, int64_t n,
+                    int64_t k, void* stream);
+
+/* h = x + residual (residual NULL: x), y = h weight / sqrt(mean of h^2 + eps) along rows.
+ *   x          rows x k of `type`, leading dimension ldx;
+ *   residual   rows x k of `sum_type` (type, or FUFFT_F32), ldr; or NULL;
+ *   total      h rounded to sum_type, ldt; or NULL.  May be residual, or x (of that type);
+ *   weight     k fp32 values, or NULL: ones;
+ *   out        y of `type`, ldo, or NULL.  May be x;
+ *   codes, scales   y as 8-bit rows, or NULL (y is rounded once, to 8 bits).
+ * out, or codes and scales, or all three are given.  y is of the unrounded h.  eps >= 0,
+ * finite; a row of zeros gives zeros where eps > 0. */
+int fufft_rms_norm(const void* x, int type, int64_t ldx, const void* residual, int64_t ldr,
+                   void* total, int64_t ldt, int sum_type, const float* weight, float eps, void* out,
+                   int64_t ldo, void* codes, float* scales, int64_t rows, int64_t k, void* stream);
+/* The gradients of y with respect to h, dx = r (w dy - n mean(w dy n)) + dtotal with r =
+ * 1 / sqrt(mean of h^2 + eps) and n = r h, and to the weight, dweight = sum over rows of dy n.
+ *   dy         rows x k of `type`, ldy: y's gradient;
+ *   h          rows x k of `sum_type` (type, or FUFFT_F32), ldh: fufft_rms_norm's total, or its
+ *              x where there was no residual;
+ *   dtotal     rows x k of sum_type, ldt: the gradient that reaches h along the residual; NULL: none;
+ *   dx         rows x k of `dx_type` (type, or sum_type), ldx: the gradient of x and of the
+ *              residual.  May be dy, or dtotal (of that type);
+ *   dweight    k fp32 values, or NULL: not wanted;
+ *   work       fp32 space for `splits` x k partial sums of dweight, which are joined in a fixed
+ *              order; at least 1 split where dweight is given.  512 are as many as help. */
+int fufft_rms_norm_grad(const void* dy, int type, int64_t ldy, const void* h, int64_t ldh,
+                        const void* dtotal, int64_t ldt, int sum_type, const float* weight,
+                        float eps, void* dx, int dx_type, int64_t ldx, float* dweight, float* work,
+                        int64_t splits, int64_t rows, int64_t k, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

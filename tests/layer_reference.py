@@ -1,0 +1,104 @@
+"""Plain 64-bit forms of the norm, 8-bit and decaying-attention calls, from their definitions,
+and the bounds that fp32 arithmetic with one rounding at the end can keep.  CPU only."""
+import numpy as np
+
+EPS24 = 2.0 ** -24          # half a step of fp32, relative
+TYPES = ("f32", "bf16", "f16")
+
+
+def torch_type(name):
+    import torch
+    return {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[name]
+
+
+def typed(x, name, dev):
+    """x rounded to the type: the tensor on the GPU, and its values in 64 bits."""
+    import torch
+    t = torch.from_numpy(np.ascontiguousarray(x)).to(torch_type(name))
+    return t.to(dev), t.double().numpy()
+
+
+def with_stride(t, extra=5, offset=3):
+    """The same matrix as rows of a wider one, its first element `offset` elements in."""
+    import torch
+    rows, k = t.shape
+    wide = torch.full((rows * (k + extra) + offset,), float("nan"), dtype=t.dtype, device=t.device)
+    v = wide[offset:].view(rows, k + extra)[:, :k]
+    v.copy_(t)
+    return v
+
+
+def padded(k):
+    return -(-k // 128) * 128
+
+
+def inside(got, want, err):
+    """Whether every element of the tensor `got` is one that a value within err of `want` gives
+    when it is rounded to got's type (rounding keeps the order, so the ends tell)."""
+    import torch
+    err = err + 2.0 ** -126         # products below the smallest normal number may be anything that small
+    lo, hi = (torch.from_numpy(np.asarray(want + d, dtype=np.float64)).to(got.dtype).double().numpy() for d in (-err, err))
+    got = got.double().cpu().numpy()
+    return bool(np.all((got >= lo) & (got <= hi)))
+
+
+# ---- 8-bit rows ----------------------------------------------------------------------
+
+def quantize(x):
+    """(codes with padding, scales fp32) of the rows of x.  127 x / top is exact enough in 64 bits: x and
+    top have 24 bits, so what is not half-way between integers is at least 2^-33 from it."""
+    x = np.asarray(x, dtype=np.float64)
+    rows, k = x.shape
+    codes = np.zeros((rows, padded(k)), dtype=np.int8)
+    scales = np.zeros(rows, dtype=np.float32)
+    for r in range(rows):
+        top = np.max(np.abs(x[r])) if k else 0.0
+        if not np.isfinite(top):
+            scales[r] = np.nan
+        elif top > 0:
+            scales[r] = np.float32(top) / np.float32(127)
+            codes[r, :k] = np.rint(127 * x[r] / top).astype(np.int8)
+    return codes, scales
+
+
+def matmul(a, sa, b, sb, bias, k):
+    """(value, bound of fp32's error): the integer sum exact, made fp32, times each scale, plus the
+    bias: four roundings, three of them of the product."""
+    s = a.astype(np.int64)[:, :k] @ b.astype(np.int64)[:, :k].T
+    v = s * sa.astype(np.float64)[:, None] * sb.astype(np.float64)
+    out = v if bias is None else v + bias
+    return out, EPS24 * (3.001 * np.abs(v) + 1.001 * np.abs(out))
+
+
+# ---- norms -----------------------------------------------------------------------------
+
+# Roundings that the sum of a row's squares goes through at most: a lane adds up to 64 of them one
+# after the other, a wavefront's lanes 6 times, 16 wavefronts; and one for the square.  All terms are
+# positive, so the relative error of the sum is at most that many half steps, of its root half
+# of it; mean, eps, root and reciprocal add four, h itself one.
+CHAIN = 64 + 6 + 16 + 1
+ROOT = CHAIN / 2 + 5
+
+
+def norm(h, weight, eps):
+    """(y, bound of fp32's relative error before the rounding to the type)."""
+    h = np.asarray(h, dtype=np.float64)
+    y = h / np.sqrt((h * h).mean(1, keepdims=True) + eps)
+    return (y if weight is None else y * weight), (ROOT + 4) * EPS24
+
+
+def norm_grad(dy, h, weight, dtotal, eps):
+    """(dx, its bound, dweight, the sum of the magnitudes of its terms)."""
+    dy, h = np.asarray(dy, dtype=np.float64), np.asarray(h, dtype=np.float64)
+    k = h.shape[1]
+    r = 1 / np.sqrt((h * h).mean(1, keepdims=True) + eps)
+    n = h * r
+    g = dy if weight is None else dy * weight
+    dx = r * (g - n * (g * n).mean(1, keepdims=True))
+    # the mean: its terms are off by ROOT + 3 roundings, their sum by CHAIN; then n, r, and the products
+    err = EPS24 * ((ROOT + 6) * np.abs(r * g) + (CHAIN + 3 * ROOT + 12) * np.abs(r * n) * np.abs(g * n).sum(1, keepdims=True) / k)
+    if dtotal is not None:
+        dx = dx + dtotal
+        err = err + EPS24 * np.abs(dx)
+    terms = dy * n
+    return dx, err, terms.sum(0), np.abs(terms).sum(0)
