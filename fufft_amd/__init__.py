@@ -132,6 +132,12 @@ def _load() -> C.CDLL:
         "fufft_rms_norm": ([vp, i32, i64, vp, i64, vp, i64, i32, vp, C.c_float, vp, i64, vp, vp, i64, i64, vp], i32),
         "fufft_rms_norm_grad": ([vp, i32, i64, vp, i64, vp, i64, i32, vp, C.c_float, vp, i32, i64, vp, vp, i64, i64, i64,
                                  vp], i32),
+        "fufft_decay_attention": ([vp, vp, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, C.c_float, i64, i64, i64, i64, i64,
+                                   vp, i64, vp], i32),
+        "fufft_decay_attention_grad": ([vp, vp, vp, vp, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp,
+                                        C.c_float, i64, i64, i64, i64, i64, vp, i64, vp], i32),
+        "fufft_decay_attention_step": ([vp, vp, vp, vp, vp, vp, i32, vp, vp, vp, vp, i64, vp, C.c_float, i64, i64, i64, i64,
+                                        vp], i32),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name, None)
@@ -1130,3 +1136,126 @@ def rms_norm_grad(dy, h, weight, dx, dweight=None, work=None, *, dtotal=None, ep
             (dtotal, "dtotal"))
     check(lib.fufft_rms_norm_grad(dy.data_ptr(), kind, ldy, ph, ldh, pt, ldt, hk, pw, eps, dx.data_ptr(), xk, ldx, pd, pk,
                                   splits, rows, k, _stream(stream)), "fufft_rms_norm_grad")
+
+
+# ---- linear attention with a decay for each head ------------------------------------------
+# q, k (batch, tokens, heads, dk), v and out (batch, tokens, heads, dv) in one type (fp32, bf16, fp16), the
+# elements of a head adjacent and any strides otherwise (of an input 0 too); log_decay fp32 (heads),
+# <= 0; states fp32 (batch, heads, dk, dv), contiguous.
+
+class _Strides(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("token", C.c_int64), ("head", C.c_int64)]
+
+
+def _heads(x, name: str, shape, kind=None):
+    """(address, strides) of a tensor of (batch, tokens, heads, dim), or (batch, heads, dim) for one token,
+    checked but for its device."""
+    if torch is None or not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch tensor in GPU memory, got {type(x).__name__}")
+    have = _ELEMENT.get(x.dtype)
+    if have is None or (kind is not None and have != kind):
+        raise ValueError(f"{name}: dtype {x.dtype} " + ("does not go with q's" if have is not None else
+                         f"is not one of {', '.join(str(d) for d in _ELEMENT)}"))
+    if x.dim() != len(shape) or any(n is not None and m != n for m, n in zip(x.shape, shape)):
+        raise ValueError(f"{name}: expected {tuple('*' if n is None else n for n in shape)}, got {tuple(x.shape)}")
+    if x.shape[-1] > 1 and x.stride(-1) != 1:
+        raise ValueError(f"{name}: the elements of a head are not contiguous")
+    s = x.stride()
+    return x.data_ptr(), _Strides(s[0], s[1] if len(s) == 4 else 0, s[-2])
+
+
+def _states(x, name: str, shape):
+    if x is None:
+        return None
+    n = 1
+    for m in shape:
+        n *= m
+    p = _array(x, name, 4 * n, "real")
+    if x.dim() > 1 and tuple(x.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected {tuple(shape)}, got {tuple(x.shape)}")
+    return p
+
+
+def _splits(work, each: int):
+    """(address, splits) of a workspace of `each` values a split."""
+    n = 0 if work is None or each == 0 else work.numel() // each
+    return (None if n == 0 else _array(work, "work", 4 * n * each, "real")), n
+
+
+def decay_attention(q, k, v, log_decay, out, *, state=None, new_state=None, lens=None, work=None, scale: float = 1.0,
+                    stream=None) -> None:
+    """out[t] = scale q[t]^T S[t] with S[t] = exp(log_decay) S[t-1] + k[t] v[t]^T, of every sequence and head.
+    state: S before the first token, None: zero; new_state: S after the last one (may be state).
+    lens (int32, batch): tokens of each sequence; rows behind them are neither read nor written.
+    work: fp32, room for splits * batch * heads * dk * dv values; the tokens are split over at most that
+    many workgroups, and about 1024 / (batch * heads) splits are as many as help."""
+    pq, sq = _heads(q, "q", (None,) * 4)
+    kind = _ELEMENT[q.dtype]
+    batch, tokens, heads, dk = q.shape
+    pk, sk = _heads(k, "k", (batch, tokens, heads, dk), kind)
+    pv, sv = _heads(v, "v", (batch, tokens, heads, None), kind)
+    dv = v.shape[3]
+    po, so = _heads(out, "out", (batch, tokens, heads, dv), kind)
+    pd = _array(log_decay, "log_decay", 4 * heads, "real")
+    ps, pn = _states(state, "state", (batch, heads, dk, dv)), _states(new_state, "new_state", (batch, heads, dk, dv))
+    pl = None if lens is None else _array(lens, "lens", 4 * batch, "words")
+    pw, splits = _splits(work, batch * heads * dk * dv)
+    _on_gpu((q, "q"), (k, "k"), (v, "v"), (out, "out"), (log_decay, "log_decay"), (state, "state"), (new_state, "new_state"),
+            (lens, "lens"), (work if splits else None, "work"))
+    check(lib.fufft_decay_attention(pq, C.byref(sq), pk, C.byref(sk), pv, C.byref(sv), kind, pd, po, C.byref(so), ps, pn, pl,
+                                    scale, batch, tokens, heads, dk, dv, pw, splits, _stream(stream)), "fufft_decay_attention")
+
+
+def decay_attention_grad(dout, q, k, v, log_decay, dq, dk, dv, *, state=None, dnew_state=None, dstate=None, lens=None,
+                         work=None, scale: float = 1.0, stream=None) -> None:
+    """Gradients of decay_attention: dq, dk, dv of dout and of dnew_state (None: zero), and dstate
+    (None: not wanted).  state and lens are that call's; log_decay is a constant.  work: as there,
+    with room for three such sets of states."""
+    pq, sq = _heads(q, "q", (None,) * 4)
+    kind = _ELEMENT[q.dtype]
+    batch, tokens, heads, nk = q.shape
+    pk, sk = _heads(k, "k", (batch, tokens, heads, nk), kind)
+    pv, sv = _heads(v, "v", (batch, tokens, heads, None), kind)
+    nv = v.shape[3]
+    po, so = _heads(dout, "dout", (batch, tokens, heads, nv), kind)
+    gq, tq = _heads(dq, "dq", (batch, tokens, heads, nk), kind)
+    gk, tk = _heads(dk, "dk", (batch, tokens, heads, nk), kind)
+    gv, tv = _heads(dv, "dv", (batch, tokens, heads, nv), kind)
+    pd = _array(log_decay, "log_decay", 4 * heads, "real")
+    shape = (batch, heads, nk, nv)
+    ps, pn, pg = _states(state, "state", shape), _states(dnew_state, "dnew_state", shape), _states(dstate, "dstate", shape)
+    pl = None if lens is None else _array(lens, "lens", 4 * batch, "words")
+    pw, splits = _splits(work, 3 * batch * heads * nk * nv)
+    _on_gpu((q, "q"), (k, "k"), (v, "v"), (dout, "dout"), (dq, "dq"), (dk, "dk"), (dv, "dv"), (log_decay, "log_decay"),
+            (state, "state"), (dnew_state, "dnew_state"), (dstate, "dstate"), (lens, "lens"), (work if splits else None, "work"))
+    check(lib.fufft_decay_attention_grad(po, C.byref(so), pq, C.byref(sq), pk, C.byref(sk), pv, C.byref(sv), kind, pd, gq,
+                                         C.byref(tq), gk, C.byref(tk), gv, C.byref(tv), ps, pn, pg, pl, scale, batch, tokens,
+                                         heads, nk, nv, pw, splits, _stream(stream)), "fufft_decay_attention_grad")
+
+
+def decay_attention_step(q, k, v, log_decay, state, out, *, slots=None, scale: float = 1.0, stream=None) -> None:
+    """One token of every sequence: q, k (batch, heads, dk), v and out (batch, heads, dv); state (slot_count,
+    heads, dk, dv) is updated in place.  slots (int64, batch): the state of each sequence, None: its own
+    number.  A slot outside, such as -1, or one that an earlier sequence of the call has, changes nothing
+    and gives zeros."""
+    pq, sq = _heads(q, "q", (None,) * 3)
+    kind = _ELEMENT[q.dtype]
+    batch, heads, dk = q.shape
+    pk, sk = _heads(k, "k", (batch, heads, dk), kind)
+    pv, sv = _heads(v, "v", (batch, heads, None), kind)
+    dv = v.shape[2]
+    po, so = _heads(out, "out", (batch, heads, dv), kind)
+    pd = _array(log_decay, "log_decay", 4 * heads, "real")
+    if torch is None or not isinstance(state, torch.Tensor):
+        raise TypeError(f"state: expected a torch tensor in GPU memory, got {type(state).__name__}")
+    if state.dim() != 4 or tuple(state.shape[1:]) != (heads, dk, dv):
+        raise ValueError(f"state: expected (slots, {heads}, {dk}, {dv}), got {tuple(state.shape)}")
+    count = state.shape[0]
+    if slots is None and count < batch:
+        raise ValueError(f"state: {count} states, q has {batch} sequences")
+    ps = _array(state, "state", 4 * count * heads * dk * dv, "real")
+    pi = None if slots is None else _array(slots, "slots", 8 * batch, "slots")
+    _on_gpu((q, "q"), (k, "k"), (v, "v"), (out, "out"), (log_decay, "log_decay"), (state, "state"), (slots, "slots"))
+    check(lib.fufft_decay_attention_step(pq, C.byref(sq), pk, C.byref(sk), pv, C.byref(sv), kind, pd, po, C.byref(so), ps,
+                                         count, pi, scale, batch, heads, dk, dv, _stream(stream)),
+          "fufft_decay_attention_step")

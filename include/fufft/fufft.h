@@ -585,8 +585,10 @@ int fufft_mx4_cache_conv(const void* codes, const uint8_t* scales, int64_t pages
                          int64_t tap_count, void* out, int type, float* work, int64_t splits,
                          void* stream);
 
-/* ---- norms and 8-bit rows --------------------------------------------------------------
- * What stands around a sequence mixer in a model.  No reference counterpart.
+/* ---- norms, 8-bit rows and decaying linear attention ------------------------------------
+ * What stands around a sequence mixer in a model, and the mixer beside the long convolution
+ * whose filter is an exponential: its history is a state of fixed size.  No reference
+ * counterpart.
  *
  * Element types, leading dimensions, alignment and sizes of zero are as in the 4-bit
  * calls above.  Every sum, state and statistic is fp32 (integer sums int32), rounded
@@ -639,6 +641,62 @@ int fufft_rms_norm_grad(const void* dy, int type, int64_t ldy, const void* h, in
                         const void* dtotal, int64_t ldt, int sum_type, const float* weight,
                         float eps, void* dx, int dx_type, int64_t ldx, float* dweight, float* work,
                         int64_t splits, int64_t rows, int64_t k, void* stream);
+
+/* Linear attention with a decay for each head.  Of a head, with a = exp(log_decay[head]):
+ *     S[t] = a S[t-1] + k[t] v[t]^T        out[t] = scale * q[t]^T S[t]
+ * S, the state, is dk x dv in fp32; S[-1] is `state`, or zero.
+ * q, k, v, out are arrays of batch x tokens x heads x dim, dim (dk of q and k, dv of v and
+ * out) from 1 to 128 (beyond: FUFFT_ERR_UNSUPPORTED), with adjacent elements and the strides
+ * (elements, >= 0; of an input 0 too: one k for all heads) of a fufft_strides.  log_decay is
+ * heads fp32 values, <= 0, -infinity included: only the token itself.
+ *   lens       batch int32: tokens of each sequence, within 0 .. tokens; rows behind the last
+ *              are neither read nor written.  NULL: tokens;
+ *   state, new_state   batch x heads x dk x dv fp32, contiguous, or NULL: zero; not wanted.
+ *              new_state is S after the last token, `state` for an empty sequence.  It may
+ *              be state;
+ *   work       fp32 space for `splits` states of every sequence and head (splits x batch x heads
+ *              x dk x dv): the tokens are split over at most that many workgroups.
+ *              0 (NULL) is allowed.  About 1024 / (batch * heads) are as many as help.
+ * Products of 16-bit inputs go through the matrix cores in that type with fp32 sums; what
+ * becomes an operand again, weighted scores and the state that q meets, is rounded to
+ * bf16 (its range is fp32's); the carried state is kept to 16 bits or better a term.  fp32 and fp16
+ * inputs are multiplied in fp32.  A token's result does not depend on later tokens, whatever
+ * they hold. */
+typedef struct fufft_strides {
+   int64_t batch, token, head;
+} fufft_strides;
+int fufft_decay_attention(const void* q, const fufft_strides* q_strides, const void* k,
+                          const fufft_strides* k_strides, const void* v,
+                          const fufft_strides* v_strides, int type, const float* log_decay,
+                          void* out, const fufft_strides* out_strides, const float* state,
+                          float* new_state, const int32_t* lens, float scale, int64_t batch,
+                          int64_t tokens, int64_t heads, int64_t dk, int64_t dv, float* work,
+                          int64_t splits, void* stream);
+/* Its gradients: dq, dk and dv of dout (and of dnew_state, new_state's gradient, or NULL), dstate
+ * of the same, or NULL: not wanted.  Of heads that share an input (stride 0) each has a
+ * gradient of its own: the caller adds them.  log_decay is a constant of the model.
+ * work is as above with room for 3 such sets: splits x 3 x batch x heads x dk x dv. */
+int fufft_decay_attention_grad(const void* dout, const fufft_strides* dout_strides, const void* q,
+                               const fufft_strides* q_strides, const void* k,
+                               const fufft_strides* k_strides, const void* v,
+                               const fufft_strides* v_strides, int type, const float* log_decay,
+                               void* dq, const fufft_strides* dq_strides, void* dk_out,
+                               const fufft_strides* dk_strides, void* dv_out,
+                               const fufft_strides* dv_strides, const float* state,
+                               const float* dnew_state, float* dstate, const int32_t* lens,
+                               float scale, int64_t batch, int64_t tokens, int64_t heads,
+                               int64_t dk, int64_t dv, float* work, int64_t splits, void* stream);
+/* One token of every sequence: q, k, v, out batch x heads x dim (strides: token unused), and
+ * state, `slot_count` x heads x dk x dv fp32, contiguous, updated in place.  slots: the state of
+ * each sequence, int64, or NULL: its own number (slot_count >= batch then).  A sequence whose slot is outside
+ * [0, slot_count) (-1: a place in the batch without a sequence), or is that of an earlier one
+ * of the call, changes no state and has zeros for its result.  All in fp32. */
+int fufft_decay_attention_step(const void* q, const fufft_strides* q_strides, const void* k,
+                               const fufft_strides* k_strides, const void* v,
+                               const fufft_strides* v_strides, int type, const float* log_decay,
+                               void* out, const fufft_strides* out_strides, float* state,
+                               int64_t slot_count, const int64_t* slots, float scale,
+                               int64_t batch, int64_t heads, int64_t dk, int64_t dv, void* stream);
 
 #ifdef __cplusplus
 }

@@ -102,3 +102,75 @@ def norm_grad(dy, h, weight, dtotal, eps):
         err = err + EPS24 * np.abs(dx)
     terms = dy * n
     return dx, err, terms.sum(0), np.abs(terms).sum(0)
+
+
+# ---- decaying attention --------------------------------------------------------------------
+
+def mixed(q, k, v, log_decay, state=None, late=0):
+    """One head, token by token: (out without a scale, state behind, and the same of the magnitudes of
+    all terms).  late: the state given meets its first token undecayed, the one returned is decayed
+    once more."""
+    a = np.exp(np.float64(log_decay))
+    tokens, dk = q.shape
+    dv = v.shape[1]
+    s = np.zeros((dk, dv)) if state is None else np.array(state, dtype=np.float64)
+    m = np.abs(s)
+    out, mags = np.zeros((tokens, dv)), np.zeros((tokens, dv))
+    for t in range(tokens):
+        if not (late and t == 0):
+            s, m = (a * s, a * m) if a > 0 else (np.zeros_like(s), np.zeros_like(m))
+        s = s + np.outer(k[t], v[t])
+        m = m + np.outer(np.abs(k[t]), np.abs(v[t]))
+        out[t], mags[t] = q[t] @ s, np.abs(q[t]) @ m
+    if late and tokens:
+        s, m = a * s, a * m
+    return out, s, mags, m
+
+
+def mixed_share(kind, tokens, dim, log_decay, carried=False):
+    """The share of the magnitudes that the call's arithmetic may be off by, before the result's own rounding.  bf16:
+    weighted scores and the state that q meets are rounded once, at 2^-8; the keys' two parts leave 2^-16.  fp32's
+    part: sums of dim and of 64 terms a chunk, twice in bf16, the chunk's decay; powers whose exponent is off by its
+    own rounding, 2^-23 of |log_decay| tokens."""
+    chunks = tokens // 64 + 1
+    decay = 0.0 if not np.isfinite(log_decay) else abs(log_decay)
+    chain = dim + 64 + 132 * chunks + 12 + 4 * decay * (tokens + 1)
+    return chain * EPS24 + (0.0 if kind != "bf16" else 1.05 * 2.0 ** -16 if carried else 1.02 * 2.0 ** -8 * 2)
+
+
+def attention(q, k, v, log_decay, state, lens, scale, kind):
+    """(out, its bound, new state, its bound) of (batch, tokens, heads, dim) arrays; rows from lens on are zero."""
+    batch, tokens, heads, dk = q.shape
+    dv = v.shape[3]
+    out, err = np.zeros((batch, tokens, heads, dv)), np.zeros((batch, tokens, heads, dv))
+    new, nerr = np.zeros((batch, heads, dk, dv)), np.zeros((batch, heads, dk, dv))
+    for b in range(batch):
+        n = tokens if lens is None else min(max(int(lens[b]), 0), tokens)
+        for h in range(heads):
+            o, s, mo, ms = mixed(q[b, :n, h], k[b, :n, h], v[b, :n, h], log_decay[h], None if state is None else state[b, h])
+            out[b, :n, h], new[b, h] = scale * o, s
+            err[b, :n, h] = abs(scale) * mo * mixed_share(kind, n, dk, log_decay[h])
+            nerr[b, h] = ms * mixed_share(kind, n, 0, log_decay[h], carried=True)
+    return out, err, new, nerr
+
+
+def attention_grad(do, q, k, v, log_decay, state, dnew, lens, scale, kind):
+    """((dq, bound), (dk, bound), (dv, bound), (dstate, bound)), from the recurrence of D[t] = q[t] do[t]^T + a D[t + 1]."""
+    batch, tokens, heads, dk = q.shape
+    dv = v.shape[3]
+    got = [(np.zeros(x.shape), np.zeros(x.shape)) for x in (q, k, v)] + [(np.zeros((batch, heads, dk, dv)), np.zeros((batch, heads, dk, dv)))]
+    for b in range(batch):
+        n = tokens if lens is None else min(max(int(lens[b]), 0), tokens)
+        for h in range(heads):
+            g = log_decay[h]
+            Q, K, V, D = q[b, :n, h], k[b, :n, h], v[b, :n, h], do[b, :n, h]
+            st = None if state is None else state[b, h].T
+            dn = None if dnew is None else dnew[b, h]
+            o, _, m, _ = mixed(D, V, K, g, st)
+            got[0][0][b, :n, h], got[0][1][b, :n, h] = scale * o, abs(scale) * m * mixed_share(kind, n, dv, g)
+            o, _, m, _ = mixed(V[::-1], scale * D[::-1], Q[::-1], g, None if dn is None else dn.T, 1)
+            got[1][0][b, :n, h], got[1][1][b, :n, h] = o[::-1], m[::-1] * mixed_share(kind, n, dv, g)
+            o, s, m, ms = mixed(K[::-1], scale * Q[::-1], D[::-1], g, dn, 1)
+            got[2][0][b, :n, h], got[2][1][b, :n, h] = o[::-1], m[::-1] * mixed_share(kind, n, dk, g)
+            got[3][0][b, h], got[3][1][b, h] = s, ms * mixed_share(kind, n, 0, g, carried=True)
+    return got
