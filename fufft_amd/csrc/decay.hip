@@ -21,6 +21,8 @@
 #include "fufft_internal.hpp"
 #include "mx4_device.hpp"
 
+#include <type_traits>
+
 namespace fufft {
 namespace layer {
 
@@ -58,18 +60,98 @@ template<> struct Cores<bf16> {
    static __device__ inline f32x4 mma(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 
-template<class T> struct __attribute__((packed, aligned(sizeof(T)))) Eight { T e[8]; };
+// N neighbours of a row as they are in memory, loaded at the element's alignment.
+template<class T, int N> struct Raw {
+   static constexpr int WORDS = N * (int)sizeof(T) / 4;
+   uint32_t w[WORDS];
 
-// Rows of 16-byte slots in LDS, a slot's bytes apart more than they hold: 16 lanes that read one slot of 16
-// rows meet all banks, and every address of a lane is one register and a constant.
+   __device__ inline float value(int j) const
+   {
+      if constexpr(sizeof(T) == 4) {
+         return __uint_as_float(w[j]);
+      } else if constexpr(std::is_same<T, bf16>::value) {
+         return __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+      } else {
+         return (float)__builtin_bit_cast(T, (uint16_t)(w[j / 2] >> (j % 2 * 16)));
+      }
+   }
+   // elements from `count` on made zero
+   __device__ inline void cut(int count)
+   {
+#pragma unroll
+      for(int j = 0; j < N; j++)
+         if(j >= count) {
+            if constexpr(sizeof(T) == 4) w[j] = 0u;
+            else w[j / 2] &= j % 2 ? 0x0000ffffu : 0xffff0000u;
+         }
+   }
+};
+template<class T, int N>
+__device__ inline Raw<T, N> raw_at(const T* p)
+{
+   typedef uint32_t V __attribute__((ext_vector_type(Raw<T, N>::WORDS), aligned(sizeof(T))));
+   const V v = *reinterpret_cast<const V*>(p);
+   Raw<T, N> x;
+#pragma unroll
+   for(int i = 0; i < Raw<T, N>::WORDS; i++) x.w[i] = v[i];
+   return x;
+}
+// the same of a row whose elements from `count` on are not there: the first one is read in their place
+template<class T, int N>
+__device__ inline Raw<T, N> raw_of(const T* p, const T* first, int count)
+{
+   Raw<T, N> x{};
+#pragma unroll
+   for(int j = 0; j < N; j++) {
+      const T e = *(j < count ? p + j : first);
+      if constexpr(sizeof(T) == 4) x.w[j] = __builtin_bit_cast(uint32_t, e);
+      else x.w[j / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, e) << (j % 2 * 16);
+   }
+   return x;
+}
+// whether one of them is infinite or NaN
+template<class T, int N>
+__device__ inline bool odd_one(const Raw<T, N> (&x)[8])
+{
+   if constexpr(sizeof(T) == 2) {
+      typedef uint16_t V __attribute__((ext_vector_type(2)));
+      V m = {0, 0};
+#pragma unroll
+      for(int i = 0; i < 8; i++)
+#pragma unroll
+         for(int j = 0; j < Raw<T, N>::WORDS; j++) m = __builtin_elementwise_max(m, __builtin_bit_cast(V, x[i].w[j] & 0x7fff7fffu));
+      constexpr uint16_t LIMIT = std::is_same<T, bf16>::value ? 0x7f80 : 0x7c00;
+      return m[0] >= LIMIT || m[1] >= LIMIT;
+   } else {
+      uint32_t m = 0;
+#pragma unroll
+      for(int i = 0; i < 8; i++)
+#pragma unroll
+         for(int j = 0; j < N; j++) m = mx4::umax(m, x[i].w[j] & 0x7fffffffu);
+      return m >= 0x7f800000u;
+   }
+}
+
+// LDS.  Keys as they are and the state: rows of 16-byte slots, a slot further apart than they are long, so that lanes
+// that read one slot of 8 rows meet all banks.  By channel, rows of a chunk's tokens: slot s of row r is at
+// s ^ turn(r), which does the same for 8 rows that follow each other, as products read them, and for 8 every
+// second one, as staging writes them.  (Padded rows there, written 8 bytes a lane, were two thirds of all
+// LDS cycles conflicts: 65536 tokens x 16 heads 457 us in the last launch.)
 constexpr int pitch_of(int bytes) { return bytes + 16; }
+__device__ inline int turn(int row) { return (row & 7) ^ (row >> 3 & 1); }
 
 // `x` as the compiler cannot know it from before: what is derived from it is not kept in registers
 // over the chunks
-__device__ inline int anew(int x)
+__device__ inline int anew(int x)       // of one value in all lanes
 {
+   x = __builtin_amdgcn_readfirstlane(x);
    asm volatile("" : "+s"(x));
    return x;
+}
+__device__ inline int64_t anew(int64_t x)
+{
+   const uint32_t lo = (uint32_t)anew((int)(uint32_t)x), hi = (uint32_t)anew((int)(uint32_t)(x >> 32));
+   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 __device__ inline int anew_lane(int x)
 {
@@ -85,19 +167,16 @@ __device__ inline float power(float g2, float n) { return __builtin_amdgcn_exp2f
 template<class T, int DK, int DV, bool LOCAL> struct Room {
    typedef Cores<T> C;
    static constexpr int E = sizeof(typename C::E);
-   static constexpr int TP = pitch_of(kChunk * E), KP = pitch_of(DK * E);       // rows of tokens, of keys' channels
+   static constexpr int TP = kChunk * E, KP = pitch_of(DK * E);       // bytes of a row of tokens, of keys' channels
    static constexpr int VALUES = 0, KEYS_T = VALUES + DV * TP, KEYS = KEYS_T + C::PARTS * DK * TP;
    static constexpr int STATE = LOCAL ? KEYS : KEYS + kChunk * KP, FLAGS = LOCAL ? KEYS : STATE + DV * KP;
    static constexpr int BYTES = FLAGS + 16;
 };
 
-// where tokens 4 q .. 4 q + 3 are in a row of tokens: in bf16 in block q / 8, of its piece q % 4 the first or
-// second half
-template<class E>
-__device__ inline int tokens_at(int q)
-{
-   return sizeof(E) == 4 ? q * 16 : ((q >> 3) * 4 + (q & 3)) * 16 + ((q >> 2) & 1) * 8;
-}
+// The slot of a row of tokens that token t is in, and its bytes in it: in bf16 a slot has tokens 4 g .. 4 g + 3 of
+// two 16 tokens, as an operand's block of 32 takes them.
+template<class E> __device__ inline int slot_of(int t) { return sizeof(E) == 4 ? t / 4 : t / 32 * 4 + t / 4 % 4; }
+template<class E> __device__ inline int in_slot(int t) { return sizeof(E) == 4 ? t % 4 * 4 : (t / 16 % 2 * 4 + t % 4) * 2; }
 template<class E>
 __device__ inline void put4(uint8_t* to, const float (&v)[4])
 {
@@ -105,7 +184,7 @@ __device__ inline void put4(uint8_t* to, const float (&v)[4])
    else *reinterpret_cast<bf16x4*>(to) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
 }
 
-template<class T, int DK, int DV, bool LOCAL>
+template<class T, int DK, int DV, bool LOCAL, bool WHOLE>
 __global__ void __launch_bounds__(kLanes)
 decay_chunks(DecayParams p)
 {
@@ -114,11 +193,12 @@ decay_chunks(DecayParams p)
    typedef typename C::Frag Frag;
    typedef Room<T, DK, DV, LOCAL> M;
    constexpr int BLOCK = sizeof(E) == 2 ? 32 : 16;             // of the summed index of a product
+   constexpr int EACH = BLOCK / 16;                            // results to a block
    constexpr int NK = DK / BLOCK, NS = kChunk / BLOCK;          // blocks of keys' channels, of tokens
    constexpr int KP = M::KP, TP = M::TP;
    constexpr int SA = DK / 64, SB = DV / 32;                   // a wavefront's results of the state; SB of out too
-   constexpr int KT = DK / 32, VT = DV / 32;                   // wavefronts that stage keys, values: 4 tokens x 8 channels a lane
-   static_assert(KT + VT <= kLanes / 64, "every piece has a lane");
+   constexpr int KJ = DK * 4, VJ = DV * 4;                     // lanes that stage keys, values: 8 tokens x 2 channels each
+   static_assert(KJ <= kLanes && VJ <= kLanes, "every piece has a lane");
    extern __shared__ uint8_t lds[];
    int* const flags = reinterpret_cast<int*>(lds + M::FLAGS);
    const DecayRole& role = p.role[blockIdx.y];
@@ -139,8 +219,8 @@ decay_chunks(DecayParams p)
    }
    const int64_t first = seg * p.segment;
    if(first >= len && seg > 0) return;
-   const int64_t left = len - first < p.segment ? len - first : p.segment;      // this segment's tokens
-   if(LOCAL && first + left >= len) return;                     // the last segment's part is not asked for
+   const int left = (int)(len - first < p.segment ? len - first : p.segment);     // this segment's tokens
+   if(LOCAL && first + left >= len) return;                    // the last segment's part is not asked for
    const int dk = role.dk, dv = role.dv, dv0 = slice * DV;
    if(dv0 >= dv) return;                                       // a role of fewer slices
    const int dvn = dv - dv0 < DV ? dv - dv0 : DV;
@@ -155,58 +235,87 @@ decay_chunks(DecayParams p)
    const T* const q = rows_of(role.q, role.sq);
    const T* const k = rows_of(role.k, role.sk);
    const T* const v = rows_of(role.v, role.sv) + dv0;
+   T* const out = LOCAL ? nullptr : static_cast<T*>(role.o) + b * role.so.batch + h * role.so.head + at0 * role.so.token + dv0;
+   const int64_t ostep = dir * role.so.token;
 
-   // staging: this lane's tokens and channels
-   const bool keys = wave < KT, values = !keys && wave < KT + VT;
-   const int piece = keys ? tid : tid - KT * 64;
-   const int width = (keys ? DK : DV) / 8, cb = piece % width, tq = piece / width;
-   const T* const src = (keys ? k : v) + cb * 8;
-   const int64_t step = dir * (keys ? role.sk.token : role.sv.token);
-   const int dim = keys ? dk : dvn;
-   Eight<T> raw[4];
-   auto fetch = [&](int64_t t0) {
-      if(!keys && !values) return;
-      const int d = anew(dim), n = (int)(left - t0 < kChunk ? left - t0 : kChunk);
-      const T* const p0 = src + (t0 + tq * 4) * step;
+   // Staging: this lane's two channels of 8 tokens of keys and of values, those of one slot of a row of tokens (of two in
+   // fp32): token i is st + i of the first four, st + 16 + i - 4 of the others.  Where a token or a channel is not there the
+   // segment's first one is read, and what came is cleared on its way to LDS: no load waits for another,
+   // and none is beyond the array.
+   typedef Raw<T, 2> Pair;
+   const bool has_k = wave < KJ / 64, has_v = wave >= (kLanes - VJ) / 64;
+   const int pv = tid - (kLanes - VJ);
+   const int kc = tid % (DK / 2) * 2, vc = pv % (DV / 2) * 2, kj = tid / (DK / 2), vj = pv / (DV / 2);
+   const int kt = kj / 4 * 32 + kj % 4 * 4, vt = vj / 4 * 32 + vj % 4 * 4;
+   const int64_t kstep = dir * role.sk.token, vstep = dir * role.sv.token;
+   Pair kr[8], vr[8];
+   auto token = [](int i) { return i < 4 ? i : i + 12; };
+   auto fetch_pairs = [&](Pair (&to)[8], const T* base, int64_t step, int t, int c, int dim, int n, int t0) {
+      const int channels = anew(dim);
+      const int64_t by = anew(step);
+      const T* const at = base + (t0 + t) * step + (c < channels ? c : 0);
 #pragma unroll
-      for(int i = 0; i < 4; i++) {
-         raw[i] = Eight<T>{};
-         if(d % 8 == 0) {
-            if(tq * 4 + i < n && cb * 8 < d) raw[i] = *reinterpret_cast<const Eight<T>*>(p0 + i * step);
-         } else if(tq * 4 + i < n) {
-#pragma unroll
-            for(int j = 0; j < 8; j++)
-               if(cb * 8 + j < d) raw[i].e[j] = p0[i * step + j];
-         }
+      for(int i = 0; i < 8; i++) {
+         const T* const from = t + token(i) < n ? at + token(i) * by : base;
+         if constexpr(WHOLE) to[i] = raw_at<T, 2>(from);
+         else                to[i] = raw_of<T, 2>(from, from, channels - c);
       }
+   };
+   auto fetch = [&](int t0) {
+      const int n = left - t0 < kChunk ? left - t0 : kChunk;
+      if(has_k) fetch_pairs(kr, k, kstep, kt, kc, dk, n, t0);
+      if(has_v) fetch_pairs(vr, v, vstep, vt, vc, dvn, n, t0);
+   };
+   // clears what is not there
+   auto clear = [&](Pair (&x)[8], int t, int c, int dim, int n) {
+      const int channels = anew(dim);
+#pragma unroll
+      for(int i = 0; i < 8; i++) x[i].cut(t + token(i) < n ? channels - c : 0);
    };
 
    // this wavefront's strip of 16 tokens and half of the values; two wavefronts of a SIMD have 5 of the
    // 8 strips' blocks of scores between them
    const int strip = wave < 4 ? wave : 7 - wave, half = wave >> 2;
    const int v0 = half * (DV / 2), k0 = (wave & 3) * (DK / 4);
-   Frag qf[NK];
-   auto fetch_q = [&](int64_t t0) {
-      constexpr int N = 16 / (int)sizeof(E);
-      struct __attribute__((packed, aligned(sizeof(T)))) Piece { T e[N]; };
-      const int d = anew(dk);
-      const bool there = t0 + strip * 16 + row < left;
-      const T* const p0 = q + (t0 + strip * 16 + row) * dir * role.sq.token + g * N;
+   constexpr int N = 16 / (int)sizeof(E);                       // values of a piece of an operand
+   Raw<T, N> qr[NK];
+   const int64_t qstep = dir * role.sq.token;
+   auto fetch_q = [&](int t0) {
+      const int channels = anew(dk);
+      const bool there = t0 + strip * 16 + row < left;          // else any row: its results are not kept
+      const T* const at = q + (there ? (t0 + strip * 16 + row) * anew(qstep) : 0);
 #pragma unroll
       for(int i = 0; i < NK; i++) {
-         const int at = i * BLOCK + g * N;
-         Piece x{};
-         if(d % N == 0) {
-            if(there && at < d) x = *reinterpret_cast<const Piece*>(p0 + i * BLOCK);
-         } else if(there) {
-#pragma unroll
-            for(int j = 0; j < N; j++)
-               if(at + j < d) x.e[j] = p0[i * BLOCK + j];
-         }
-#pragma unroll
-         for(int j = 0; j < N; j++) qf[i][j] = (E)x.e[j];
+         const int c = i * BLOCK + g * N;
+         const T* const from = at + (c < channels ? c : 0);
+         if constexpr(WHOLE) qr[i] = raw_at<T, N>(from);
+         else                qr[i] = raw_of<T, N>(from, from, channels - c);
       }
    };
+   auto operand_q = [&](int i) {
+      if(dk < DK) qr[i].cut(anew(dk) - i * BLOCK - g * N);
+      Frag f;
+      if constexpr(sizeof(E) == sizeof(T)) {
+         f = __builtin_bit_cast(Frag, qr[i]);
+      } else {
+#pragma unroll
+         for(int j = 0; j < N; j++) f[j] = (E)qr[i].value(j);
+      }
+      return f;
+   };
+
+   // weights of keys on their way into the state; those of tokens that are not there meet zeros
+   const int late = role.late;
+   const float kv_scale = role.kv_scale;
+   float wk[8];
+   auto key_weights = [&](int n) {
+#pragma unroll
+      for(int i = 0; i < 8; i++) {
+         const int d = n - 1 - kt - token(i) + late;
+         wk[i] = power(g2, (float)(d < 0 ? 0 : d)) * kv_scale;
+      }
+   };
+   key_weights(kChunk);
 
    // weights of scores: a^(t - s), rows s of result i, column t; and of q S at t
    float wt[4][4], wq = 0.0f;
@@ -218,7 +327,7 @@ decay_chunks(DecayParams p)
             const int d = (strip - i) * 16 + row - g * 4 - r;
             wt[i][r] = d >= 0 ? power(g2, (float)d) * role.p_scale * role.out_scale : 0.0f;
          }
-      wq = power(g2, (float)(strip * 16 + row + 1 - role.late)) * role.out_scale;
+      wq = power(g2, (float)(strip * 16 + row + 1 - late)) * role.out_scale;
    }
 
    // the state before the segment: keys' channels k0 + 16 a + 4 g + r, value v0 + 16 b + row
@@ -234,12 +343,15 @@ decay_chunks(DecayParams p)
             const int i = k0 + a * 16 + g * 4, j = dv0 + v0 + c * 16 + row;
             const int at = turned ? j * rows + i : i * cols + j, step = turned ? 1 : cols;
 #pragma unroll
-            for(int r = 0; r < 4; r++) if(j < cols && i + r < rows) body(a, c, r, at + r * step);
+            for(int r = 0; r < 4; r++)
+               if(j < cols && i + r < rows) body(a, c, r, at + r * step);
          }
    };
    const float* const from = LOCAL ? nullptr
                              : p.segments > 1 ? role.work + (seg * p.pairs + bh) * count
                              : role.state ? role.state + bh * count : nullptr;
+   float* const behind = LOCAL ? role.work + (seg * p.pairs + bh) * count
+                         : role.new_state && first + left >= len ? role.new_state + bh * count : nullptr;
 #pragma unroll
    for(int a = 0; a < SA; a++)
 #pragma unroll
@@ -253,65 +365,70 @@ decay_chunks(DecayParams p)
    if(tid < 2) flags[tid] = 0;
    __syncthreads();
    int side = 0;
-   for(int64_t t0 = 0; t0 < left; t0 += kChunk, side ^= 1) {
-      const int n = (int)(left - t0 < kChunk ? left - t0 : kChunk);
+   for(int t0 = 0; t0 < left; t0 += kChunk, side ^= 1) {
+      const int n = left - t0 < kChunk ? left - t0 : kChunk;
       // to LDS: values and weighted keys by channel, keys as they are, the state by value
-      if(keys) {
-         float w[4];
+      auto put_tokens = [&](int base, int row, int slot, const float (&x)[8]) {
+         uint8_t* const to = lds + base + row * TP;
+         if constexpr(sizeof(E) == 4) {
+            *reinterpret_cast<f32x4*>(to + (slot ^ turn(row)) * 16) = f32x4{x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<f32x4*>(to + ((slot + 4) ^ turn(row)) * 16) = f32x4{x[4], x[5], x[6], x[7]};
+         } else {
+            bf16x8 e;
 #pragma unroll
-         for(int i = 0; i < 4; i++) {
-            const int s = tq * 4 + i;
-            w[i] = s < n ? power(g2, (float)(n - 1 - s + role.late)) * role.kv_scale : 0.0f;
+            for(int i = 0; i < 8; i++) e[i] = (bf16)x[i];
+            *reinterpret_cast<bf16x8*>(to + (slot ^ turn(row)) * 16) = e;
          }
-         uint8_t* const to = lds + M::KEYS_T + cb * 8 * TP + tokens_at<E>(tq);
+      };
+      if(has_v) {
+         if(n < kChunk || dvn < DV) clear(vr, vt, vc, dvn, n);
+         if(!LOCAL && odd_one(vr)) flags[side] = 1;
+         if constexpr(std::is_same<T, bf16>::value) {
 #pragma unroll
-         for(int j = 0; j < 8; j++) {
-            float x[4];
+            for(int j = 0; j < 2; j++) {
+               mx4::u32x4 e;
 #pragma unroll
-            for(int i = 0; i < 4; i++) x[i] = (float)raw[i].e[j] * w[i];
-            put4<E>(to + j * TP, x);
-            if constexpr(C::PARTS == 2) {
-               // what bf16 leaves of it; nothing of an infinity
-               float y[4];
-#pragma unroll
-               for(int i = 0; i < 4; i++) {
-                  const float whole = (float)(bf16)x[i];
-                  y[i] = fabsf(whole) < __builtin_inff() ? x[i] - whole : 0.0f;
-               }
-               put4<E>(to + (DK + j) * TP, y);
+               for(int i = 0; i < 4; i++) e[i] = __builtin_amdgcn_perm(vr[2 * i + 1].w[0], vr[2 * i].w[0], j ? 0x07060302 : 0x05040100);
+               *reinterpret_cast<mx4::u32x4*>(lds + M::VALUES + (vc + j) * TP + (slot_of<E>(vt) ^ turn(vc + j)) * 16) = e;
             }
-         }
-         if constexpr(!LOCAL) {
-            uint8_t* const plain = lds + M::KEYS + tq * 4 * KP + cb * 8 * (int)sizeof(E);
+         } else {
 #pragma unroll
-            for(int i = 0; i < 4; i++) {
-               if constexpr(sizeof(E) == 2) {
-                  *reinterpret_cast<bf16x8*>(plain + i * KP) = __builtin_bit_cast(bf16x8, raw[i]);
-               } else {
+            for(int j = 0; j < 2; j++) {
+               float x[8];
 #pragma unroll
-                  for(int j = 0; j < 2; j++) {
-                     const float x[4] = {(float)raw[i].e[4 * j], (float)raw[i].e[4 * j + 1], (float)raw[i].e[4 * j + 2],
-                                         (float)raw[i].e[4 * j + 3]};
-                     put4<E>(plain + i * KP + j * 16, x);
-                  }
-               }
+               for(int i = 0; i < 8; i++) x[i] = vr[i].value(j);
+               put_tokens(M::VALUES, vc + j, slot_of<E>(vt), x);
             }
          }
       }
-      if(values) {
-         bool odd = false;
-         uint8_t* const to = lds + M::VALUES + cb * 8 * TP + tokens_at<E>(tq);
+      if(has_k) {
+         if(n < kChunk || dk < DK) clear(kr, kt, kc, dk, n);
+         if constexpr(!LOCAL) {
+            uint8_t* const plain = lds + M::KEYS + kt * KP + kc * (int)sizeof(E);
 #pragma unroll
-         for(int j = 0; j < 8; j++) {
-            float x[4];
-#pragma unroll
-            for(int i = 0; i < 4; i++) {
-               x[i] = (float)raw[i].e[j];
-               odd |= !(fabsf(x[i]) < __builtin_inff());
+            for(int i = 0; i < 8; i++) {
+               if constexpr(sizeof(E) == 2) *reinterpret_cast<uint32_t*>(plain + token(i) * KP) = kr[i].w[0];
+               else *reinterpret_cast<mx4::f32x2*>(plain + token(i) * KP) = mx4::f32x2{kr[i].value(0), kr[i].value(1)};
             }
-            put4<E>(to + j * TP, x);
          }
-         if(odd) flags[side] = 1;
+         if(n < kChunk) key_weights(n);
+         const bool odd = C::PARTS == 2 && odd_one(kr);
+#pragma unroll
+         for(int j = 0; j < 2; j++) {
+            float x[8];
+#pragma unroll
+            for(int i = 0; i < 8; i++) x[i] = kr[i].value(j) * wk[i];
+            put_tokens(M::KEYS_T, kc + j, slot_of<E>(kt), x);
+            if constexpr(C::PARTS == 2) {
+               // what bf16 leaves of it; nothing of an infinity
+#pragma unroll
+               for(int i = 0; i < 8; i++) x[i] -= (float)(bf16)x[i];
+               if(odd)
+#pragma unroll
+                  for(int i = 0; i < 8; i++) x[i] = fabsf(x[i]) < __builtin_inff() ? x[i] : 0.0f;
+               put_tokens(M::KEYS_T + DK * TP, kc + j, slot_of<E>(kt), x);
+            }
+         }
       }
       if constexpr(!LOCAL) {
          uint8_t* const to = lds + M::STATE + (v0 + row) * KP + (k0 + g * 4) * (int)sizeof(E);
@@ -323,42 +440,56 @@ decay_chunks(DecayParams p)
                put4<E>(to + c * 16 * KP + a * 16 * (int)sizeof(E), x);
             }
       }
+      Frag qf[NK];
+      if constexpr(!LOCAL) {
+#pragma unroll
+         for(int i = 0; i < NK; i++) qf[i] = operand_q(i);
+      }
       __syncthreads();
       const bool special = flags[side] != 0;
       if(tid == 0) flags[side ^ 1] = 0;
-      auto frag = [&](int base, int pitch, int r, int block) {
-         return *reinterpret_cast<const Frag*>(lds + base + (r + row) * pitch + (block * 4 + g) * 16);
+      auto frag = [&](int base, int r, int block) {             // of keys or the state
+         return *reinterpret_cast<const Frag*>(lds + base + (r + row) * KP + (block * 4 + g) * 16);
       };
-      auto value_frag = [&](int c, int sb) { return frag(M::VALUES, TP, v0 + c * 16, sb); };
-      const bool more = t0 + kChunk < left;
-      if(more) fetch(t0 + kChunk);                              // on its way under the products
+      auto token_frag = [&](int base, int r, int block) {       // of a row of tokens, r a multiple of 16
+         return *reinterpret_cast<const Frag*>(lds + base + (r + row) * TP + ((block * 4 + g) ^ turn(row)) * 16);
+      };
+      if(t0 + kChunk < left) fetch(t0 + kChunk);                // on their way under the products
 
       if constexpr(!LOCAL) {
          f32x4 o[SB] = {};
 #pragma unroll
-         for(int i = 0; i < NK; i++)
+         for(int i = 0; i < NK; i++) {
+            Frag x[SB];
 #pragma unroll
-            for(int c = 0; c < SB; c++)
-               o[c] = C::mma(frag(M::STATE, KP, v0 + c * 16, i), qf[i], o[c]);
+            for(int c = 0; c < SB; c++) x[c] = frag(M::STATE, v0 + c * 16, i);
+#pragma unroll
+            for(int c = 0; c < SB; c++) o[c] = C::mma(x[c], qf[i], o[c]);
+         }
 #pragma unroll
          for(int c = 0; c < SB; c++) o[c] *= wq;
          const int reach = anew_lane(strip * 16 + row - g * 4);      // scores of tokens up to this plus 4 g count
 #pragma unroll
          for(int sb = 0; sb < NS; sb++) {
-            constexpr int EACH = BLOCK / 16;                    // results to a block
             if(sb * EACH > strip) break;
             f32x4 s[EACH];
 #pragma unroll
             for(int e = 0; e < EACH; e++) {
                const int tile = sb * EACH + e;
                f32x4 x = {};
-               if(tile <= strip)
+               if(tile <= strip) {
+                  Frag kf[NK];
 #pragma unroll
-                  for(int i = 0; i < NK; i++)
-                     x = C::mma(frag(M::KEYS, KP, tile * 16, i), qf[i], x);
+                  for(int i = 0; i < NK; i++) kf[i] = frag(M::KEYS, tile * 16, i);
+#pragma unroll
+                  for(int i = 0; i < NK; i++) x = C::mma(kf[i], qf[i], x);
+               }
+#pragma unroll
+               for(int r = 0; r < 4; r++) s[e][r] = x[r] * wt[tile][r];
                // tokens behind t have no part in it, whatever they hold
+               if(tile == strip)
 #pragma unroll
-               for(int r = 0; r < 4; r++) s[e][r] = tile * 16 + r <= reach ? x[r] * wt[tile][r] : 0.0f;
+                  for(int r = 0; r < 4; r++) s[e][r] = tile * 16 + r <= reach ? s[e][r] : 0.0f;
             }
             Frag w;
 #pragma unroll
@@ -366,14 +497,17 @@ decay_chunks(DecayParams p)
 #pragma unroll
                for(int r = 0; r < 4; r++) w[e * 4 + r] = (E)s[e][r];
             if(!special) {
+               Frag x[SB];
 #pragma unroll
-               for(int c = 0; c < SB; c++) o[c] = C::mma(value_frag(c, sb), w, o[c]);
+               for(int c = 0; c < SB; c++) x[c] = token_frag(M::VALUES, v0 + c * 16, sb);
+#pragma unroll
+               for(int c = 0; c < SB; c++) o[c] = C::mma(x[c], w, o[c]);
             } else {
                // A value that is infinite or NaN times a weight of zero would reach tokens before it.  Such values
                // are left out of the products, and added one by one to the results that they belong to.
 #pragma unroll
                for(int c = 0; c < SB; c++) {
-                  Frag x = value_frag(c, sb);
+                  Frag x = token_frag(M::VALUES, v0 + c * 16, sb);
 #pragma unroll
                   for(int i = 0; i < EACH * 4; i++) x[i] = fabsf((float)x[i]) < __builtin_inff() ? x[i] : (E)0.0f;
                   o[c] = C::mma(x, w, o[c]);
@@ -385,22 +519,22 @@ decay_chunks(DecayParams p)
                      const int t1 = sb * BLOCK + (i / 4) * 16 + from_g * 4 + i % 4;
                      const float weight = __shfl((float)w[i], row + from_g * 16);
                      if(t1 > strip * 16 + row) continue;
-                     const uint8_t* const at = lds + M::VALUES + (v0 + g * 4) * TP + tokens_at<E>(t1 / 4) + t1 % 4 * (int)sizeof(E);
 #pragma unroll
                      for(int c = 0; c < SB; c++)
 #pragma unroll
                         for(int r = 0; r < 4; r++) {
-                           const float x = (float)*reinterpret_cast<const E*>(at + (c * 16 + r) * TP);
+                           const int channel = v0 + c * 16 + g * 4 + r;
+                           const float x = (float)*reinterpret_cast<const E*>(
+                              lds + M::VALUES + channel * TP + (slot_of<E>(t1) ^ turn(channel)) * 16 + in_slot<E>(t1));
                            if(!(fabsf(x) < __builtin_inff())) o[c][r] += weight * x;
                         }
                   }
             }
          }
-         if(more) fetch_q(t0 + kChunk);
          const int t = strip * 16 + row;
          if(t < n) {
             const int d = anew(dvn);
-            T* const out = static_cast<T*>(role.o) + b * role.so.batch + h * role.so.head + (at0 + dir * (t0 + t)) * role.so.token + dv0;
+            T* const to = out + (t0 + t) * ostep;
             struct __attribute__((packed, aligned(sizeof(T)))) Four { T e[4]; };
 #pragma unroll
             for(int c = 0; c < SB; c++) {
@@ -408,16 +542,18 @@ decay_chunks(DecayParams p)
                Four x;
 #pragma unroll
                for(int r = 0; r < 4; r++) x.e[r] = (T)o[c][r];
-               if(d % 4 == 0) {
-                  if(j < d) *reinterpret_cast<Four*>(out + j) = x;
+               if constexpr(WHOLE) {
+                  if(j < d) *reinterpret_cast<Four*>(to + j) = x;
                } else {
 #pragma unroll
                   for(int r = 0; r < 4; r++)
-                     if(j + r < d) out[j + r] = x.e[r];
+                     if(j + r < d) to[j + r] = x.e[r];
                }
             }
          }
       }
+      if constexpr(!LOCAL)
+         if(t0 + kChunk < left) fetch_q(t0 + kChunk);
       // the state behind the chunk
       const float an = power(g2, (float)n);
 #pragma unroll
@@ -426,25 +562,24 @@ decay_chunks(DecayParams p)
          for(int c = 0; c < SB; c++) S[a][c] *= an;
 #pragma unroll
       for(int sb = 0; sb < NS; sb++) {
-         Frag x[SB];
+         Frag x[SB], w[SA][C::PARTS];
 #pragma unroll
-         for(int c = 0; c < SB; c++) x[c] = value_frag(c, sb);
+         for(int c = 0; c < SB; c++) x[c] = token_frag(M::VALUES, v0 + c * 16, sb);
+#pragma unroll
+         for(int a = 0; a < SA; a++)
+#pragma unroll
+            for(int part = 0; part < C::PARTS; part++) w[a][part] = token_frag(M::KEYS_T, part * DK + k0 + a * 16, sb);
 #pragma unroll
          for(int part = 0; part < C::PARTS; part++)
 #pragma unroll
-            for(int a = 0; a < SA; a++) {
-               const Frag w = frag(M::KEYS_T, TP, part * DK + k0 + a * 16, sb);
+            for(int a = 0; a < SA; a++)
 #pragma unroll
-               for(int c = 0; c < SB; c++) S[a][c] = C::mma(w, x[c], S[a][c]);
-            }
+               for(int c = 0; c < SB; c++) S[a][c] = C::mma(w[a][part], x[c], S[a][c]);
       }
       __syncthreads();
    }
 
-   float* const to = LOCAL ? role.work + (seg * p.pairs + bh) * count
-                     : role.new_state && first + left >= len ? role.new_state + bh * count : nullptr;
-   if(!to) return;
-   each_state(!LOCAL && role.turned, [&](int a, int c, int r, int at) { to[at] = S[a][c][r]; });
+   if(behind) each_state(!LOCAL && role.turned, [&](int a, int c, int r, int at) { behind[at] = S[a][c][r]; });
 }
 
 // Every segment's part of the state in work becomes the state before that segment.  A lane has one
@@ -576,13 +711,13 @@ decay_step(StepParams p)
 
 // ---- launches --------------------------------------------------------------------------------
 
-template<class T, int DK, int DV, bool LOCAL>
+template<class T, int DK, int DV, bool LOCAL, bool WHOLE>
 hipError_t chunks_shape(DecayParams p, int roles, hipStream_t s)
 {
    constexpr int bytes = Room<T, DK, DV, LOCAL>::BYTES;
    static_assert(bytes <= 160 * 1024, "fits the LDS");
    static std::atomic<uint64_t> mask{0};
-   const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(&decay_chunks<T, DK, DV, LOCAL>), bytes, mask);
+   const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(&decay_chunks<T, DK, DV, LOCAL, WHOLE>), bytes, mask);
    if(e != hipSuccess) return e;
    int most = 0;
    for(int r = 0; r < roles; r++) most = p.role[r].dv > most ? p.role[r].dv : most;
@@ -590,12 +725,12 @@ hipError_t chunks_shape(DecayParams p, int roles, hipStream_t s)
    p.items = p.pairs * (LOCAL ? p.segments - 1 : p.segments);
    const int64_t groups = (p.items + 7) / 8 * 8 * p.slices;
    if(!grid_ok(groups, kLanes)) return kTooLarge;
-   decay_chunks<T, DK, DV, LOCAL><<<dim3((unsigned)groups, (unsigned)roles), kLanes, bytes, s>>>(p);
+   decay_chunks<T, DK, DV, LOCAL, WHOLE><<<dim3((unsigned)groups, (unsigned)roles), kLanes, bytes, s>>>(p);
    return hipGetLastError();
 }
 
-template<class T, int DK, int DV>
-hipError_t chunks_launches(DecayParams p, int roles, hipStream_t s)
+template<class T, int DK, int DV, bool WHOLE>
+hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
 {
    // Segments so that each CU has as many workgroups as fit its LDS, none of fewer than 4 chunks
    const int64_t chunks = (p.tokens + kChunk - 1) / kChunk;
@@ -609,7 +744,7 @@ hipError_t chunks_launches(DecayParams p, int roles, hipStream_t s)
    p.segment = each * kChunk;
    p.segments = chunks > 0 ? (chunks + each - 1) / each : 1;
    if(p.segments > 1) {
-      hipError_t e = chunks_shape<T, DK, DV, true>(p, roles, s);
+      hipError_t e = chunks_shape<T, DK, DV, true, WHOLE>(p, roles, s);
       if(e != hipSuccess) return e;
       int64_t most = 0;
       for(int r = 0; r < roles; r++) {
@@ -621,7 +756,15 @@ hipError_t chunks_launches(DecayParams p, int roles, hipStream_t s)
       e = hipGetLastError();
       if(e != hipSuccess) return e;
    }
-   return chunks_shape<T, DK, DV, false>(p, roles, s);
+   return chunks_shape<T, DK, DV, false, WHOLE>(p, roles, s);
+}
+
+// WHOLE: heads of whole groups of 8 channels
+template<class T, int DK, int DV>
+hipError_t chunks_launches(const DecayParams& p, int roles, hipStream_t s)
+{
+   return p.role[0].dk % 8 == 0 && p.role[0].dv % 8 == 0 ? segments_launches<T, DK, DV, true>(p, roles, s)
+                                                         : segments_launches<T, DK, DV, false>(p, roles, s);
 }
 
 // roles whose keys have the same width

@@ -172,7 +172,7 @@ int fufft_decay_attention(const void* q, const fufft_strides* q_strides, const v
    all.bytes(lens, lens ? batch * 4 : 0, 4, false);
    all.bytes(work, z.state_bytes(splits), 4, true);
    FUFFT_MX4_CHECK(all.check(state, new_state));
-   if(dk > kWidestHead || dv > kWidestHead) return FUFFT_ERR_UNSUPPORTED;
+   if(dk > kWidestHead || dv > kWidestHead || tokens > kLongestText) return FUFFT_ERR_UNSUPPORTED;
    DecayParams p{};
    p.role[0] = DecayRole{q, k, v, out, strides_of(q_strides), strides_of(k_strides), strides_of(v_strides), strides_of(out_strides),
                          state, new_state, work, (int)dk, (int)dv, 0, 0, 0, 1.0f, 1.0f, scale};
@@ -212,7 +212,7 @@ int fufft_decay_attention_grad(const void* dout, const fufft_strides* dout_strid
    all.bytes(lens, lens ? batch * 4 : 0, 4, false);
    all.bytes(work, z.state_bytes(splits * 3), 4, true);
    FUFFT_MX4_CHECK(all.check(nullptr, nullptr));
-   if(dk > kWidestHead || dv > kWidestHead) return FUFFT_ERR_UNSUPPORTED;
+   if(dk > kWidestHead || dv > kWidestHead || tokens > kLongestText) return FUFFT_ERR_UNSUPPORTED;
    const Strides sd = strides_of(dout_strides), sq = strides_of(q_strides), sk = strides_of(k_strides), sv = strides_of(v_strides);
    const int64_t set = splits * batch * heads * dk * dv;
    DecayParams p{};

@@ -7,7 +7,7 @@
 namespace fufft {
 namespace layer {
 
-constexpr int64_t kWidestHead = 128;
+constexpr int64_t kWidestHead = 128, kLongestText = (int64_t)1 << 30;
 
 // in elements; the elements of a head are adjacent
 struct Strides {
