@@ -103,7 +103,7 @@ __device__ inline Raw<T, N> raw_of(const T* p, const T* first, int count)
    Raw<T, N> x{};
 #pragma unroll
    for(int j = 0; j < N; j++) {
-      const T e = *(j < count ? p + j : first);
+      const T e = *(j == 0 || j < count ? p + j : first);
       if constexpr(sizeof(T) == 4) x.w[j] = __builtin_bit_cast(uint32_t, e);
       else x.w[j / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, e) << (j % 2 * 16);
    }
@@ -217,9 +217,10 @@ decay_chunks(DecayParams p)
       len = p.lens[b];
       len = len < 0 ? 0 : len > p.tokens ? p.tokens : len;
    }
-   const int64_t first = seg * p.segment;
+   const int64_t first = seg * (LOCAL ? p.part : p.segment);
    if(first >= len && seg > 0) return;
-   const int left = (int)(len - first < p.segment ? len - first : p.segment);     // this segment's tokens
+   const int64_t most = LOCAL ? p.part : p.segment;
+   const int left = (int)(len - first < most ? len - first : most);      // this segment's tokens
    if(LOCAL && first + left >= len) return;                    // the last segment's part is not asked for
    const int dk = role.dk, dv = role.dv, dv0 = slice * DV;
    if(dv0 >= dv) return;                                       // a role of fewer slices
@@ -250,21 +251,20 @@ decay_chunks(DecayParams p)
    const int64_t kstep = dir * role.sk.token, vstep = dir * role.sv.token;
    Pair kr[8], vr[8];
    auto token = [](int i) { return i < 4 ? i : i + 12; };
-   auto fetch_pairs = [&](Pair (&to)[8], const T* base, int64_t step, int t, int c, int dim, int n, int t0) {
-      const int channels = anew(dim);
-      const int64_t by = anew(step);
-      const T* const at = base + (t0 + t) * step + (c < channels ? c : 0);
-#pragma unroll
-      for(int i = 0; i < 8; i++) {
-         const T* const from = t + token(i) < n ? at + token(i) * by : base;
-         if constexpr(WHOLE) to[i] = raw_at<T, 2>(from);
-         else                to[i] = raw_of<T, 2>(from, from, channels - c);
-      }
+   // where this lane's first token of the segment is; the others are multiples of a step on, which scalar
+   // code makes (as products of each lane's they took 16 clocks each)
+   const T* const klane = k + kt * kstep + (kc < dk ? kc : 0);
+   const T* const vlane = v + vt * vstep + (vc < dvn ? vc : 0);
+   auto fetch_pair = [&](Pair& to, const T* at, const T* base, int64_t step, int t, int c, int dim, int n, int t0, int i) {
+      const T* const from = t + token(i) < n ? at + (t0 + token(i)) * anew(step) : base;
+      if constexpr(WHOLE) to = raw_at<T, 2>(from);
+      else                to = raw_of<T, 2>(from, from, anew(dim) - c);
    };
-   auto fetch = [&](int t0) {
+   // tokens i of chunk t0
+   auto fetch = [&](int t0, int i) {
       const int n = left - t0 < kChunk ? left - t0 : kChunk;
-      if(has_k) fetch_pairs(kr, k, kstep, kt, kc, dk, n, t0);
-      if(has_v) fetch_pairs(vr, v, vstep, vt, vc, dvn, n, t0);
+      if(has_k) fetch_pair(kr[i], klane, k, kstep, kt, kc, dk, n, t0, i);
+      if(has_v) fetch_pair(vr[i], vlane, v, vstep, vt, vc, dvn, n, t0, i);
    };
    // clears what is not there
    auto clear = [&](Pair (&x)[8], int t, int c, int dim, int n) {
@@ -277,17 +277,19 @@ decay_chunks(DecayParams p)
    // 8 strips' blocks of scores between them
    const int strip = wave < 4 ? wave : 7 - wave, half = wave >> 2;
    const int v0 = half * (DV / 2), k0 = (wave & 3) * (DK / 4);
+   T* const olane = out + (strip * 16 + row) * ostep;
    constexpr int N = 16 / (int)sizeof(E);                       // values of a piece of an operand
    Raw<T, N> qr[NK];
    const int64_t qstep = dir * role.sq.token;
-   auto fetch_q = [&](int t0) {
+   const T* const qlane = q + (strip * 16 + row) * qstep + g * N;
+   auto fetch_q = [&](int t0, int from_block, int to_block) {
       const int channels = anew(dk);
       const bool there = t0 + strip * 16 + row < left;          // else any row: its results are not kept
-      const T* const at = q + (there ? (t0 + strip * 16 + row) * anew(qstep) : 0);
+      const T* const at = there ? qlane + t0 * anew(qstep) : q + g * N;
 #pragma unroll
-      for(int i = 0; i < NK; i++) {
+      for(int i = from_block; i < to_block; i++) {
          const int c = i * BLOCK + g * N;
-         const T* const from = at + (c < channels ? c : 0);
+         const T* const from = at + (c < channels ? i * BLOCK : -g * N);
          if constexpr(WHOLE) qr[i] = raw_at<T, N>(from);
          else                qr[i] = raw_of<T, N>(from, from, channels - c);
       }
@@ -348,7 +350,7 @@ decay_chunks(DecayParams p)
          }
    };
    const float* const from = LOCAL ? nullptr
-                             : p.segments > 1 ? role.work + (seg * p.pairs + bh) * count
+                             : p.segments > 1 ? role.work + (first / p.part * p.pairs + bh) * count
                              : role.state ? role.state + bh * count : nullptr;
    float* const behind = LOCAL ? role.work + (seg * p.pairs + bh) * count
                          : role.new_state && first + left >= len ? role.new_state + bh * count : nullptr;
@@ -359,8 +361,9 @@ decay_chunks(DecayParams p)
    if(from) each_state(p.segments > 1 ? false : role.turned, [&](int a, int c, int r, int at) { S[a][c][r] = from[at]; });
 
    if(left > 0) {
-      fetch(0);
-      if constexpr(!LOCAL) fetch_q(0);
+#pragma unroll
+      for(int i = 0; i < 8; i++) fetch(0, i);
+      if constexpr(!LOCAL) fetch_q(0, 0, NK);
    }
    if(tid < 2) flags[tid] = 0;
    __syncthreads();
@@ -412,7 +415,6 @@ decay_chunks(DecayParams p)
             }
          }
          if(n < kChunk) key_weights(n);
-         const bool odd = C::PARTS == 2 && odd_one(kr);
 #pragma unroll
          for(int j = 0; j < 2; j++) {
             float x[8];
@@ -420,12 +422,9 @@ decay_chunks(DecayParams p)
             for(int i = 0; i < 8; i++) x[i] = kr[i].value(j) * wk[i];
             put_tokens(M::KEYS_T, kc + j, slot_of<E>(kt), x);
             if constexpr(C::PARTS == 2) {
-               // what bf16 leaves of it; nothing of an infinity
+               // what bf16 leaves of it (of an infinity NaN: a key that is infinite makes its row of the state NaN)
 #pragma unroll
                for(int i = 0; i < 8; i++) x[i] -= (float)(bf16)x[i];
-               if(odd)
-#pragma unroll
-                  for(int i = 0; i < 8; i++) x[i] = fabsf(x[i]) < __builtin_inff() ? x[i] : 0.0f;
                put_tokens(M::KEYS_T + DK * TP, kc + j, slot_of<E>(kt), x);
             }
          }
@@ -454,7 +453,18 @@ decay_chunks(DecayParams p)
       auto token_frag = [&](int base, int r, int block) {       // of a row of tokens, r a multiple of 16
          return *reinterpret_cast<const Frag*>(lds + base + (r + row) * TP + ((block * 4 + g) ^ turn(row)) * 16);
       };
-      if(t0 + kChunk < left) fetch(t0 + kChunk);                // on their way under the products
+      // The next chunk's loads go out between the products, a few at a time: a CU takes in 9 bytes a clock at most, and
+      // a wavefront that issues more than are on their way stands still (all 16 at once: 3600 clocks).
+      const int t1 = t0 + kChunk;
+      const bool more = t1 < left;
+      auto fetch_some = [&](int from, int to) {
+         __builtin_amdgcn_sched_barrier(0);
+         if(more)
+#pragma unroll
+            for(int i = from; i < to; i++) fetch(t1, i);
+         __builtin_amdgcn_sched_barrier(0);
+      };
+      if constexpr(LOCAL) fetch_some(0, 8);
 
       if constexpr(!LOCAL) {
          f32x4 o[SB] = {};
@@ -465,13 +475,15 @@ decay_chunks(DecayParams p)
             for(int c = 0; c < SB; c++) x[c] = frag(M::STATE, v0 + c * 16, i);
 #pragma unroll
             for(int c = 0; c < SB; c++) o[c] = C::mma(x[c], qf[i], o[c]);
+            fetch_some(i * 4 / NK, (i + 1) * 4 / NK);
          }
 #pragma unroll
          for(int c = 0; c < SB; c++) o[c] *= wq;
          const int reach = anew_lane(strip * 16 + row - g * 4);      // scores of tokens up to this plus 4 g count
 #pragma unroll
          for(int sb = 0; sb < NS; sb++) {
-            if(sb * EACH > strip) break;
+            fetch_some(4 + sb * 4 / NS, 4 + (sb + 1) * 4 / NS);
+            if(sb * EACH > strip) continue;
             f32x4 s[EACH];
 #pragma unroll
             for(int e = 0; e < EACH; e++) {
@@ -516,16 +528,16 @@ decay_chunks(DecayParams p)
                for(int i = 0; i < EACH * 4; i++)
 #pragma unroll 1
                   for(int from_g = 0; from_g < 4; from_g++) {
-                     const int t1 = sb * BLOCK + (i / 4) * 16 + from_g * 4 + i % 4;
+                     const int s1 = sb * BLOCK + (i / 4) * 16 + from_g * 4 + i % 4;
                      const float weight = __shfl((float)w[i], row + from_g * 16);
-                     if(t1 > strip * 16 + row) continue;
+                     if(s1 > strip * 16 + row) continue;
 #pragma unroll
                      for(int c = 0; c < SB; c++)
 #pragma unroll
                         for(int r = 0; r < 4; r++) {
                            const int channel = v0 + c * 16 + g * 4 + r;
                            const float x = (float)*reinterpret_cast<const E*>(
-                              lds + M::VALUES + channel * TP + (slot_of<E>(t1) ^ turn(channel)) * 16 + in_slot<E>(t1));
+                              lds + M::VALUES + channel * TP + (slot_of<E>(s1) ^ turn(channel)) * 16 + in_slot<E>(s1));
                            if(!(fabsf(x) < __builtin_inff())) o[c][r] += weight * x;
                         }
                   }
@@ -534,7 +546,7 @@ decay_chunks(DecayParams p)
          const int t = strip * 16 + row;
          if(t < n) {
             const int d = anew(dvn);
-            T* const to = out + (t0 + t) * ostep;
+            T* const to = olane + t0 * anew(ostep);
             struct __attribute__((packed, aligned(sizeof(T)))) Four { T e[4]; };
 #pragma unroll
             for(int c = 0; c < SB; c++) {
@@ -552,8 +564,6 @@ decay_chunks(DecayParams p)
             }
          }
       }
-      if constexpr(!LOCAL)
-         if(t0 + kChunk < left) fetch_q(t0 + kChunk);
       // the state behind the chunk
       const float an = power(g2, (float)n);
 #pragma unroll
@@ -563,6 +573,8 @@ decay_chunks(DecayParams p)
 #pragma unroll
       for(int sb = 0; sb < NS; sb++) {
          Frag x[SB], w[SA][C::PARTS];
+         if constexpr(!LOCAL)
+            if(more) fetch_q(t1, sb * NK / NS, (sb + 1) * NK / NS);
 #pragma unroll
          for(int c = 0; c < SB; c++) x[c] = token_frag(M::VALUES, v0 + c * 16, sb);
 #pragma unroll
@@ -582,8 +594,8 @@ decay_chunks(DecayParams p)
    if(behind) each_state(!LOCAL && role.turned, [&](int a, int c, int r, int at) { behind[at] = S[a][c][r]; });
 }
 
-// Every segment's part of the state in work becomes the state before that segment.  A lane has one
-// element of a state; the parts of eight segments are read ahead of their sums.
+// What every part of the tokens adds to the state, in work, becomes the state before that part.  A lane has one
+// element of a state; eight parts are read ahead of their sums.
 __global__ void __launch_bounds__(256)
 decay_scan(DecayParams p)
 {
@@ -599,19 +611,19 @@ decay_scan(DecayParams p)
    }
    float g2 = p.log_decay[h] * 1.44269504f;
    g2 = g2 < -1e30f ? -1e30f : g2;
-   const float a = power(g2, (float)p.segment);                  // every segment but the last is whole
+   const float a = power(g2, (float)p.part);                  // every part but the last is whole
    float s = 0.0f;
    if(role.state) s = role.state[bh * count + (role.turned ? e % role.dv * role.dk + e / role.dv : e)];
    float* const work = role.work + bh * count + e;
    const int64_t pitch = p.pairs * count;
    constexpr int AHEAD = 8;
-   for(int64_t seg = 0; seg < p.segments && (seg == 0 || seg * p.segment < len); seg += AHEAD) {
+   for(int64_t seg = 0; seg < p.parts && (seg == 0 || seg * p.part < len); seg += AHEAD) {
       float part[AHEAD];
 #pragma unroll
-      for(int i = 0; i < AHEAD; i++) part[i] = (seg + i + 1) * p.segment < len ? work[(seg + i) * pitch] : 0.0f;
+      for(int i = 0; i < AHEAD; i++) part[i] = (seg + i + 1) * p.part < len ? work[(seg + i) * pitch] : 0.0f;
 #pragma unroll
       for(int i = 0; i < AHEAD; i++) {
-         if(seg + i < p.segments && (seg + i == 0 || (seg + i) * p.segment < len)) work[(seg + i) * pitch] = s;
+         if(seg + i < p.parts && (seg + i == 0 || (seg + i) * p.part < len)) work[(seg + i) * pitch] = s;
          s = a * s + part[i];
       }
    }
@@ -722,7 +734,7 @@ hipError_t chunks_shape(DecayParams p, int roles, hipStream_t s)
    int most = 0;
    for(int r = 0; r < roles; r++) most = p.role[r].dv > most ? p.role[r].dv : most;
    p.slices = (most + DV - 1) / DV;
-   p.items = p.pairs * (LOCAL ? p.segments - 1 : p.segments);
+   p.items = p.pairs * (LOCAL ? p.parts - 1 : p.segments);
    const int64_t groups = (p.items + 7) / 8 * 8 * p.slices;
    if(!grid_ok(groups, kLanes)) return kTooLarge;
    decay_chunks<T, DK, DV, LOCAL, WHOLE><<<dim3((unsigned)groups, (unsigned)roles), kLanes, bytes, s>>>(p);
@@ -732,7 +744,9 @@ hipError_t chunks_shape(DecayParams p, int roles, hipStream_t s)
 template<class T, int DK, int DV, bool WHOLE>
 hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
 {
-   // Segments so that each CU has as many workgroups as fit its LDS, none of fewer than 4 chunks
+   // Segments so that each CU has as many workgroups as fit its LDS, none of fewer than 4 chunks.  Each is one to
+   // PARTS parts in the first launch, which has room for more workgroups on a CU.
+   constexpr int64_t PARTS = 2;
    const int64_t chunks = (p.tokens + kChunk - 1) / kChunk;
    const int64_t groups = p.pairs * roles * ((p.role[0].dv + DV - 1) / DV);
    const int64_t fit = 256 * (160 * 1024 / Room<T, DK, DV, false>::BYTES);
@@ -740,9 +754,13 @@ hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
    if(n > p.splits) n = p.splits;
    if(n > chunks / 4) n = chunks / 4;
    if(n < 1) n = 1;
-   const int64_t each = chunks > 0 ? (chunks + n - 1) / n : 1;
-   p.segment = each * kChunk;
-   p.segments = chunks > 0 ? (chunks + each - 1) / each : 1;
+   int64_t parts = p.splits / n < PARTS ? p.splits / n : PARTS;
+   if(parts < 1) parts = 1;
+   const int64_t each = chunks > 0 ? (chunks + n * parts - 1) / (n * parts) : 1;       // chunks of a part
+   p.part = each * kChunk;
+   p.segment = p.part * parts;
+   p.parts = chunks > 0 ? (chunks + each - 1) / each : 1;
+   p.segments = (p.parts + parts - 1) / parts;
    if(p.segments > 1) {
       hipError_t e = chunks_shape<T, DK, DV, true, WHOLE>(p, roles, s);
       if(e != hipSuccess) return e;

@@ -23,7 +23,7 @@ struct DecayRole {
    Strides      sq, sk, sv, so;
    const float* state;       // batch x heads x dk x dv, or dv x dk where turned; or NULL
    float*       new_state;   // the same, or NULL
-   float*       work;        // segments x batch x heads x dk x dv
+   float*       work;        // parts x batch x heads x dk x dv
    int          dk, dv;
    int          turned;
    int          reverse;     // from the last token back
@@ -37,7 +37,7 @@ struct DecayParams {
    const int32_t* lens;      // or NULL
    int64_t        pairs;     // batch x heads
    int64_t        heads, tokens, splits;
-   int64_t        segment, segments, items, slices;     // set by the launch
+   int64_t        segment, segments, part, parts, items, slices;     // set by the launch
    int            type;
 };
 hipError_t launch_decay(const DecayParams& p, int roles, hipStream_t s);
