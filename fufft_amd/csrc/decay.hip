@@ -631,93 +631,98 @@ decay_scan(DecayParams p)
 
 // ---- one token ------------------------------------------------------------------------------
 //
-// A workgroup has 32 values of one sequence and head: 8 lanes of 4 values, 32 rows of the state at a
-// time, all of them on their way at once.  Bound by the state's bytes, read and written once.
-constexpr int kStepValues = 32, kStepRows = 4;          // 4 x 32 rows: dk up to 128
+// A workgroup has 4 LANES values of one sequence and head: LANES lanes of 4 values, 256 / LANES rows of the state at
+// a time, all of them on their way at once.  Bound by the state's bytes, read and written once.
+constexpr int kStepLanes = 256;
 
-template<class T>
-__global__ void __launch_bounds__(256)
+// WHOLE: values in whole fours.  What is not there is read at its row's or column's first place instead, and not written.
+template<class T, int LANES, bool WHOLE>
+__global__ void __launch_bounds__(kStepLanes)
 decay_step(StepParams p)
 {
-   __shared__ float join[4][kStepValues];
+   constexpr int ROWS = kStepLanes / LANES, PASSES = 128 / ROWS;       // dk up to 128
+   __shared__ float join[kStepLanes / 64][LANES * 4];
    __shared__ int taken;
-   struct __attribute__((packed, aligned(4))) Four { float e[4]; };
-   const int tid = threadIdx.x, c = tid & 7, r0 = tid >> 3;
+   const int tid = threadIdx.x, c = tid % LANES, r0 = tid / LANES;
    const int64_t b = blockIdx.x / (p.heads * p.slices), rest = blockIdx.x % (p.heads * p.slices);
    const int64_t h = rest / p.slices;
-   const int j0 = (int)(rest % p.slices) * kStepValues + c * 4;
+   const int first = (int)(rest % p.slices) * LANES * 4, j0 = first + c * 4;
+   T* const out = static_cast<T*>(p.out) + b * p.so.batch + h * p.so.head + first;
    const int64_t slot = p.slots ? p.slots[b] : b;
-   const bool inside = slot >= 0 && slot < p.slot_count;
-   float* const state = inside ? p.state + (slot * p.heads + h) * p.dk * p.dv : nullptr;
-   Four s[kStepRows];
-   float kk[kStepRows], qq[kStepRows];
+   if(slot < 0 || slot >= p.slot_count) {
+      if(tid < LANES * 4 && first + tid < p.dv) out[tid] = (T)0.0f;
+      return;
+   }
+   float* const state = p.state + (slot * p.heads + h) * p.dk * p.dv;
    const T* const q = static_cast<const T*>(p.q) + b * p.sq.batch + h * p.sq.head;
    const T* const k = static_cast<const T*>(p.k) + b * p.sk.batch + h * p.sk.head;
    const T* const v = static_cast<const T*>(p.v) + b * p.sv.batch + h * p.sv.head;
-   const bool whole = j0 + 4 <= p.dv;
+   int at[4];                                              // columns
 #pragma unroll
-   for(int i = 0; i < kStepRows; i++) {
-      const int r = r0 + i * 32;
-      s[i] = Four{};
-      kk[i] = qq[i] = 0.0f;
-      if(inside && r < p.dk) {
-         const float* const at = state + r * p.dv + j0;
-         if(whole) s[i] = *reinterpret_cast<const Four*>(at);
-         else
+   for(int e = 0; e < 4; e++) at[e] = WHOLE ? (j0 < p.dv ? j0 : 0) + e : j0 + e < p.dv ? j0 + e : 0;
+   f32x4 s[PASSES];
+   T kk[PASSES], qq[PASSES];
 #pragma unroll
-            for(int e = 0; e < 4; e++)
-               if(j0 + e < p.dv) s[i].e[e] = at[e];
-         kk[i] = (float)k[r];
-         qq[i] = (float)q[r];
+   for(int i = 0; i < PASSES; i++) {
+      const int r = r0 + i * ROWS < p.dk ? r0 + i * ROWS : 0;
+      if constexpr(WHOLE) {
+         typedef float V __attribute__((ext_vector_type(4), aligned(4)));
+         s[i] = *reinterpret_cast<const V*>(state + r * p.dv + at[0]);
+      } else {
+#pragma unroll
+         for(int e = 0; e < 4; e++) s[i][e] = state[r * p.dv + at[e]];
       }
+      kk[i] = k[r];
+      qq[i] = q[r];
    }
    float vv[4];
 #pragma unroll
-   for(int e = 0; e < 4; e++) vv[e] = j0 + e < p.dv ? (float)v[j0 + e] : 0.0f;
+   for(int e = 0; e < 4; e++) vv[e] = (float)v[at[e]];
    // whether an earlier sequence has the same state
-   bool mine = inside;
+   bool mine = true;
    if(p.slots) {
       if(tid == 0) taken = 0;
       __syncthreads();
       bool found = false;
-      for(int64_t i = tid; i < b; i += 256) found |= p.slots[i] == slot;
+      for(int64_t i = tid; i < b; i += kStepLanes) found |= p.slots[i] == slot;
       if(found) taken = 1;
       __syncthreads();
-      mine = inside && !taken;
+      mine = !taken;
    }
    const float a = expf(p.log_decay[h]);
    float acc[4] = {};
 #pragma unroll
-   for(int i = 0; i < kStepRows; i++) {
+   for(int i = 0; i < PASSES; i++) {
+      const bool there = r0 + i * ROWS < p.dk;
 #pragma unroll
       for(int e = 0; e < 4; e++) {
-         s[i].e[e] = a * s[i].e[e] + kk[i] * vv[e];
-         acc[e] += qq[i] * s[i].e[e];
+         s[i][e] = a * s[i][e] + (float)kk[i] * vv[e];
+         acc[e] += there ? (float)qq[i] * s[i][e] : 0.0f;
       }
-      const int r = r0 + i * 32;
-      if(mine && r < p.dk) {
-         float* const at = state + r * p.dv + j0;
-         if(whole) *reinterpret_cast<Four*>(at) = s[i];
-         else
+      if(mine && there) {
+         float* const to = state + (r0 + i * ROWS) * p.dv;
+         if constexpr(WHOLE) {
+            typedef float V __attribute__((ext_vector_type(4), aligned(4)));
+            if(j0 < p.dv) *reinterpret_cast<V*>(to + j0) = s[i];
+         } else {
 #pragma unroll
             for(int e = 0; e < 4; e++)
-               if(j0 + e < p.dv) at[e] = s[i].e[e];
+               if(j0 + e < p.dv) to[j0 + e] = s[i][e];
+         }
       }
    }
+   // the rows' sums: of a wavefront's lanes, then of the wavefronts in their order
 #pragma unroll
-   for(int e = 0; e < 4; e++) {
-      acc[e] += __shfl_xor(acc[e], 8);
-      acc[e] += __shfl_xor(acc[e], 16);
-      acc[e] += __shfl_xor(acc[e], 32);
-   }
-   if((tid & 63) < 8)
+   for(int e = 0; e < 4; e++)
+#pragma unroll
+      for(int by = LANES; by < 64; by *= 2) acc[e] += __shfl_xor(acc[e], by);
+   if((tid & 63) < LANES)
 #pragma unroll
       for(int e = 0; e < 4; e++) join[tid >> 6][c * 4 + e] = acc[e];
    __syncthreads();
-   const int j = (int)(rest % p.slices) * kStepValues + tid;
-   if(tid < kStepValues && j < p.dv) {
+   if(tid < LANES * 4 && first + tid < p.dv) {
       const float sum = ((join[0][tid] + join[1][tid]) + join[2][tid]) + join[3][tid];
-      static_cast<T*>(p.out)[b * p.so.batch + h * p.so.head + j] = (T)(mine ? sum * p.scale : 0.0f);
+      out[tid] = (T)(mine ? sum * p.scale : 0.0f);
    }
 }
 
@@ -744,18 +749,18 @@ hipError_t chunks_shape(DecayParams p, int roles, hipStream_t s)
 template<class T, int DK, int DV, bool WHOLE>
 hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
 {
-   // Segments so that each CU has as many workgroups as fit its LDS, none of fewer than 4 chunks.  Each is one to
-   // PARTS parts in the first launch, which has room for more workgroups on a CU.
+   // Segments so that each CU has as many workgroups as fit its LDS; below 4 chunks the two launches more cost what
+   // they save.  A segment of several chunks is PARTS parts in the first launch, which has room for more workgroups on
+   // a CU (65536 tokens x 16 heads: 197 us in one part, 152 in 3, 142 in 2).
    constexpr int64_t PARTS = 2;
    const int64_t chunks = (p.tokens + kChunk - 1) / kChunk;
    const int64_t groups = p.pairs * roles * ((p.role[0].dv + DV - 1) / DV);
    const int64_t fit = 256 * (160 * 1024 / Room<T, DK, DV, false>::BYTES);
    int64_t n = fit / (groups > 0 ? groups : 1);
    if(n > p.splits) n = p.splits;
-   if(n > chunks / 4) n = chunks / 4;
-   if(n < 1) n = 1;
-   int64_t parts = p.splits / n < PARTS ? p.splits / n : PARTS;
-   if(parts < 1) parts = 1;
+   if(n > chunks) n = chunks;
+   if(n < 1 || chunks < 4) n = 1;
+   const int64_t parts = p.splits / n >= PARTS && chunks / n >= 2 * PARTS ? PARTS : 1;
    const int64_t each = chunks > 0 ? (chunks + n * parts - 1) / (n * parts) : 1;       // chunks of a part
    p.part = each * kChunk;
    p.segment = p.part * parts;
@@ -825,19 +830,37 @@ hipError_t launch_decay(const DecayParams& p, int roles, hipStream_t s)
    return hipSuccess;
 }
 
-hipError_t launch_decay_step(const StepParams& params, hipStream_t s)
+namespace {
+
+template<class T, int LANES>
+hipError_t step_shape(StepParams p, hipStream_t s)
 {
-   StepParams p = params;
-   p.slices = (p.dv + kStepValues - 1) / kStepValues;
+   p.slices = (p.dv + LANES * 4 - 1) / (LANES * 4);
    const int64_t groups = p.batch * p.heads * p.slices;
-   if(groups <= 0) return hipSuccess;
-   if(!grid_ok(groups, 256)) return kTooLarge;
-   switch(p.type) {
-      case T_F32:  decay_step<float><<<(unsigned)groups, 256, 0, s>>>(p); break;
-      case T_BF16: decay_step<bf16><<<(unsigned)groups, 256, 0, s>>>(p); break;
-      default:     decay_step<f16><<<(unsigned)groups, 256, 0, s>>>(p); break;
-   }
+   if(!grid_ok(groups, kStepLanes)) return kTooLarge;
+   if(p.dv % 4 == 0) decay_step<T, LANES, true><<<(unsigned)groups, kStepLanes, 0, s>>>(p);
+   else              decay_step<T, LANES, false><<<(unsigned)groups, kStepLanes, 0, s>>>(p);
    return hipGetLastError();
+}
+
+// Whole rows of the state a workgroup where there are states enough for all CUs, else 32 values.
+template<class T>
+hipError_t step_typed(const StepParams& p, hipStream_t s)
+{
+   if(p.dv <= 32 || p.batch * p.heads < 512) return step_shape<T, 8>(p, s);
+   return p.dv <= 64 ? step_shape<T, 16>(p, s) : step_shape<T, 32>(p, s);
+}
+
+}  // namespace
+
+hipError_t launch_decay_step(const StepParams& p, hipStream_t s)
+{
+   if(p.batch <= 0 || p.heads <= 0) return hipSuccess;
+   switch(p.type) {
+      case T_F32:  return step_typed<float>(p, s);
+      case T_BF16: return step_typed<bf16>(p, s);
+      default:     return step_typed<f16>(p, s);
+   }
 }
 
 }  // namespace layer

@@ -25,6 +25,76 @@ using mx4::u32x4;
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
+// ---- single tokens: rows of b whole, products of four bytes -------------------------------
+//
+// A wavefront has 4 rows of b and M of a (those that are not there are zeros), the lanes 16 bytes each of 1 KiB
+// of every row; the wavefronts of a workgroup share K, and their sums are joined in LDS.  Bound by b's bytes: a load
+// is 1 KiB of one row, where the matrix cores' operands are 64 bytes of 16 rows (1 x 8192 x 8192 18.8 us so).
+constexpr int kTokenRows = 4;
+
+template<class O, int M, int UNROLL>
+__global__ void __launch_bounds__(512)
+i8_tokens(I8Params p, int64_t row_bytes)
+{
+   __shared__ int join[8][kTokenRows * M];
+   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+   const int waves = blockDim.x >> 6;
+   const int64_t n0 = (int64_t)blockIdx.x * kTokenRows;
+   const int8_t* b[kTokenRows];
+#pragma unroll
+   for(int r = 0; r < kTokenRows; r++) b[r] = p.b + (n0 + r < p.n ? n0 + r : p.n - 1) * row_bytes;
+   int sum[kTokenRows][M] = {};
+   const int64_t step = 1024 * UNROLL;
+   for(int64_t k = wave * step; k < row_bytes; k += waves * step) {
+      i32x4 w[UNROLL][kTokenRows], x[UNROLL][M];
+#pragma unroll
+      for(int u = 0; u < UNROLL; u++) {
+         const int64_t at = k + u * 1024 + lane * 16;
+         const bool in = at < row_bytes;
+         const int64_t from = in ? at : 0;                  // beyond the end: any bytes of b, times zeros
+#pragma unroll
+         for(int r = 0; r < kTokenRows; r++) w[u][r] = *reinterpret_cast<const i32x4*>(b[r] + from);
+#pragma unroll
+         for(int i = 0; i < M; i++) {
+            x[u][i] = *reinterpret_cast<const i32x4*>(p.a + (i < p.m ? i : 0) * row_bytes + from);
+#pragma unroll
+            for(int e = 0; e < 4; e++) x[u][i][e] = in ? x[u][i][e] : 0;
+         }
+      }
+#pragma unroll
+      for(int u = 0; u < UNROLL; u++)
+#pragma unroll
+         for(int i = 0; i < M; i++)
+#pragma unroll
+            for(int r = 0; r < kTokenRows; r++)
+#pragma unroll
+               for(int e = 0; e < 4; e++) sum[r][i] = __builtin_amdgcn_sdot4(w[u][r][e], x[u][i][e], sum[r][i], false);
+   }
+#pragma unroll
+   for(int r = 0; r < kTokenRows; r++)
+#pragma unroll
+      for(int i = 0; i < M; i++) {
+         uint32_t v = (uint32_t)sum[r][i];
+         v += mx4::dpp<mx4::kQuadSwap1>(v);
+         v += mx4::dpp<mx4::kQuadSwap2>(v);
+         v += mx4::dpp<0x141>(v);                            // the mirrors within 8 and 16 lanes
+         v += mx4::dpp<0x140>(v);
+         const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)v, 0) + (uint32_t)__builtin_amdgcn_readlane((int)v, 16) +
+                              (uint32_t)__builtin_amdgcn_readlane((int)v, 32) + (uint32_t)__builtin_amdgcn_readlane((int)v, 48);
+         if(lane == 0) join[wave][i * kTokenRows + r] = (int)all;
+      }
+   __syncthreads();
+   const int i = threadIdx.x / kTokenRows, r = threadIdx.x % kTokenRows;
+   const int64_t n = n0 + r;
+   if(threadIdx.x < kTokenRows * M && i < p.m && n < p.n) {
+      int total = 0;
+      for(int w = 0; w < waves; w++) total += join[w][threadIdx.x];
+      float v = row_bytes ? (float)total * p.a_scales[i] * p.b_scales[n] : 0.0f;
+      if(p.bias) v += p.bias[n];
+      static_cast<O*>(p.out)[i * p.ld + n] = (O)v;
+   }
+}
+
 // ---- few rows: operands straight from memory, K split over the wavefronts ----------
 //
 // A workgroup computes 16 MT rows of a times 16 NT rows of b; its wavefronts take runs of
@@ -113,8 +183,8 @@ i8_rows(I8Params p, int pieces, int waves)
 // ---- many rows: tiles staged in LDS ---------------------------------------------------
 //
 // A workgroup of WM x WN wavefronts computes BM x BN results, a wavefront FM x FN products
-// of 32 x 32.  K goes by slabs of 128 bytes of BM + BN rows.  Two slabs are in LDS, one read, one
-// on its way there straight from memory, so that no register waits for it.  The loads
+// of 32 x 32.  K goes by slabs of 128 bytes of BM + BN rows.  STAGES slabs are in LDS, one read, the others
+// on their way there straight from memory, so that no register waits for them.  The loads
 // write lane after lane, 8 rows of 8 chunks of 16 bytes; slot c of row r gets chunk c ^ (r % 8) ^
 // (r / 8 % 2), so that the lanes of a product, which read one chunk of 32 rows, meet all banks.
 constexpr int kFlags = 0x00020000;     // raw buffer, 32-bit elements
@@ -152,7 +222,7 @@ __device__ inline void tile_of(uint32_t id, uint32_t tm, uint32_t tn, uint32_t* 
    *n = in / high;
 }
 
-template<class O, int BM, int BN, int WM, int WN>
+template<class O, int BM, int BN, int WM, int WN, int STAGES>
 __global__ void __launch_bounds__(64 * WM * WN)
 i8_tiles(I8Params p, uint32_t slabs, uint32_t tm, uint32_t tn)
 {
@@ -180,12 +250,15 @@ i8_tiles(I8Params p, uint32_t slabs, uint32_t tm, uint32_t tn)
       const uint32_t chunk = (lane & 7) ^ (lane >> 3) ^ (r8 & 1);
       voff[j] = (uint32_t)in * row_bytes + chunk * 16;
    }
+   // slab s to its place among the STAGES; beyond the last one that again, so that all wavefronts always have the same
+   // number of fetches on their way
    auto fetch_slab = [&](uint32_t s) {
-      uint8_t* const to = lds + (s & 1) * SLAB + wave * JOBS * 1024;
+      uint8_t* const to = lds + s % STAGES * SLAB + wave * JOBS * 1024;
+      const uint32_t from = s < slabs ? s : slabs - 1;
 #pragma unroll
       for(int j = 0; j < JOBS; j++) {
          const int row = (wave * JOBS + j) * 8;
-         fetch16(row < BM ? ra : rb, to + j * 1024, voff[j], s * 128);
+         fetch16(row < BM ? ra : rb, to + j * 1024, voff[j], from * 128);
       }
    };
    const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
@@ -197,34 +270,57 @@ i8_tiles(I8Params p, uint32_t slabs, uint32_t tm, uint32_t tn)
    const uint32_t turn = (lane & 7) ^ ((lane >> 3) & 1);       // the slot's turn of this lane's rows
 
    i32x16 acc[FM][FN] = {};
-   if(slabs) fetch_slab(0);
-   for(uint32_t s = 0; s < slabs; s++) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+   // Operands of a step of 32 bytes are read while the step before is multiplied, those of a slab's first step under the
+   // last one of the slab before: the barrier between slabs, after which one may be read and the other
+   // overwritten, stands before that last step's products.
+   struct Step {
+      i32x4 x[FM], w[FN];
+   };
+   auto read = [&](Step& to, uint32_t slab, int t) {
+      const uint8_t* const data = lds + slab % STAGES * SLAB;
+      const uint32_t slot = ((2 * t + half) ^ turn) * 16;
+#pragma unroll
+      for(int b = 0; b < FN; b++) to.w[b] = *reinterpret_cast<const i32x4*>(data + wat[b] * 128 + slot);
+#pragma unroll
+      for(int a = 0; a < FM; a++) to.x[a] = *reinterpret_cast<const i32x4*>(data + xat[a] * 128 + slot);
+   };
+   auto multiply = [&](const Step& f) {
+#pragma unroll
+      for(int a = 0; a < FM; a++)
+#pragma unroll
+         for(int b = 0; b < FN; b++) acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[b], f.x[a], acc[a][b], 0, 0, 0);
+   };
+   Step even, odd;
+   if(slabs) {
+#pragma unroll
+      for(int i = 0; i < STAGES; i++) fetch_slab(i);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * JOBS) : "memory");
       __syncthreads();
-      if(s + 1 < slabs) fetch_slab(s + 1);
-      const uint8_t* const data = lds + (s & 1) * SLAB;
-#pragma unroll
-      for(int t = 0; t < 4; t++) {
-         const uint32_t slot = ((2 * t + half) ^ turn) * 16;
-         i32x4 x[FM], w[FN];
-#pragma unroll
-         for(int b = 0; b < FN; b++) w[b] = *reinterpret_cast<const i32x4*>(data + wat[b] * 128 + slot);
-#pragma unroll
-         for(int a = 0; a < FM; a++) x[a] = *reinterpret_cast<const i32x4*>(data + xat[a] * 128 + slot);
-#pragma unroll
-         for(int a = 0; a < FM; a++)
-#pragma unroll
-            for(int b = 0; b < FN; b++)
-               acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[b], x[a], acc[a][b], 0, 0, 0);
-      }
+      read(even, 0, 0);
    }
+   for(uint32_t s = 0; s < slabs; s++) {
+      read(odd, s, 1);
+      multiply(even);
+      read(even, s, 2);
+      multiply(odd);
+      read(odd, s, 3);
+      multiply(even);
+      if(s + 1 < slabs) {
+         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * JOBS) : "memory");
+         __syncthreads();
+         fetch_slab(s + STAGES);
+         read(even, s + 1, 0);
+      }
+      multiply(odd);
+   }
+   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // nothing is on its way to the LDS that the results take
    // scales and bias beyond the matrix, or not given, are zeros
    const __amdgpu_buffer_rsrc_t rsa = buffer(p.a_scales + m0, slabs ? ml * 4 : 0);
    const __amdgpu_buffer_rsrc_t rsb = buffer(p.b_scales + n0, slabs ? nl * 4 : 0);
    const __amdgpu_buffer_rsrc_t rbias = buffer(p.bias + n0, p.bias ? nl * 4 : 0);
    // Each wavefront turns its results in its share of the LDS and stores whole 16-byte pieces of
    // rows.
-   constexpr int COLS = FN * 32, PITCH = COLS * (int)sizeof(O) + 16, SHARE = 2 * SLAB / WAVES;
+   constexpr int COLS = FN * 32, PITCH = COLS * (int)sizeof(O) + 16, SHARE = STAGES * SLAB / WAVES;
    constexpr int ROOM = SHARE / (32 * PITCH);
    constexpr int PASS = ROOM >= FM ? FM : ROOM >= 2 && FM % 2 == 0 ? 2 : 1;       // 32-row parts at a time
    static_assert(ROOM > 0 && FM % PASS == 0, "a wavefront's share of the LDS holds whole parts");
@@ -278,16 +374,16 @@ i8_tiles(I8Params p, uint32_t slabs, uint32_t tm, uint32_t tn)
    }
 }
 
-template<class O, int BM, int BN, int WM, int WN>
+template<class O, int BM, int BN, int WM, int WN, int STAGES>
 hipError_t tiles_shape(const I8Params& p, hipStream_t s)
 {
-   constexpr size_t bytes = (size_t)(BM + BN) * 256;
+   constexpr size_t bytes = (size_t)(BM + BN) * 128 * STAGES;
    const int64_t slabs = padded(p.k) / 128, tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
    if(!grid_ok(tm * tn, 64 * WM * WN)) return kTooLarge;
    static std::atomic<uint64_t> mask{0};
-   const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(&i8_tiles<O, BM, BN, WM, WN>), bytes, mask);
+   const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(&i8_tiles<O, BM, BN, WM, WN, STAGES>), bytes, mask);
    if(e != hipSuccess) return e;
-   i8_tiles<O, BM, BN, WM, WN><<<(unsigned)(tm * tn), 64 * WM * WN, bytes, s>>>(p, (uint32_t)slabs, (uint32_t)tm,
+   i8_tiles<O, BM, BN, WM, WN, STAGES><<<(unsigned)(tm * tn), 64 * WM * WN, bytes, s>>>(p, (uint32_t)slabs, (uint32_t)tm,
                                                                                (uint32_t)tn);
    return hipGetLastError();
 }
@@ -312,24 +408,49 @@ hipError_t rows_shape(const I8Params& p, hipStream_t s)
    return hipGetLastError();
 }
 
+template<class O, int M>
+hipError_t tokens_shape(const I8Params& p, hipStream_t s)
+{
+   // K shared until there are 16 wavefronts a CU or each has its last KiB
+   const int64_t row_bytes = padded(p.k), groups = (p.n + kTokenRows - 1) / kTokenRows;
+   constexpr int UNROLL = M <= 4 ? 2 : 1;
+   int waves = 1;
+   while(waves < 8 && waves * 1024 * UNROLL < row_bytes && groups * waves < 16 * 256) waves *= 2;
+   if(!grid_ok(groups, waves * 64)) return kTooLarge;
+   i8_tokens<O, M, UNROLL><<<(unsigned)groups, waves * 64, 0, s>>>(p, row_bytes);
+   return hipGetLastError();
+}
+
 int64_t tiles(const I8Params& p, int64_t rows, int64_t cols)
 {
    return ((p.m + rows - 1) / rows) * ((p.n + cols - 1) / cols);
 }
 
+// The kernel for a size, on MI355X's 256 CUs; us at m x n x k.
+//   Up to 8 rows: four-byte products, 1 KiB of a row of b a load (16 rows on the matrix cores / so: 1 x 8192 x 8192
+//     18.8 / 12.3, 1 x 16384 x 8192 37.4 / 23.6, 8 x 16384 x 8192 37 / 29; 8 x 8192 x 8192 21.0 / 21.9).
+//   K split over wavefronts, operands straight from memory, where at most 256 workgroups of 16 or 32 rows by 16
+//     columns have all results and K is long, and up to 16 rows by 8192 columns (against 64 x 64 staged: 24 x 4096 x
+//     4096 8.4 / 10.7, 100 x 100 x 1024 3.8 / 5.2, 16 x 8192 x 8192 19.9 / 21.5; but 16 x 16384 x 8192 37.2 / 24.9).
+//   Staged tiles: 256 x 256, one a CU, against 128 x 128, two a CU, by the rounds that each needs; 64 x 64, four slabs
+//     on their way, below 256 tiles of 128 x 128 (128 x 4096 x 4096 10.9 / 21.8, 1001 x 2000 x 1504 9.7 / 12.7; with two
+//     slabs 128 x 4096 x 4096 16.8, 64 x 16384 x 8192 48.6 / 27.1).
 template<class O>
 hipError_t matmul_typed(const I8Params& p, hipStream_t s)
 {
-   if(p.m <= 16) return p.n > 16 * 256 ? rows_shape<O, 1, 2, 2>(p, s) : rows_shape<O, 1, 1, 2>(p, s);
+   if(p.m <= 1) return tokens_shape<O, 1>(p, s);
+   if(p.m <= 2) return tokens_shape<O, 2>(p, s);
+   if(p.m <= 4) return tokens_shape<O, 4>(p, s);
+   if(p.m <= 8) return tokens_shape<O, 8>(p, s);
+   if(p.m <= 16 && p.n <= 16 * 512) return p.n > 16 * 256 ? rows_shape<O, 1, 2, 2>(p, s) : rows_shape<O, 1, 1, 2>(p, s);
    if(p.k >= 1024) {
       if(tiles(p, 16, 16) <= 256) return rows_shape<O, 1, 1, 2>(p, s);
       if(tiles(p, 32, 16) <= 256) return rows_shape<O, 2, 1, 2>(p, s);
-      if(tiles(p, 32, 32) <= 256) return rows_shape<O, 2, 2, 2>(p, s);
    }
    const int64_t big = tiles(p, 256, 256), mid = tiles(p, 128, 128);
-   if(5 * ((big + 255) / 256) <= 3 * ((mid + 511) / 512)) return tiles_shape<O, 256, 256, 2, 4>(p, s);
-   if(mid >= 256) return tiles_shape<O, 128, 128, 2, 2>(p, s);
-   return tiles_shape<O, 64, 64, 2, 2>(p, s);
+   if(5 * ((big + 255) / 256) <= 3 * ((mid + 511) / 512)) return tiles_shape<O, 256, 256, 2, 4, 2>(p, s);
+   if(mid >= 256) return tiles_shape<O, 128, 128, 2, 2, 2>(p, s);
+   return tiles_shape<O, 64, 64, 2, 2, 4>(p, s);
 }
 
 }  // namespace
