@@ -37,6 +37,12 @@ __device__ inline Eight<T> fetch8(const T* row, int64_t col, int64_t k)
    for(int i = 0; i < 8; i++) v.e[i] = col + i < k ? row[col + i] : (T)0.0f;
    return v;
 }
+// the same where k is a multiple of 8: no branch, the row's first eight in place of those that are not there
+template<class T>
+__device__ inline Eight<T> fetch8_whole(const T* row, int64_t col, int64_t k)
+{
+   return *reinterpret_cast<const Eight<T>*>(row + (col < k ? col : 0));
+}
 template<class T>
 __device__ inline void put8(T* row, int64_t col, int64_t k, const float (&v)[8])
 {
@@ -57,30 +63,52 @@ __device__ inline float lane_value(float v, int lane)
 {
    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
-// the sum over the 64 lanes, the same in all of them: within rows of 16 by DPP, then the four rows
-__device__ inline float wave_sum(float v)
+// over 16 lanes by DPP, the same in all of them
+__device__ inline float sum16(float v)
 {
    v += __uint_as_float(dpp<mx4::kQuadSwap1>(__float_as_uint(v)));
    v += __uint_as_float(dpp<mx4::kQuadSwap2>(__float_as_uint(v)));
    v += __uint_as_float(dpp<kHalfMirror>(__float_as_uint(v)));
-   v += __uint_as_float(dpp<kMirror>(__float_as_uint(v)));
-   return (lane_value(v, 0) + lane_value(v, 16)) + (lane_value(v, 32) + lane_value(v, 48));
+   return v + __uint_as_float(dpp<kMirror>(__float_as_uint(v)));
 }
-__device__ inline uint32_t wave_max(uint32_t v)
+__device__ inline uint32_t max16(uint32_t v)
 {
    v = umax(v, dpp<mx4::kQuadSwap1>(v));
    v = umax(v, dpp<mx4::kQuadSwap2>(v));
    v = umax(v, dpp<kHalfMirror>(v));
-   v = umax(v, dpp<kMirror>(v));
+   return umax(v, dpp<kMirror>(v));
+}
+__device__ inline float sum4(float v)
+{
+   v += __uint_as_float(dpp<mx4::kQuadSwap1>(__float_as_uint(v)));
+   return v + __uint_as_float(dpp<mx4::kQuadSwap2>(__float_as_uint(v)));
+}
+__device__ inline uint32_t max4(uint32_t v)
+{
+   v = umax(v, dpp<mx4::kQuadSwap1>(v));
+   return umax(v, dpp<mx4::kQuadSwap2>(v));
+}
+// over the wavefront: the four sixteens
+__device__ inline float wave_sum(float v)
+{
+   v = sum16(v);
+   return (lane_value(v, 0) + lane_value(v, 16)) + (lane_value(v, 32) + lane_value(v, 48));
+}
+__device__ inline uint32_t wave_max(uint32_t v)
+{
+   v = max16(v);
    const uint32_t a = umax(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
    return umax(a, umax(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
 
-// Over LANES lanes; `turn` counts a row's uses of the exchange, which has two sides so that
-// one barrier a use is enough.
+// Over the LANES lanes of a row, several rows a workgroup.  `turn` counts the uses of the exchange between
+// wavefronts, which has two sides so that one barrier a use is enough; all rows of a workgroup
+// come to it alike.
 template<int LANES>
 __device__ inline float row_sum(float v, uint32_t (&side)[2][16], int& turn)
 {
+   if constexpr(LANES == 4) return sum4(v);
+   if constexpr(LANES == 16) return sum16(v);
    v = wave_sum(v);
    if constexpr(LANES == 64) return v;
    uint32_t* const at = side[turn++ & 1];
@@ -88,12 +116,34 @@ __device__ inline float row_sum(float v, uint32_t (&side)[2][16], int& turn)
    __syncthreads();
    float s = 0.0f;
 #pragma unroll
-   for(int w = 0; w < LANES / 64; w++) s += __uint_as_float(at[w]);
+   for(int w = 0; w < LANES / 64; w++) s += __uint_as_float(at[threadIdx.x / LANES * (LANES / 64) + w]);
    return s;
+}
+// three sums in one exchange, up to 4 wavefronts
+template<int LANES>
+__device__ inline void row_sums(float (&v)[3], uint32_t (&side)[2][16], int& turn)
+{
+   static_assert(LANES > 64 && LANES <= 256, "");
+   __shared__ float more[2][3][16];
+   const int t = turn++ & 1, first = threadIdx.x / LANES * (LANES / 64);
+#pragma unroll
+   for(int i = 0; i < 3; i++) {
+      v[i] = wave_sum(v[i]);
+      if((threadIdx.x & 63) == 0) more[t][i][threadIdx.x >> 6] = v[i];
+   }
+   __syncthreads();
+#pragma unroll
+   for(int i = 0; i < 3; i++) {
+      v[i] = 0.0f;
+#pragma unroll
+      for(int w = 0; w < LANES / 64; w++) v[i] += more[t][i][first + w];
+   }
 }
 template<int LANES>
 __device__ inline uint32_t row_max(uint32_t v, uint32_t (&side)[2][16], int& turn)
 {
+   if constexpr(LANES == 4) return max4(v);
+   if constexpr(LANES == 16) return max16(v);
    v = wave_max(v);
    if constexpr(LANES == 64) return v;
    uint32_t* const at = side[turn++ & 1];
@@ -101,7 +151,7 @@ __device__ inline uint32_t row_max(uint32_t v, uint32_t (&side)[2][16], int& tur
    __syncthreads();
    uint32_t m = 0;
 #pragma unroll
-   for(int w = 0; w < LANES / 64; w++) m = umax(m, at[w]);
+   for(int w = 0; w < LANES / 64; w++) m = umax(m, at[threadIdx.x / LANES * (LANES / 64) + w]);
    return m;
 }
 
@@ -114,25 +164,35 @@ __device__ inline float squares(const float (&h)[8], float c)
 {
    float ss = 0.0f;
 #pragma unroll
-   for(int i = 0; i < 8; i++) ss += (h[i] * c) * (h[i] * c);
+   for(int i = 0; i < 8; i++) ss = __builtin_fmaf(h[i] * c, h[i] * c, ss);
    return ss;
 }
 // part(c): the lane's share of the sum of (h c)^2
-template<int LANES, class F>
+template<int LANES, int ROWS, class F>
 __device__ inline Factors factors_from(F part, int64_t k, float eps, uint32_t (&side)[2][16], int& turn)
 {
-   float c = 1.0f, ss = row_sum<LANES>(part(c), side, turn);
-   const bool large = !(ss < __builtin_inff()), small = ss < 0x1p-60f && eps < 0x1p-60f;
-   if(large || small) {                 // the same in all lanes of the row
-      c = large ? 0x1p-80f : 0x1p+80f;
-      ss = row_sum<LANES>(part(c), side, turn);
+   constexpr float DOWN = 0x1p-80f, UP = 0x1p+80f;
+   if constexpr(ROWS > 1 && LANES > 64) {
+      // rows that share barriers cannot go back for another sum: all three in one exchange
+      float sums[3] = {part(1.0f), part(DOWN), part(UP)};
+      row_sums<LANES>(sums, side, turn);
+      const bool large = !(sums[0] < __builtin_inff()), small = sums[0] < 0x1p-60f && eps < 0x1p-60f;
+      const float c = large ? DOWN : small ? UP : 1.0f, ss = large ? sums[1] : small ? sums[2] : sums[0];
+      return {c, 1.0f / sqrtf(ss / (float)k + (eps * c) * c)};
+   } else {
+      float c = 1.0f, ss = row_sum<LANES>(part(c), side, turn);
+      const bool large = !(ss < __builtin_inff()), small = ss < 0x1p-60f && eps < 0x1p-60f;
+      if(large || small) {                 // the same in all lanes of the row
+         c = large ? DOWN : UP;
+         ss = row_sum<LANES>(part(c), side, turn);
+      }
+      return {c, 1.0f / sqrtf(ss / (float)k + (eps * c) * c)};
    }
-   return {c, 1.0f / sqrtf(ss / (float)k + (eps * c) * c)};
 }
-template<int LANES, int V>
+template<int LANES, int ROWS, int V>
 __device__ inline Factors factors_of(const float (&h)[V][8], int64_t k, float eps, uint32_t (&side)[2][16], int& turn)
 {
-   return factors_from<LANES>([&](float c) {
+   return factors_from<LANES, ROWS>([&](float c) {
       float ss = 0.0f;
 #pragma unroll
       for(int v = 0; v < V; v++) ss += squares(h[v], c);
@@ -188,7 +248,7 @@ __device__ inline u32x2 codes8(const float (&y)[8], const Step& s)
 
 // ---- the norm, and rows to 8 bits (NORM false: y = x) -----------------------------------
 //
-// LANES lanes have a row, V vectors of 8 elements each; a workgroup of 256 has 4 rows at 64.
+// LANES lanes have a row, V vectors of 8 elements each; a workgroup of 256 has 64 rows at 4 lanes, 16 at 16, 4 at 64.
 template<class X, class S, int LANES, int V, bool NORM>
 __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES)
 norm_rows(NormParams p, int64_t kp)
@@ -197,7 +257,7 @@ norm_rows(NormParams p, int64_t kp)
    constexpr int PER = LANES < 256 ? 256 / LANES : 1;
    const int lane = threadIdx.x % LANES;
    const int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
-   if(row >= p.rows) return;                     // whole wavefronts; with more lanes a row, never
+   if(row >= p.rows) return;                     // all lanes of a row, which meet no barrier where rows share a workgroup
    const X* const x = static_cast<const X*>(p.x) + row * p.ldx;
    int turn = 0;
    float h[V][8];
@@ -222,7 +282,7 @@ norm_rows(NormParams p, int64_t kp)
       }
    }
    if constexpr(NORM) {
-      const Factors f = factors_of<LANES, V>(h, p.k, p.eps, side, turn);
+      const Factors f = factors_of<LANES, PER, V>(h, p.k, p.eps, side, turn);
       S* const total = p.total ? static_cast<S*>(p.total) + row * p.ldt : nullptr;
       X* const out = p.out ? static_cast<X*>(p.out) + row * p.ldo : nullptr;
 #pragma unroll
@@ -284,7 +344,7 @@ norm_long(NormParams p, int64_t kp)
    };
    Factors f{1.0f, 1.0f};
    if constexpr(NORM)
-      f = factors_from<1024>([&](float c) {
+      f = factors_from<1024, 1>([&](float c) {
          float ss = 0.0f;
          for(int64_t col = threadIdx.x * 8; col < p.k; col += 8192) {
             float h[8];
@@ -349,78 +409,106 @@ dequantize_rows(const int8_t* codes, const float* scales, O* out, int64_t ld, in
 
 // ---- the norm's gradients ----------------------------------------------------------------
 //
-// Workgroup i of `groups` has rows i, i + groups, .. (times PER), and the sums of its rows'
-// part of dweight in registers; the next row's values are on their way while one is summed.
+// Workgroup i of `groups` has PER rows from PER i on, then every PER groups'th, and the sums of its rows' part of
+// dweight in registers; the next row's values are on their way while one is summed (not with V > 1, which
+// has no registers for it).  8 elements a lane: more wavefronts to a row wait for each other, but as many
+// more loads are on their way (8192 x 4096 in bf16 with 256 lanes of 16 elements 79 us).  V > 1 is for widths
+// in whole eights.
+constexpr int kGradBlock = 512;
+
 template<class D, class S, class O, int LANES, int V>
-__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES)
+__global__ void __launch_bounds__(LANES < kGradBlock ? kGradBlock : LANES)
 norm_grad_rows(NormGradParams p, int64_t groups)
 {
    __shared__ uint32_t side[2][16];
-   constexpr int PER = LANES < 256 ? 256 / LANES : 1;
-   const int lane = threadIdx.x % LANES;
+   constexpr int PER = LANES < kGradBlock ? kGradBlock / LANES : 1;
+   const int lane = threadIdx.x % LANES, mine = threadIdx.x / LANES;
    const int64_t step = groups * PER;
    int turn = 0;
    Eight<D> dy[V];
    Eight<S> hh[V], dt[V];
+   // rows beyond the last read that one
    auto fetch = [&](int64_t row) {
+      const int64_t r = row < p.rows ? row : p.rows - 1;
 #pragma unroll
       for(int v = 0; v < V; v++) {
          const int64_t col = (int64_t)(v * LANES + lane) * 8;
-         dy[v] = fetch8<D>(static_cast<const D*>(p.dy) + row * p.ldy, col, p.k);
-         hh[v] = fetch8<S>(static_cast<const S*>(p.h) + row * p.ldh, col, p.k);
-         if(p.dtotal) dt[v] = fetch8<S>(static_cast<const S*>(p.dtotal) + row * p.ldt, col, p.k);
+         const D* const y = static_cast<const D*>(p.dy) + r * p.ldy;
+         const S* const x = static_cast<const S*>(p.h) + r * p.ldh;
+         const S* const t = static_cast<const S*>(p.dtotal) + r * p.ldt;
+         dy[v] = V > 1 ? fetch8_whole<D>(y, col, p.k) : fetch8<D>(y, col, p.k);
+         hh[v] = V > 1 ? fetch8_whole<S>(x, col, p.k) : fetch8<S>(x, col, p.k);
+         if(V == 1 && p.dtotal) dt[v] = fetch8<S>(t, col, p.k);
       }
    };
    float dw[V][8] = {};
-   int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
-   if(row < p.rows) fetch(row);
-   for(; row < p.rows; row += step) {
-      float g[V][8], h[V][8], through[V][8];
+   int64_t row0 = (int64_t)blockIdx.x * PER;
+   if(V == 1) fetch(row0 + mine);
+   for(; row0 < p.rows; row0 += step) {
+      const int64_t row = row0 + mine;
+      const bool there = row < p.rows;
+      if(V > 1) fetch(row);
+      float g[V][8], h[V][8], through[8];
 #pragma unroll
       for(int v = 0; v < V; v++)
 #pragma unroll
          for(int i = 0; i < 8; i++) {
-            g[v][i] = (float)dy[v].e[i];
-            h[v][i] = (float)hh[v].e[i];
-            through[v][i] = p.dtotal ? (float)dt[v].e[i] : 0.0f;
+            const bool in = there && (V == 1 || (v * LANES + lane) * 8 < p.k);
+            g[v][i] = in ? (float)dy[v].e[i] : 0.0f;
+            h[v][i] = in ? (float)hh[v].e[i] : 0.0f;
+            if(V == 1) through[i] = p.dtotal ? (float)dt[0].e[i] : 0.0f;
          }
-      if(row + step < p.rows) fetch(row + step);
-      const Factors f = factors_of<LANES, V>(h, p.k, p.eps, side, turn);
+      if(V == 1) fetch(row + step);
+      auto add_through = [&](int v, int64_t r, float (&o)[8]) {
+         if(V > 1) {                                           // read only now: no registers to hold it
+            Eight<S> t{};
+            if(p.dtotal) t = fetch8_whole<S>(static_cast<const S*>(p.dtotal) + r * p.ldt, (int64_t)(v * LANES + lane) * 8, p.k);
+#pragma unroll
+            for(int i = 0; i < 8; i++) through[i] = (float)t.e[i];
+         }
+#pragma unroll
+         for(int i = 0; i < 8; i++) o[i] += through[i];
+      };
+      const Factors f = factors_of<LANES, PER, V>(h, p.k, p.eps, side, turn);
       float mean = 0.0f;
 #pragma unroll
       for(int v = 0; v < V; v++) {
          const int64_t col = (int64_t)(v * LANES + lane) * 8;
          Eight<float> w;
-         if(p.weight) w = fetch8<float>(p.weight, col, p.k);
+         if(p.weight) w = V > 1 ? fetch8_whole<float>(p.weight, col, p.k) : fetch8<float>(p.weight, col, p.k);
 #pragma unroll
          for(int i = 0; i < 8; i++) {
             h[v][i] = h[v][i] * f.c * f.r;
-            dw[v][i] += g[v][i] * h[v][i];
+            dw[v][i] = __builtin_fmaf(g[v][i], there ? h[v][i] : 0.0f, dw[v][i]);
             if(p.weight) g[v][i] *= w.e[i];
-            mean += g[v][i] * h[v][i];
+            mean = __builtin_fmaf(g[v][i], h[v][i], mean);
          }
       }
       mean = row_sum<LANES>(mean, side, turn) / (float)p.k;
+      if(!there) continue;
       O* const dx = static_cast<O*>(p.dx) + row * p.ldx;
 #pragma unroll
       for(int v = 0; v < V; v++) {
          float o[8];
 #pragma unroll
-         for(int i = 0; i < 8; i++) o[i] = (g[v][i] - h[v][i] * mean) * f.r * f.c + through[v][i];
-         put8<O>(dx, (int64_t)(v * LANES + lane) * 8, p.k, o);
+         for(int i = 0; i < 8; i++) o[i] = __builtin_fmaf(-h[v][i], mean, g[v][i]) * f.r * f.c;
+         add_through(v, row, o);
+         const int64_t col = (int64_t)(v * LANES + lane) * 8;
+         if(V == 1) put8<O>(dx, col, p.k, o);
+         else if(col < p.k) store8<O>(dx + col, o);
       }
    }
    if(!p.dweight) return;
    float* const work = p.work + (int64_t)blockIdx.x * p.k;
    if constexpr(PER > 1) {
-      // the wavefronts' sums, in their order
+      // the rows' sums, in their order
       __shared__ float join[PER][V * LANES * 8];
 #pragma unroll
       for(int v = 0; v < V; v++)
 #pragma unroll
-         for(int i = 0; i < 8; i++) join[threadIdx.x / LANES][(v * 8 + i) * LANES + lane] = dw[v][i];
+         for(int i = 0; i < 8; i++) join[mine][(v * 8 + i) * LANES + lane] = dw[v][i];
       __syncthreads();
-      for(int i = threadIdx.x; i < V * 8 * LANES; i += 256) {
+      for(int i = threadIdx.x; i < V * 8 * LANES; i += kGradBlock) {
          const int64_t col = (int64_t)(i / (8 * LANES) * LANES + i % LANES) * 8 + i / LANES % 8;
          float s = 0.0f;
 #pragma unroll
@@ -429,7 +517,11 @@ norm_grad_rows(NormGradParams p, int64_t groups)
       }
    } else {
 #pragma unroll
-      for(int v = 0; v < V; v++) put8<float>(work, (int64_t)(v * LANES + lane) * 8, p.k, dw[v]);
+      for(int v = 0; v < V; v++) {
+         const int64_t col = (int64_t)(v * LANES + lane) * 8;
+         if(V == 1) put8<float>(work, col, p.k, dw[v]);
+         else if(col < p.k) store8<float>(work + col, dw[v]);
+      }
    }
 }
 
@@ -445,7 +537,7 @@ norm_grad_long(NormGradParams p, int64_t groups)
    for(int64_t row = blockIdx.x; row < p.rows; row += groups) {
       const D* const dy = static_cast<const D*>(p.dy) + row * p.ldy;
       const S* const hh = static_cast<const S*>(p.h) + row * p.ldh;
-      const Factors f = factors_from<1024>([&](float c) {
+      const Factors f = factors_from<1024, 1>([&](float c) {
          float ss = 0.0f;
          for(int64_t col = threadIdx.x * 8; col < p.k; col += 8192) {
             const Eight<S> a = fetch8<S>(hh, col, p.k);
@@ -491,7 +583,7 @@ norm_grad_long(NormGradParams p, int64_t groups)
             put8<float>(work, col, p.k, sum);
          }
 #pragma unroll
-         for(int i = 0; i < 8; i++) g[i] = (g[i] - h[i] * mean) * f.r * f.c + (dt ? (float)t.e[i] : 0.0f);
+         for(int i = 0; i < 8; i++) g[i] = __builtin_fmaf(-h[i], mean, g[i]) * f.r * f.c + (dt ? (float)t.e[i] : 0.0f);
          put8<O>(static_cast<O*>(p.dx) + row * p.ldx, col, p.k, g);
       }
    }
@@ -534,6 +626,9 @@ hipError_t norm_shape(const NormParams& p, hipStream_t s)
 template<class X, class S, bool NORM>
 hipError_t norm_typed(const NormParams& p, hipStream_t s)
 {
+   if constexpr(NORM)                                        // 16 lanes write the padding of a row of codes too
+      if(p.k <= 32 && !p.codes) return norm_shape<X, S, 4, 1, NORM>(p, s);
+   if(p.k <= 128)   return norm_shape<X, S, 16, 1, NORM>(p, s);
    if(p.k <= 512)   return norm_shape<X, S, 64, 1, NORM>(p, s);
    if(p.k <= 1024)  return norm_shape<X, S, 64, 2, NORM>(p, s);
    if(p.k <= 2048)  return norm_shape<X, S, 256, 1, NORM>(p, s);
@@ -568,7 +663,7 @@ hipError_t dequantize_typed(const int8_t* codes, const float* scales, void* out,
 template<class D, class S, class O, int LANES, int V>
 hipError_t grad_shape(const NormGradParams& p, hipStream_t s)
 {
-   constexpr int PER = LANES == 64 ? 4 : 1, BLOCK = LANES == 64 ? 256 : LANES;
+   constexpr int PER = LANES == 0 || LANES >= kGradBlock ? 1 : kGradBlock / (LANES ? LANES : 1), BLOCK = LANES < kGradBlock ? kGradBlock : LANES;
    int64_t groups = (p.rows + PER - 1) / PER;
    if(p.dweight) groups = groups < p.splits ? groups : p.splits;
    if(groups > 2048) groups = 2048;
@@ -587,11 +682,14 @@ hipError_t grad_shape(const NormGradParams& p, hipStream_t s)
 template<class D, class S, class O>
 hipError_t grad_typed(const NormGradParams& p, hipStream_t s)
 {
+   if(p.k <= 32)    return grad_shape<D, S, O, 4, 1>(p, s);
+   if(p.k <= 128)   return grad_shape<D, S, O, 16, 1>(p, s);
    if(p.k <= 512)   return grad_shape<D, S, O, 64, 1>(p, s);
-   if(p.k <= 1024)  return grad_shape<D, S, O, 64, 2>(p, s);
+   if(p.k <= 1024)  return grad_shape<D, S, O, 128, 1>(p, s);
    if(p.k <= 2048)  return grad_shape<D, S, O, 256, 1>(p, s);
-   if(p.k <= 4096)  return grad_shape<D, S, O, 256, 2>(p, s);
-   if(p.k <= 8192)  return grad_shape<D, S, O, 512, 2>(p, s);
+   if(p.k <= 4096)  return grad_shape<D, S, O, 512, 1>(p, s);
+   if(p.k <= 8192)  return grad_shape<D, S, O, 1024, 1>(p, s);
+   if(p.k <= 16384 && p.k % 8 == 0) return grad_shape<D, S, O, 1024, 2>(p, s);
    return grad_shape<D, S, O, 0, 0>(p, s);
 }
 
