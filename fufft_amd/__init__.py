@@ -1052,6 +1052,11 @@ def _eight(codes, scales, name: str, rows: int, k: int):
 def i8_quantize(x, codes, scales, stream=None) -> None:
     """x (rows, k) as 8-bit rows: each row's scale is its largest magnitude over 127, its bytes
     the nearest multiples."""
+    if _native(x):
+        gpu = _current_device()
+        status = _binding.i8_quantize(x, codes, scales, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_i8_quantize")
     kind, ld, rows, k = _matrix(x, "x")
     pc, ps = _eight(codes, scales, "codes", rows, k)
     _on_gpu((x, "x"), (codes, "codes"), (scales, "scales"))
@@ -1060,6 +1065,11 @@ def i8_quantize(x, codes, scales, stream=None) -> None:
 
 def i8_dequantize(codes, scales, out, stream=None) -> None:
     """The values that 8-bit rows stand for, into out (rows, k)."""
+    if _native(out):
+        gpu = _current_device()
+        status = _binding.i8_dequantize(codes, scales, out, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_i8_dequantize")
     kind, ld, rows, k = _matrix(out, "out")
     pc, ps = _eight(codes, scales, "codes", rows, k)
     _on_gpu((out, "out"), (codes, "codes"), (scales, "scales"))
@@ -1069,6 +1079,11 @@ def i8_dequantize(codes, scales, out, stream=None) -> None:
 def i8_matmul(a, a_scales, b, b_scales, out, k: int, bias=None, stream=None) -> None:
     """out (m, n) = a b^T + bias: a is m 8-bit rows of k values (tokens), b n (channels), bias
     fp32.  The integer sum is exact; k goes up to 131071."""
+    if _native(out):
+        gpu = _current_device()
+        status = _binding.i8_matmul(a, a_scales, b, b_scales, out, k, bias, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_i8_matmul")
     kind, ld, m, n = _matrix(out, "out")
     k = operator.index(k)
     pa, pas = _eight(a, a_scales, "a", m, k)
@@ -1096,6 +1111,11 @@ def rms_norm(x, weight=None, out=None, *, codes=None, scales=None, residual=None
     """y = h weight / sqrt(mean(h^2) + eps) along rows, h = x + residual: into out (x's type),
     as 8-bit rows into codes and scales, or both.  total takes h, in residual's type (x's or
     fp32), and may be residual itself, or x; out may be x.  weight: fp32, None: ones."""
+    if _native(x):
+        gpu = _current_device()
+        status = _binding.rms_norm(x, weight, out, codes, scales, residual, total, eps, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_rms_norm")
     kind, ldx, rows, k = _matrix(x, "x")
     pr, ldr, rk = _like(residual, "residual", rows, k, (kind, 0))
     pt, ldt, tk = _like(total, "total", rows, k, (kind, 0) if rk is None else (rk,))
@@ -1118,6 +1138,11 @@ def rms_norm_grad(dy, h, weight, dx, dweight=None, work=None, *, dtotal=None, ep
     reaches h along the residual, added; dweight (fp32).  h is rms_norm's total, or x where there was
     no residual.  dx is of dy's type or h's, and may be dy or dtotal.  work: fp32 (splits, k), needed
     for dweight; 512 splits are as many as help."""
+    if _native(dy):
+        gpu = _current_device()
+        status = _binding.rms_norm_grad(dy, h, weight, dx, dweight, work, dtotal, eps, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_rms_norm_grad")
     kind, ldy, rows, k = _matrix(dy, "dy")
     ph, ldh, hk = _like(h, "h", rows, k, (kind, 0))
     if ph is None:
@@ -1189,6 +1214,11 @@ def decay_attention(q, k, v, log_decay, out, *, state=None, new_state=None, lens
     lens (int32, batch): tokens of each sequence; rows behind them are neither read nor written.
     work: fp32, room for splits * batch * heads * dk * dv values; the tokens are split over at most that
     many workgroups, and about 1024 / (batch * heads) splits are as many as help."""
+    if _native(q):
+        gpu = _current_device()
+        status = _binding.decay_attention(q, k, v, log_decay, out, state, new_state, lens, work, scale, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_decay_attention")
     pq, sq = _heads(q, "q", (None,) * 4)
     kind = _ELEMENT[q.dtype]
     batch, tokens, heads, dk = q.shape
@@ -1211,6 +1241,11 @@ def decay_attention_grad(dout, q, k, v, log_decay, dq, dk, dv, *, state=None, dn
     """Gradients of decay_attention: dq, dk, dv of dout and of dnew_state (None: zero), and dstate
     (None: not wanted).  state and lens are that call's; log_decay is a constant.  work: as there,
     with room for three such sets of states."""
+    if _native(q):
+        gpu = _current_device()
+        status = _binding.decay_attention_grad(dout, q, k, v, log_decay, dq, dk, dv, state, dnew_state, dstate, lens, work, scale, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_decay_attention_grad")
     pq, sq = _heads(q, "q", (None,) * 4)
     kind = _ELEMENT[q.dtype]
     batch, tokens, heads, nk = q.shape
@@ -1238,6 +1273,11 @@ def decay_attention_step(q, k, v, log_decay, state, out, *, slots=None, scale: f
     heads, dk, dv) is updated in place.  slots (int64, batch): the state of each sequence, None: its own
     number.  A slot outside, such as -1, or one that an earlier sequence of the call has, changes nothing
     and gives zeros."""
+    if _native(q):
+        gpu = _current_device()
+        status = _binding.decay_attention_step(q, k, v, log_decay, state, out, slots, scale, _handle(stream, gpu), gpu)
+        if status is not None:
+            return check(status, "fufft_decay_attention_step")
     pq, sq = _heads(q, "q", (None,) * 3)
     kind = _ELEMENT[q.dtype]
     batch, heads, dk = q.shape

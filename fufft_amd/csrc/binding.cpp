@@ -1,4 +1,4 @@
-// The short way from Python to the 4-bit calls: reads the tensors' properties, checks them
+// The short way from Python to the 4-bit, 8-bit, norm and decaying-attention calls: reads the tensors' properties, checks them
 // and calls the C ABI, all in native code.  These calls are short (a few rows take
 // the GPU 2 to 4 us), so what the host spends on a call is what a small one costs: 48 rows
 // of 4096 made 4-bit, host time a call, 5.5 us through ctypes, 3.6 so, 3.2 of them the launch.
@@ -284,11 +284,258 @@ PyObject* cache_conv(PyObject*, PyObject* const* a, Py_ssize_t n)
    });
 }
 
+// ---- 8-bit rows and norms -----------------------------------------------------------------
+
+struct Eight {
+   void*  codes;
+   float* scales;
+};
+// `rows` 8-bit rows of k values
+Eight eight(PyObject* codes, PyObject* scales, int64_t rows, int64_t k, int64_t gpu)
+{
+   const int64_t width = (k + 127) / 128 * 128;
+   void* const p = array(codes, at::kChar, rows * width, gpu);
+   const at::Tensor& t = THPVariable_Unpack(codes);
+   if(t.dim() > 1 && rows * width > 0 && t.size(t.dim() - 1) != width) throw Refused();
+   return {p, static_cast<float*>(array(scales, at::kFloat, 4 * rows, gpu))};
+}
+float* floats_of(PyObject* o, int64_t n, int64_t gpu)
+{
+   return o == Py_None ? nullptr : static_cast<float*>(array(o, at::kFloat, 4 * n, gpu));
+}
+double number(PyObject* o)
+{
+   const double v = PyFloat_AsDouble(o);
+   if(v == -1.0 && PyErr_Occurred()) throw Refused();
+   return v;
+}
+// a matrix of rows x k, or nothing where None is given
+Matrix like(PyObject* o, int64_t rows, int64_t k, int64_t gpu)
+{
+   if(o == Py_None) return Matrix{nullptr, -1, 0, rows, k};
+   const Matrix m = matrix(o, gpu);
+   if(m.rows != rows || m.k != k) throw Refused();
+   return m;
+}
+
+PyObject* i8_quantize(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+   return guarded(n, 5, [&] {
+      const int64_t gpu = integer(a[4]);
+      void* const stream = handle(a[3]);
+      const Matrix x = matrix(a[0], gpu);
+      const Eight q = eight(a[1], a[2], x.rows, x.k, gpu);
+      return status_of([&] { return fufft_i8_quantize(x.p, x.type, x.ld, x.rows, x.k, q.codes, q.scales, stream); });
+   });
+}
+
+PyObject* i8_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+   return guarded(n, 5, [&] {
+      const int64_t gpu = integer(a[4]);
+      void* const stream = handle(a[3]);
+      const Matrix out = matrix(a[2], gpu);
+      const Eight q = eight(a[0], a[1], out.rows, out.k, gpu);
+      return status_of([&] { return fufft_i8_dequantize(q.codes, q.scales, out.p, out.type, out.ld, out.rows, out.k, stream); });
+   });
+}
+
+PyObject* i8_matmul(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+   return guarded(n, 9, [&] {
+      const int64_t gpu = integer(a[8]), k = integer(a[5]);
+      void* const stream = handle(a[7]);
+      const Matrix out = matrix(a[4], gpu);
+      if(k < 0 || k > ((int64_t)1 << 40)) throw Refused();
+      const Eight x = eight(a[0], a[1], out.rows, k, gpu), w = eight(a[2], a[3], out.k, k, gpu);
+      const float* const bias = bias_of(a[6], out.k, gpu);
+      return status_of([&] {
+         return fufft_i8_matmul(x.codes, x.scales, w.codes, w.scales, bias, out.p, out.type, out.ld, out.rows, out.k, k, stream);
+      });
+   });
+}
+
+PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+   return guarded(n, 10, [&] {
+      const int64_t gpu = integer(a[9]);
+      void* const stream = handle(a[8]);
+      const float eps = (float)number(a[7]);
+      const Matrix x = matrix(a[0], gpu);
+      const Matrix out = like(a[2], x.rows, x.k, gpu), r = like(a[5], x.rows, x.k, gpu), t = like(a[6], x.rows, x.k, gpu);
+      const int sum = r.p || a[5] != Py_None ? r.type : a[6] != Py_None ? t.type : x.type;
+      if((a[2] != Py_None && out.type != x.type) || (sum != x.type && sum != FUFFT_F32) || (a[6] != Py_None && t.type != sum))
+         throw Refused();
+      const bool codes = a[3] != Py_None || a[4] != Py_None;
+      if(!codes && a[2] == Py_None) throw Refused();
+      const Eight q = codes ? eight(a[3], a[4], x.rows, x.k, gpu) : Eight{nullptr, nullptr};
+      const float* const w = floats_of(a[1], x.k, gpu);
+      return status_of([&] {
+         return fufft_rms_norm(x.p, x.type, x.ld, r.p, r.ld, t.p, t.ld, sum, w, eps, out.p, out.ld, q.codes, q.scales, x.rows,
+                               x.k, stream);
+      });
+   });
+}
+
+PyObject* rms_norm_grad(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+   return guarded(n, 10, [&] {
+      const int64_t gpu = integer(a[9]);
+      void* const stream = handle(a[8]);
+      const float eps = (float)number(a[7]);
+      const Matrix dy = matrix(a[0], gpu);
+      if(a[1] == Py_None || a[3] == Py_None) throw Refused();
+      const Matrix h = like(a[1], dy.rows, dy.k, gpu), dx = like(a[3], dy.rows, dy.k, gpu), t = like(a[6], dy.rows, dy.k, gpu);
+      if((h.type != dy.type && h.type != FUFFT_F32) || (dx.type != dy.type && dx.type != h.type) ||
+         (a[6] != Py_None && t.type != h.type))
+         throw Refused();
+      const float* const w = floats_of(a[2], dy.k, gpu);
+      float* const dw = floats_of(a[4], dy.k, gpu);
+      int64_t splits = 0;
+      float* work = nullptr;
+      if(dw && a[5] != Py_None && dy.k > 0) {
+         splits = tensor(a[5], gpu).numel() / dy.k;
+         if(splits > 0) work = static_cast<float*>(array(a[5], at::kFloat, 4 * splits * dy.k, gpu));
+      }
+      if(a[4] != Py_None && splits == 0 && dy.k > 0) throw Refused();
+      return status_of([&] {
+         return fufft_rms_norm_grad(dy.p, dy.type, dy.ld, h.p, h.ld, t.p, t.ld, h.type, w, eps, dx.p, dx.type, dx.ld, dw, work,
+                                    splits, dy.rows, dy.k, stream);
+      });
+   });
+}
+
+// ---- decaying attention ----------------------------------------------------------------------
+
+// a tensor of (batch, tokens, heads, dim), or (batch, heads, dim) for one token
+struct Heads {
+   void*         p;
+   int           type;
+   fufft_strides s;
+   int64_t       batch, tokens, heads, dim;
+};
+Heads heads_of(PyObject* o, int dims, int64_t gpu)
+{
+   const at::Tensor& t = tensor(o, gpu);
+   if(t.dim() != dims) throw Refused();
+   const bool many = dims == 4;
+   Heads h{nullptr, element(t), {t.stride(0), many ? t.stride(1) : 0, t.stride(dims - 2)},
+           t.size(0), many ? t.size(1) : 1, t.size(dims - 2), t.size(dims - 1)};
+   if(h.dim > 1 && t.stride(dims - 1) != 1) throw Refused();
+   h.p = t.data_ptr();
+   return h;
+}
+void alike(const Heads& a, const Heads& b, bool dim)
+{
+   if(a.type != b.type || a.batch != b.batch || a.tokens != b.tokens || a.heads != b.heads || (dim && a.dim != b.dim))
+      throw Refused();
+}
+float* states_of(PyObject* o, const Heads& q, int64_t dv, int64_t gpu)
+{
+   if(o == Py_None) return nullptr;
+   float* const p = static_cast<float*>(array(o, at::kFloat, 4 * q.batch * q.heads * q.dim * dv, gpu));
+   const at::Tensor& t = THPVariable_Unpack(o);
+   if(t.dim() > 1 && (t.dim() != 4 || t.size(0) != q.batch || t.size(1) != q.heads || t.size(2) != q.dim || t.size(3) != dv))
+      throw Refused();
+   return p;
+}
+struct Work {
+   float*  p;
+   int64_t splits;
+};
+Work work_of(PyObject* o, int64_t each, int64_t gpu)
+{
+   if(o == Py_None || each == 0) return {nullptr, 0};
+   const int64_t n = tensor(o, gpu).numel() / each;
+   return {n == 0 ? nullptr : static_cast<float*>(array(o, at::kFloat, 4 * n * each, gpu)), n};
+}
+const int32_t* lens_of(PyObject* o, int64_t batch, int64_t gpu)
+{
+   return o == Py_None ? nullptr : static_cast<const int32_t*>(array(o, at::kInt, 4 * batch, gpu));
+}
+
+PyObject* decay_attention(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+   return guarded(n, 12, [&] {
+      const int64_t gpu = integer(a[11]);
+      void* const stream = handle(a[10]);
+      const float scale = (float)number(a[9]);
+      const Heads q = heads_of(a[0], 4, gpu), k = heads_of(a[1], 4, gpu), v = heads_of(a[2], 4, gpu), out = heads_of(a[4], 4, gpu);
+      alike(q, k, true);
+      alike(q, v, false);
+      alike(v, out, true);
+      const float* const g = static_cast<const float*>(array(a[3], at::kFloat, 4 * q.heads, gpu));
+      const float* const state = states_of(a[5], q, v.dim, gpu);
+      float* const next = states_of(a[6], q, v.dim, gpu);
+      const int32_t* const lens = lens_of(a[7], q.batch, gpu);
+      const Work w = work_of(a[8], q.batch * q.heads * q.dim * v.dim, gpu);
+      return status_of([&] {
+         return fufft_decay_attention(q.p, &q.s, k.p, &k.s, v.p, &v.s, q.type, g, out.p, &out.s, state, next, lens, scale, q.batch,
+                                      q.tokens, q.heads, q.dim, v.dim, w.p, w.splits, stream);
+      });
+   });
+}
+
+PyObject* decay_attention_grad(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+   return guarded(n, 16, [&] {
+      const int64_t gpu = integer(a[15]);
+      void* const stream = handle(a[14]);
+      const float scale = (float)number(a[13]);
+      const Heads o = heads_of(a[0], 4, gpu), q = heads_of(a[1], 4, gpu), k = heads_of(a[2], 4, gpu), v = heads_of(a[3], 4, gpu);
+      const Heads dq = heads_of(a[5], 4, gpu), dk = heads_of(a[6], 4, gpu), dv = heads_of(a[7], 4, gpu);
+      alike(q, k, true);
+      alike(q, v, false);
+      alike(v, o, true);
+      alike(q, dq, true);
+      alike(q, dk, true);
+      alike(v, dv, true);
+      const float* const g = static_cast<const float*>(array(a[4], at::kFloat, 4 * q.heads, gpu));
+      const float *const state = states_of(a[8], q, v.dim, gpu), *const dnew = states_of(a[9], q, v.dim, gpu);
+      float* const dstate = states_of(a[10], q, v.dim, gpu);
+      const int32_t* const lens = lens_of(a[11], q.batch, gpu);
+      const Work w = work_of(a[12], 3 * q.batch * q.heads * q.dim * v.dim, gpu);
+      return status_of([&] {
+         return fufft_decay_attention_grad(o.p, &o.s, q.p, &q.s, k.p, &k.s, v.p, &v.s, q.type, g, dq.p, &dq.s, dk.p, &dk.s, dv.p,
+                                           &dv.s, state, dnew, dstate, lens, scale, q.batch, q.tokens, q.heads, q.dim, v.dim, w.p,
+                                           w.splits, stream);
+      });
+   });
+}
+
+PyObject* decay_attention_step(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+   return guarded(n, 10, [&] {
+      const int64_t gpu = integer(a[9]);
+      void* const stream = handle(a[8]);
+      const float scale = (float)number(a[7]);
+      const Heads q = heads_of(a[0], 3, gpu), k = heads_of(a[1], 3, gpu), v = heads_of(a[2], 3, gpu), out = heads_of(a[5], 3, gpu);
+      alike(q, k, true);
+      alike(q, v, false);
+      alike(v, out, true);
+      const float* const g = static_cast<const float*>(array(a[3], at::kFloat, 4 * q.heads, gpu));
+      const at::Tensor& s = tensor(a[4], gpu);
+      if(s.dim() != 4 || s.size(1) != q.heads || s.size(2) != q.dim || s.size(3) != v.dim) throw Refused();
+      const int64_t count = s.size(0);
+      if(a[6] == Py_None && count < q.batch) throw Refused();
+      float* const state = static_cast<float*>(array(a[4], at::kFloat, 4 * count * q.heads * q.dim * v.dim, gpu));
+      const int64_t* const slots = a[6] == Py_None ? nullptr : static_cast<const int64_t*>(array(a[6], at::kLong, 8 * q.batch, gpu));
+      return status_of([&] {
+         return fufft_decay_attention_step(q.p, &q.s, k.p, &k.s, v.p, &v.s, q.type, g, out.p, &out.s, state, count, slots, scale,
+                                           q.batch, q.heads, q.dim, v.dim, stream);
+      });
+   });
+}
+
 #define FUFFT_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FUFFT_METHOD(quantize),    FUFFT_METHOD(dequantize), FUFFT_METHOD(matmul),
                          FUFFT_METHOD(linear),      FUFFT_METHOD(cache_write), FUFFT_METHOD(cache_read),
-                         FUFFT_METHOD(cache_conv), {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", "The 4-bit calls, checked and made in native code.", -1, methods,
+                         FUFFT_METHOD(cache_conv),
+                         FUFFT_METHOD(i8_quantize), FUFFT_METHOD(i8_dequantize), FUFFT_METHOD(i8_matmul),
+                         FUFFT_METHOD(rms_norm),    FUFFT_METHOD(rms_norm_grad), FUFFT_METHOD(decay_attention),
+                         FUFFT_METHOD(decay_attention_grad), FUFFT_METHOD(decay_attention_step),
+                         {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", "The 4-bit, 8-bit, norm and decaying-attention calls, checked and made in native code.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -55,13 +55,14 @@ bool distinct(const Array& a)
       if(a.axis[i].stride < extent(a, i + 1)) return false;
    return true;
 }
-// Whether the parts below axis i of two arrays of the same axes share nothing, the second one's `by`
-// elements behind the first one's.
+// Whether the parts below axis i of two arrays share nothing, the second one's `by` elements behind the first
+// one's: far from each other, or, along an axis that both step through alike, each in the gaps of the other (parts
+// of one row a token, whose heads may have other widths).
 bool parts_apart(const Array& a, const Array& b, int i, int64_t by)
 {
    const int64_t wa = extent(a, i), wb = extent(b, i);
    if(by >= wa || by + wb <= 0) return true;
-   if(i == a.axes) return false;
+   if(i >= a.axes || i >= b.axes || a.axis[i].stride != b.axis[i].stride) return false;
    const int64_t s = a.axis[i].stride;
    if(s == 0) return false;
    const int64_t r = (by % s + s) % s;                 // the second's first part in a step of the first
@@ -71,11 +72,8 @@ bool parts_apart(const Array& a, const Array& b, int i, int64_t by)
 bool arrays_apart(const Array& a, const Array& b)
 {
    if(disjoint(span_of(a), span_of(b))) return true;
-   if(a.axes != b.axes || a.element != b.element || !distinct(a)) return false;
-   for(int i = 0; i < a.axes; i++)
-      if(a.axis[i].stride != b.axis[i].stride || a.axis[i].count != b.axis[i].count) return false;
    const int64_t bytes = static_cast<const char*>(b.p) - static_cast<const char*>(a.p);
-   return bytes % a.element == 0 && parts_apart(a, b, 0, bytes / a.element);
+   return a.element == b.element && bytes % a.element == 0 && parts_apart(a, b, 0, bytes / a.element);
 }
 
 Strides strides_of(const fufft_strides* s) { return s ? Strides{s->batch, s->token, s->head} : Strides{}; }

@@ -74,7 +74,40 @@ def test_gradient_refusals():
     assert call(dq=P[5], dk_=P[5] + 4 * HEADS * 130, dv_=P[5] + 8 * HEADS * 130, **kw) == UNSUP
     assert call(dq=P[5], dk_=P[5] + 8 * HEADS * 130, dv_=P[5] + 4 * HEADS * 130, **kw) == UNSUP
     assert call(dq=P[5], dk_=P[5] + 4 * HEADS * 130, dv_=P[5] + 8 * HEADS * 130 + 4, **kw) == INV      # wraps into the next token's dq
+    # heads of two widths side by side, and one element into each other
+    row = HEADS * (2 * 130 + 30)
+    kw = dict(dk=130, dv=30, sdo=strides(30), sk=s, sv=strides(30), sq2=(TOKENS * row, row, 130), sk2=(TOKENS * row, row, 130),
+              sv2=(TOKENS * row, row, 30))
+    assert call(dq=P[5], dk_=P[5] + 4 * HEADS * 130, dv_=P[5] + 8 * HEADS * 130, **kw) == UNSUP
+    assert call(dq=P[5], dk_=P[5] + 4 * HEADS * 130, dv_=P[5] + 8 * HEADS * 130 - 4, **kw) == INV
+    assert call(dq=P[5], dk_=P[5] + 4 * HEADS * 130, dv_=P[5] + 8 * HEADS * 130 + 4, **kw) == INV
+    # a step that is no whole part of the other's row
+    assert call(dq=P[5], dk_=P[5] + 4 * HEADS * 130, dv_=P[5] + 8 * HEADS * 130, **{**kw, "sv2": (TOKENS * row, row - 1, 30)}) == INV
     assert call(batch=0) == OK
+
+
+def test_apart_by_brute_force():
+    """What a call takes of an input and an output in one array, against the sets of their elements.  (Heads of 129
+    and more, which are refused last of all, so that nothing is launched.)"""
+    rng = np.random.default_rng(7)
+    taken = apart = 0
+    for _ in range(1500):
+        heads, tokens = int(rng.integers(1, 4)), int(rng.integers(1, 4))
+        dk, dv = int(rng.integers(129, 132)), int(rng.integers(129, 132))
+        sk = (0, int(rng.integers(0, 900)), dk + int(rng.integers(0, 150)))
+        sv = (0, sk[1] if rng.random() < 0.8 else int(rng.integers(0, 900)), sk[2] if rng.random() < 0.5 else dv + int(rng.integers(0, 150)))
+        at = int(rng.integers(0, 900))
+
+        def places(s, d, off):
+            return [off + t * s[1] + h * s[2] + i for t in range(tokens) for h in range(heads) for i in range(d)]
+        q, o = places(sk, dk, 0), places(sv, dv, at)
+        status = forward(sq=sk, sk=strides(dk, tokens, heads), sv=strides(dv, tokens, heads), so=sv, out=P[0] + 4 * at, batch=1, tokens=tokens,
+                         heads=heads, dk=dk, dv=dv, splits=0, work=None)
+        assert status in (INV, UNSUP)
+        fine = len(set(o)) == len(o) and not set(q) & set(o)
+        assert fine or status == INV, (heads, tokens, dk, dv, sk, sv, at)
+        taken, apart = taken + (status == UNSUP), apart + fine
+    assert apart > 200 and taken > 0.7 * apart, (taken, apart)
 
 
 def test_step_refusals():
