@@ -485,21 +485,26 @@ decay_chunks(DecayParams p)
             fetch_some(4 + sb * 4 / NS, 4 + (sb + 1) * 4 / NS);
             if(sb * EACH > strip) continue;
             f32x4 s[EACH];
+            Frag kf[EACH][NK], vf[SB];
+#pragma unroll
+            for(int e = 0; e < EACH; e++)
+#pragma unroll
+               for(int i = 0; i < NK; i++) kf[e][i] = frag(M::KEYS, (sb * EACH + e) * 16, i);
+#pragma unroll
+            for(int c = 0; c < SB; c++) vf[c] = token_frag(M::VALUES, v0 + c * 16, sb);
+#pragma unroll
+            for(int e = 0; e < EACH; e++) s[e] = f32x4{};
+#pragma unroll
+            for(int i = 0; i < NK; i++)
+#pragma unroll
+               for(int e = 0; e < EACH; e++) s[e] = C::mma(kf[e][i], qf[i], s[e]);
 #pragma unroll
             for(int e = 0; e < EACH; e++) {
                const int tile = sb * EACH + e;
-               f32x4 x = {};
-               if(tile <= strip) {
-                  Frag kf[NK];
 #pragma unroll
-                  for(int i = 0; i < NK; i++) kf[i] = frag(M::KEYS, tile * 16, i);
-#pragma unroll
-                  for(int i = 0; i < NK; i++) x = C::mma(kf[i], qf[i], x);
-               }
-#pragma unroll
-               for(int r = 0; r < 4; r++) s[e][r] = x[r] * wt[tile][r];
+               for(int r = 0; r < 4; r++) s[e][r] *= wt[tile][r];
                // tokens behind t have no part in it, whatever they hold
-               if(tile == strip)
+               if(tile >= strip)
 #pragma unroll
                   for(int r = 0; r < 4; r++) s[e][r] = tile * 16 + r <= reach ? s[e][r] : 0.0f;
             }
@@ -509,11 +514,8 @@ decay_chunks(DecayParams p)
 #pragma unroll
                for(int r = 0; r < 4; r++) w[e * 4 + r] = (E)s[e][r];
             if(!special) {
-               Frag x[SB];
 #pragma unroll
-               for(int c = 0; c < SB; c++) x[c] = token_frag(M::VALUES, v0 + c * 16, sb);
-#pragma unroll
-               for(int c = 0; c < SB; c++) o[c] = C::mma(x[c], w, o[c]);
+               for(int c = 0; c < SB; c++) o[c] = C::mma(vf[c], w, o[c]);
             } else {
                // A value that is infinite or NaN times a weight of zero would reach tokens before it.  Such values
                // are left out of the products, and added one by one to the results that they belong to.
