@@ -34,31 +34,67 @@ using mx4::f32x4;
 
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kChunk = 64, kLanes = 512;
 
-// What the matrix cores take for an input type: bf16 as it is, fp16 and fp32 in fp32.  Every operand
-// is 16 bytes a lane: row lane % 16, of each block of the summed index (32 or 16 values)
-// the lane / 16-th piece of 8 or 4.  A result of 16 x 16: column lane % 16, rows 4 (lane / 16) ..
-// + 3.  So a result is, piece by piece, an operand again whose block of 32 takes rows 4 g .. 4 g + 3 of
-// two results (with g = lane / 16), or whose block of 16 takes those of one.
+// What the matrix cores take for an input type.  Every operand is 16 bytes a lane: row lane % 16, of each block
+// of the summed index (32 or 16 values) the lane / 16-th piece of 8 or 4.  A result of 16 x 16: column lane %
+// 16, rows 4 (lane / 16) .. + 3.  So a result is, piece by piece, an operand again whose block of 32 takes rows 4 g .. 4 g + 3
+// of two results (with g = lane / 16), or whose block of 16 takes those of one.
+//
+//   fp32: everything in fp32, whose products run at a sixteenth of the others' rate and bound these kernels.
+//   bf16: what becomes an operand again is rounded to it; weighted keys are a sum of two bf16 parts, 16 bits, as the
+//     state may be returned (with one part, 7 % less time for the gradients).
+//   fp16: scores in fp16 as they are.  fp16's range would not hold what becomes an operand again, so that
+//     and what meets it are sums of two bf16 parts, 16 bits of a value and all 11 of fp16; of the four products the
+//     smallest, of both second parts, is left out (2^-16).
 template<class T> struct Cores {
    typedef float E;
-   typedef f32x4 Frag;
-   static constexpr int PARTS = 1;
+   typedef f32x4 Frag, Plain;            // operands in E; of q and k as they are
+   static constexpr int KEY_PARTS = 1;   // of weighted keys
+   static constexpr int PARTS = 1;       // of values, weights, the state, and q where it meets that
    static __device__ inline f32x4 mma(Frag a, Frag b, f32x4 c)
    {
 #pragma unroll
       for(int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
       return c;
    }
+   static __device__ inline f32x4 scores(Plain a, Plain b, f32x4 c) { return mma(a, b, c); }
 };
 template<> struct Cores<bf16> {
    typedef bf16 E;
-   typedef bf16x8 Frag;
-   static constexpr int PARTS = 2;       // weighted keys are a sum of two bf16 parts, 16 bits
+   typedef bf16x8 Frag, Plain;
+   static constexpr int KEY_PARTS = 2, PARTS = 1;
    static __device__ inline f32x4 mma(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+   static __device__ inline f32x4 scores(Plain a, Plain b, f32x4 c) { return mma(a, b, c); }
 };
+template<> struct Cores<f16> {
+   typedef bf16 E;
+   typedef bf16x8 Frag;
+   typedef f16x8 Plain;
+   static constexpr int KEY_PARTS = 2, PARTS = 2;
+   static __device__ inline f32x4 mma(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+   static __device__ inline f32x4 scores(Plain a, Plain b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+// sums of parts, all products but that of both second parts
+template<class C, int A, int B>
+__device__ inline f32x4 mma_parts(const typename C::Frag (&a)[A], const typename C::Frag (&b)[B], f32x4 c)
+{
+#pragma unroll
+   for(int i = 0; i < A; i++)
+#pragma unroll
+      for(int j = 0; j < B; j++)
+         if(i + j < 2) c = C::mma(a[i], b[j], c);
+   return c;
+}
+// what bf16 leaves of values (NaN of an infinity)
+template<int N>
+__device__ inline void rest(float (&x)[N])
+{
+#pragma unroll
+   for(int i = 0; i < N; i++) x[i] -= (float)(bf16)x[i];
+}
 
 // N neighbours of a row as they are in memory, loaded at the element's alignment.
 template<class T, int N> struct Raw {
@@ -168,8 +204,8 @@ template<class T, int DK, int DV, bool LOCAL> struct Room {
    typedef Cores<T> C;
    static constexpr int E = sizeof(typename C::E);
    static constexpr int TP = kChunk * E, KP = pitch_of(DK * E);       // bytes of a row of tokens, of keys' channels
-   static constexpr int VALUES = 0, KEYS_T = VALUES + DV * TP, KEYS = KEYS_T + C::PARTS * DK * TP;
-   static constexpr int STATE = LOCAL ? KEYS : KEYS + kChunk * KP, FLAGS = LOCAL ? KEYS : STATE + DV * KP;
+   static constexpr int VALUES = 0, KEYS_T = VALUES + C::PARTS * DV * TP, KEYS = KEYS_T + C::KEY_PARTS * DK * TP;
+   static constexpr int STATE = LOCAL ? KEYS : KEYS + kChunk * KP, FLAGS = LOCAL ? KEYS : STATE + C::PARTS * DV * KP;
    static constexpr int BYTES = FLAGS + 16;
 };
 
@@ -191,6 +227,7 @@ decay_chunks(DecayParams p)
    typedef Cores<T> C;
    typedef typename C::E E;
    typedef typename C::Frag Frag;
+   typedef typename C::Plain Plain;
    typedef Room<T, DK, DV, LOCAL> M;
    constexpr int BLOCK = sizeof(E) == 2 ? 32 : 16;             // of the summed index of a product
    constexpr int EACH = BLOCK / 16;                            // results to a block
@@ -296,9 +333,9 @@ decay_chunks(DecayParams p)
    };
    auto operand_q = [&](int i) {
       if(dk < DK) qr[i].cut(anew(dk) - i * BLOCK - g * N);
-      Frag f;
+      Plain f;
       if constexpr(sizeof(E) == sizeof(T)) {
-         f = __builtin_bit_cast(Frag, qr[i]);
+         f = __builtin_bit_cast(Plain, qr[i]);
       } else {
 #pragma unroll
          for(int j = 0; j < N; j++) f[j] = (E)qr[i].value(j);
@@ -401,6 +438,10 @@ decay_chunks(DecayParams p)
 #pragma unroll
                for(int i = 0; i < 8; i++) x[i] = vr[i].value(j);
                put_tokens(M::VALUES, vc + j, slot_of<E>(vt), x);
+               if constexpr(C::PARTS == 2) {
+                  rest(x);
+                  put_tokens(M::VALUES + DV * TP, vc + j, slot_of<E>(vt), x);
+               }
             }
          }
       }
@@ -421,10 +462,8 @@ decay_chunks(DecayParams p)
 #pragma unroll
             for(int i = 0; i < 8; i++) x[i] = kr[i].value(j) * wk[i];
             put_tokens(M::KEYS_T, kc + j, slot_of<E>(kt), x);
-            if constexpr(C::PARTS == 2) {
-               // what bf16 leaves of it (of an infinity NaN: a key that is infinite makes its row of the state NaN)
-#pragma unroll
-               for(int i = 0; i < 8; i++) x[i] -= (float)(bf16)x[i];
+            if constexpr(C::KEY_PARTS == 2) {
+               rest(x);
                put_tokens(M::KEYS_T + DK * TP, kc + j, slot_of<E>(kt), x);
             }
          }
@@ -435,11 +474,15 @@ decay_chunks(DecayParams p)
          for(int a = 0; a < SA; a++)
 #pragma unroll
             for(int c = 0; c < SB; c++) {
-               const float x[4] = {S[a][c][0], S[a][c][1], S[a][c][2], S[a][c][3]};
+               float x[4] = {S[a][c][0], S[a][c][1], S[a][c][2], S[a][c][3]};
                put4<E>(to + c * 16 * KP + a * 16 * (int)sizeof(E), x);
+               if constexpr(C::PARTS == 2) {
+                  rest(x);
+                  put4<E>(to + (DV + c * 16) * KP + a * 16 * (int)sizeof(E), x);
+               }
             }
       }
-      Frag qf[NK];
+      Plain qf[NK];
       if constexpr(!LOCAL) {
 #pragma unroll
          for(int i = 0; i < NK; i++) qf[i] = operand_q(i);
@@ -447,8 +490,11 @@ decay_chunks(DecayParams p)
       __syncthreads();
       const bool special = flags[side] != 0;
       if(tid == 0) flags[side ^ 1] = 0;
-      auto frag = [&](int base, int r, int block) {             // of keys or the state
-         return *reinterpret_cast<const Frag*>(lds + base + (r + row) * KP + (block * 4 + g) * 16);
+      auto key_frag = [&](int r, int block) {
+         return *reinterpret_cast<const Plain*>(lds + M::KEYS + (r + row) * KP + (block * 4 + g) * 16);
+      };
+      auto state_frag = [&](int r, int block) {
+         return *reinterpret_cast<const Frag*>(lds + M::STATE + (r + row) * KP + (block * 4 + g) * 16);
       };
       auto token_frag = [&](int base, int r, int block) {       // of a row of tokens, r a multiple of 16
          return *reinterpret_cast<const Frag*>(lds + base + (r + row) * TP + ((block * 4 + g) ^ turn(row)) * 16);
@@ -470,11 +516,23 @@ decay_chunks(DecayParams p)
          f32x4 o[SB] = {};
 #pragma unroll
          for(int i = 0; i < NK; i++) {
-            Frag x[SB];
+            Frag x[SB][C::PARTS], qs[C::PARTS];
 #pragma unroll
-            for(int c = 0; c < SB; c++) x[c] = frag(M::STATE, v0 + c * 16, i);
+            for(int c = 0; c < SB; c++)
 #pragma unroll
-            for(int c = 0; c < SB; c++) o[c] = C::mma(x[c], qf[i], o[c]);
+               for(int part = 0; part < C::PARTS; part++) x[c][part] = state_frag(part * DV + v0 + c * 16, i);
+            if constexpr(C::PARTS == 1) {
+               qs[0] = qf[i];
+            } else {
+#pragma unroll
+               for(int j = 0; j < N; j++) {
+                  const float whole = (float)qf[i][j];
+                  qs[0][j] = (bf16)whole;
+                  qs[1][j] = (bf16)(whole - (float)(bf16)whole);
+               }
+            }
+#pragma unroll
+            for(int c = 0; c < SB; c++) o[c] = mma_parts<C>(x[c], qs, o[c]);
             fetch_some(i * 4 / NK, (i + 1) * 4 / NK);
          }
 #pragma unroll
@@ -485,19 +543,22 @@ decay_chunks(DecayParams p)
             fetch_some(4 + sb * 4 / NS, 4 + (sb + 1) * 4 / NS);
             if(sb * EACH > strip) continue;
             f32x4 s[EACH];
-            Frag kf[EACH][NK], vf[SB];
+            Plain kf[EACH][NK];
+            Frag vf[SB][C::PARTS];
 #pragma unroll
             for(int e = 0; e < EACH; e++)
 #pragma unroll
-               for(int i = 0; i < NK; i++) kf[e][i] = frag(M::KEYS, (sb * EACH + e) * 16, i);
+               for(int i = 0; i < NK; i++) kf[e][i] = key_frag((sb * EACH + e) * 16, i);
 #pragma unroll
-            for(int c = 0; c < SB; c++) vf[c] = token_frag(M::VALUES, v0 + c * 16, sb);
+            for(int c = 0; c < SB; c++)
+#pragma unroll
+               for(int part = 0; part < C::PARTS; part++) vf[c][part] = token_frag(M::VALUES, part * DV + v0 + c * 16, sb);
 #pragma unroll
             for(int e = 0; e < EACH; e++) s[e] = f32x4{};
 #pragma unroll
             for(int i = 0; i < NK; i++)
 #pragma unroll
-               for(int e = 0; e < EACH; e++) s[e] = C::mma(kf[e][i], qf[i], s[e]);
+               for(int e = 0; e < EACH; e++) s[e] = C::scores(kf[e][i], qf[i], s[e]);
 #pragma unroll
             for(int e = 0; e < EACH; e++) {
                const int tile = sb * EACH + e;
@@ -508,30 +569,35 @@ decay_chunks(DecayParams p)
 #pragma unroll
                   for(int r = 0; r < 4; r++) s[e][r] = tile * 16 + r <= reach ? s[e][r] : 0.0f;
             }
-            Frag w;
+            Frag w[C::PARTS];
 #pragma unroll
             for(int e = 0; e < EACH; e++)
 #pragma unroll
-               for(int r = 0; r < 4; r++) w[e * 4 + r] = (E)s[e][r];
+               for(int r = 0; r < 4; r++) {
+                  w[0][e * 4 + r] = (E)s[e][r];
+                  if constexpr(C::PARTS == 2) w[1][e * 4 + r] = (E)(s[e][r] - (float)(E)s[e][r]);
+               }
             if(!special) {
 #pragma unroll
-               for(int c = 0; c < SB; c++) o[c] = C::mma(vf[c], w, o[c]);
+               for(int c = 0; c < SB; c++) o[c] = mma_parts<C>(vf[c], w, o[c]);
             } else {
                // A value that is infinite or NaN times a weight of zero would reach tokens before it.  Such values
                // are left out of the products, and added one by one to the results that they belong to.
 #pragma unroll
                for(int c = 0; c < SB; c++) {
-                  Frag x = token_frag(M::VALUES, v0 + c * 16, sb);
 #pragma unroll
-                  for(int i = 0; i < EACH * 4; i++) x[i] = fabsf((float)x[i]) < __builtin_inff() ? x[i] : (E)0.0f;
-                  o[c] = C::mma(x, w, o[c]);
+                  for(int part = 0; part < C::PARTS; part++)
+#pragma unroll
+                     for(int i = 0; i < EACH * 4; i++)
+                        vf[c][part][i] = fabsf((float)vf[c][part][i]) < __builtin_inff() ? vf[c][part][i] : (E)0.0f;
+                  o[c] = mma_parts<C>(vf[c], w, o[c]);
                }
 #pragma unroll
                for(int i = 0; i < EACH * 4; i++)
 #pragma unroll 1
                   for(int from_g = 0; from_g < 4; from_g++) {
                      const int s1 = sb * BLOCK + (i / 4) * 16 + from_g * 4 + i % 4;
-                     const float weight = __shfl((float)w[i], row + from_g * 16);
+                     const float weight = __shfl(s[i / 4][i % 4], row + from_g * 16);
                      if(s1 > strip * 16 + row) continue;
 #pragma unroll
                      for(int c = 0; c < SB; c++)
@@ -574,21 +640,26 @@ decay_chunks(DecayParams p)
          for(int c = 0; c < SB; c++) S[a][c] *= an;
 #pragma unroll
       for(int sb = 0; sb < NS; sb++) {
-         Frag x[SB], w[SA][C::PARTS];
+         Frag x[SB][C::PARTS], w[SA][C::KEY_PARTS];
          if constexpr(!LOCAL)
             if(more) fetch_q(t1, sb * NK / NS, (sb + 1) * NK / NS);
 #pragma unroll
-         for(int c = 0; c < SB; c++) x[c] = token_frag(M::VALUES, v0 + c * 16, sb);
+         for(int c = 0; c < SB; c++)
+#pragma unroll
+            for(int part = 0; part < C::PARTS; part++) x[c][part] = token_frag(M::VALUES, part * DV + v0 + c * 16, sb);
 #pragma unroll
          for(int a = 0; a < SA; a++)
 #pragma unroll
-            for(int part = 0; part < C::PARTS; part++) w[a][part] = token_frag(M::KEYS_T, part * DK + k0 + a * 16, sb);
+            for(int part = 0; part < C::KEY_PARTS; part++) w[a][part] = token_frag(M::KEYS_T, part * DK + k0 + a * 16, sb);
 #pragma unroll
-         for(int part = 0; part < C::PARTS; part++)
+         for(int i = 0; i < C::KEY_PARTS; i++)
 #pragma unroll
-            for(int a = 0; a < SA; a++)
+            for(int j = 0; j < C::PARTS; j++)
+               if(i + j < 2)
 #pragma unroll
-               for(int c = 0; c < SB; c++) S[a][c] = C::mma(w[a][part], x[c], S[a][c]);
+                  for(int a = 0; a < SA; a++)
+#pragma unroll
+                     for(int c = 0; c < SB; c++) S[a][c] = C::mma(w[a][i], x[c][j], S[a][c]);
       }
       __syncthreads();
    }
@@ -788,8 +859,10 @@ hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
 template<class T, int DK, int DV>
 hipError_t chunks_launches(const DecayParams& p, int roles, hipStream_t s)
 {
-   return p.role[0].dk % 8 == 0 && p.role[0].dv % 8 == 0 ? segments_launches<T, DK, DV, true>(p, roles, s)
-                                                         : segments_launches<T, DK, DV, false>(p, roles, s);
+   const bool whole = p.role[0].dk % 8 == 0 && p.role[0].dv % 8 == 0;
+   if(whole) return segments_launches<T, DK, DV, true>(p, roles, s);
+   if constexpr(DV == 64 || Cores<T>::PARTS == 1) return segments_launches<T, DK, DV, false>(p, roles, s);
+   else return segments_launches<T, DK, 64, false>(p, roles, s);        // two parts of everything leave no registers for more
 }
 
 // roles whose keys have the same width
