@@ -44,15 +44,17 @@ constexpr int kChunk = 64, kLanes = 512;
 // of two results (with g = lane / 16), or whose block of 16 takes those of one.
 //
 //   fp32: everything in fp32, whose products run at a sixteenth of the others' rate and bound these kernels.
-//   bf16: what becomes an operand again is rounded to it; weighted keys are a sum of two bf16 parts, 16 bits, as the
-//     state may be returned (with one part, 7 % less time for the gradients).
+//   bf16: what becomes an operand again, weighted keys among it, is rounded to it.
 //   fp16: scores in fp16 as they are.  fp16's range would not hold what becomes an operand again, so that
 //     and what meets it are sums of two bf16 parts, 16 bits of a value and all 11 of fp16; of the four products the
 //     smallest, of both second parts, is left out (2^-16).
+//
+// Where the state is returned, weighted keys are three bf16 parts in both, fp32's 24 bits (FINE; 4 x 4096 tokens x 16 heads
+// in bf16, gradients: 272 us with one part, 295 with two).
 template<class T> struct Cores {
    typedef float E;
    typedef f32x4 Frag, Plain;            // operands in E; of q and k as they are
-   static constexpr int KEY_PARTS = 1;   // of weighted keys
+   static constexpr int KEY_PARTS = 1, FINE_PARTS = 1;       // of weighted keys
    static constexpr int PARTS = 1;       // of values, weights, the state, and q where it meets that
    static __device__ inline f32x4 mma(Frag a, Frag b, f32x4 c)
    {
@@ -65,7 +67,7 @@ template<class T> struct Cores {
 template<> struct Cores<bf16> {
    typedef bf16 E;
    typedef bf16x8 Frag, Plain;
-   static constexpr int KEY_PARTS = 2, PARTS = 1;
+   static constexpr int KEY_PARTS = 1, FINE_PARTS = 3, PARTS = 1;
    static __device__ inline f32x4 mma(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
    static __device__ inline f32x4 scores(Plain a, Plain b, f32x4 c) { return mma(a, b, c); }
 };
@@ -73,7 +75,7 @@ template<> struct Cores<f16> {
    typedef bf16 E;
    typedef bf16x8 Frag;
    typedef f16x8 Plain;
-   static constexpr int KEY_PARTS = 2, PARTS = 2;
+   static constexpr int KEY_PARTS = 2, FINE_PARTS = 3, PARTS = 2;
    static __device__ inline f32x4 mma(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
    static __device__ inline f32x4 scores(Plain a, Plain b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
@@ -200,11 +202,11 @@ __device__ inline float power(float g2, float n) { return __builtin_amdgcn_exp2f
 
 // LDS of a kernel: keys as they are, values by channel, weighted keys by channel, the state by
 // value channel; the first and the last are not needed for a segment's own part.
-template<class T, int DK, int DV, bool LOCAL> struct Room {
+template<class T, int DK, int DV, bool LOCAL, bool FINE> struct Room {
    typedef Cores<T> C;
-   static constexpr int E = sizeof(typename C::E);
+   static constexpr int E = sizeof(typename C::E), KEY_PARTS = FINE ? C::FINE_PARTS : C::KEY_PARTS;
    static constexpr int TP = kChunk * E, KP = pitch_of(DK * E);       // bytes of a row of tokens, of keys' channels
-   static constexpr int VALUES = 0, KEYS_T = VALUES + C::PARTS * DV * TP, KEYS = KEYS_T + C::KEY_PARTS * DK * TP;
+   static constexpr int VALUES = 0, KEYS_T = VALUES + C::PARTS * DV * TP, KEYS = KEYS_T + KEY_PARTS * DK * TP;
    static constexpr int STATE = LOCAL ? KEYS : KEYS + kChunk * KP, FLAGS = LOCAL ? KEYS : STATE + C::PARTS * DV * KP;
    static constexpr int BYTES = FLAGS + 16;
 };
@@ -220,7 +222,7 @@ __device__ inline void put4(uint8_t* to, const float (&v)[4])
    else *reinterpret_cast<bf16x4*>(to) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
 }
 
-template<class T, int DK, int DV, bool LOCAL, bool WHOLE>
+template<class T, int DK, int DV, bool LOCAL, bool WHOLE, bool FINE>
 __global__ void __launch_bounds__(kLanes)
 decay_chunks(DecayParams p)
 {
@@ -228,7 +230,7 @@ decay_chunks(DecayParams p)
    typedef typename C::E E;
    typedef typename C::Frag Frag;
    typedef typename C::Plain Plain;
-   typedef Room<T, DK, DV, LOCAL> M;
+   typedef Room<T, DK, DV, LOCAL, FINE> M;
    constexpr int BLOCK = sizeof(E) == 2 ? 32 : 16;             // of the summed index of a product
    constexpr int EACH = BLOCK / 16;                            // results to a block
    constexpr int NK = DK / BLOCK, NS = kChunk / BLOCK;          // blocks of keys' channels, of tokens
@@ -462,9 +464,10 @@ decay_chunks(DecayParams p)
 #pragma unroll
             for(int i = 0; i < 8; i++) x[i] = kr[i].value(j) * wk[i];
             put_tokens(M::KEYS_T, kc + j, slot_of<E>(kt), x);
-            if constexpr(C::KEY_PARTS == 2) {
+#pragma unroll
+            for(int part = 1; part < M::KEY_PARTS; part++) {
                rest(x);
-               put_tokens(M::KEYS_T + DK * TP, kc + j, slot_of<E>(kt), x);
+               put_tokens(M::KEYS_T + part * DK * TP, kc + j, slot_of<E>(kt), x);
             }
          }
       }
@@ -640,7 +643,7 @@ decay_chunks(DecayParams p)
          for(int c = 0; c < SB; c++) S[a][c] *= an;
 #pragma unroll
       for(int sb = 0; sb < NS; sb++) {
-         Frag x[SB][C::PARTS], w[SA][C::KEY_PARTS];
+         Frag x[SB][C::PARTS], w[SA][M::KEY_PARTS];
          if constexpr(!LOCAL)
             if(more) fetch_q(t1, sb * NK / NS, (sb + 1) * NK / NS);
 #pragma unroll
@@ -650,12 +653,12 @@ decay_chunks(DecayParams p)
 #pragma unroll
          for(int a = 0; a < SA; a++)
 #pragma unroll
-            for(int part = 0; part < C::KEY_PARTS; part++) w[a][part] = token_frag(M::KEYS_T, part * DK + k0 + a * 16, sb);
+            for(int part = 0; part < M::KEY_PARTS; part++) w[a][part] = token_frag(M::KEYS_T, part * DK + k0 + a * 16, sb);
 #pragma unroll
-         for(int i = 0; i < C::KEY_PARTS; i++)
+         for(int i = 0; i < M::KEY_PARTS; i++)
 #pragma unroll
             for(int j = 0; j < C::PARTS; j++)
-               if(i + j < 2)
+               if(i + j < M::KEY_PARTS)
 #pragma unroll
                   for(int a = 0; a < SA; a++)
 #pragma unroll
@@ -801,13 +804,13 @@ decay_step(StepParams p)
 
 // ---- launches --------------------------------------------------------------------------------
 
-template<class T, int DK, int DV, bool LOCAL, bool WHOLE>
+template<class T, int DK, int DV, bool LOCAL, bool WHOLE, bool FINE>
 hipError_t chunks_shape(DecayParams p, int roles, hipStream_t s)
 {
-   constexpr int bytes = Room<T, DK, DV, LOCAL>::BYTES;
+   constexpr int bytes = Room<T, DK, DV, LOCAL, FINE>::BYTES;
    static_assert(bytes <= 160 * 1024, "fits the LDS");
    static std::atomic<uint64_t> mask{0};
-   const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(&decay_chunks<T, DK, DV, LOCAL, WHOLE>), bytes, mask);
+   const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(&decay_chunks<T, DK, DV, LOCAL, WHOLE, FINE>), bytes, mask);
    if(e != hipSuccess) return e;
    int most = 0;
    for(int r = 0; r < roles; r++) most = p.role[r].dv > most ? p.role[r].dv : most;
@@ -815,11 +818,11 @@ hipError_t chunks_shape(DecayParams p, int roles, hipStream_t s)
    p.items = p.pairs * (LOCAL ? p.parts - 1 : p.segments);
    const int64_t groups = (p.items + 7) / 8 * 8 * p.slices;
    if(!grid_ok(groups, kLanes)) return kTooLarge;
-   decay_chunks<T, DK, DV, LOCAL, WHOLE><<<dim3((unsigned)groups, (unsigned)roles), kLanes, bytes, s>>>(p);
+   decay_chunks<T, DK, DV, LOCAL, WHOLE, FINE><<<dim3((unsigned)groups, (unsigned)roles), kLanes, bytes, s>>>(p);
    return hipGetLastError();
 }
 
-template<class T, int DK, int DV, bool WHOLE>
+template<class T, int DK, int DV, bool WHOLE, bool FINE>
 hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
 {
    // Segments so that each CU has as many workgroups as fit its LDS; below 4 chunks the two launches more cost what
@@ -828,7 +831,7 @@ hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
    constexpr int64_t PARTS = 2;
    const int64_t chunks = (p.tokens + kChunk - 1) / kChunk;
    const int64_t groups = p.pairs * roles * ((p.role[0].dv + DV - 1) / DV);
-   const int64_t fit = 256 * (160 * 1024 / Room<T, DK, DV, false>::BYTES);
+   const int64_t fit = 256 * (160 * 1024 / Room<T, DK, DV, false, FINE>::BYTES);
    int64_t n = fit / (groups > 0 ? groups : 1);
    if(n > p.splits) n = p.splits;
    if(n > chunks) n = chunks;
@@ -840,7 +843,7 @@ hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
    p.parts = chunks > 0 ? (chunks + each - 1) / each : 1;
    p.segments = (p.parts + parts - 1) / parts;
    if(p.segments > 1) {
-      hipError_t e = chunks_shape<T, DK, DV, true, WHOLE>(p, roles, s);
+      hipError_t e = chunks_shape<T, DK, DV, true, WHOLE, FINE>(p, roles, s);
       if(e != hipSuccess) return e;
       int64_t most = 0;
       for(int r = 0; r < roles; r++) {
@@ -852,17 +855,29 @@ hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
       e = hipGetLastError();
       if(e != hipSuccess) return e;
    }
-   return chunks_shape<T, DK, DV, false, WHOLE>(p, roles, s);
+   return chunks_shape<T, DK, DV, false, WHOLE, FINE>(p, roles, s);
 }
 
-// WHOLE: heads of whole groups of 8 channels
+// WHOLE: heads of whole groups of 8 channels.  Two parts of everything leave neither registers nor LDS for 128 values
+// of other heads, or with three of the keys.
+template<class T, int DK, int DV, bool FINE>
+hipError_t chunks_fine(const DecayParams& p, int roles, hipStream_t s)
+{
+   if constexpr(Cores<T>::PARTS == 2 && DV == 128 && FINE) {
+      return chunks_fine<T, DK, 64, FINE>(p, roles, s);
+   } else {
+      const bool whole = p.role[0].dk % 8 == 0 && p.role[0].dv % 8 == 0;
+      if(whole) return segments_launches<T, DK, DV, true, FINE>(p, roles, s);
+      return segments_launches<T, DK, Cores<T>::PARTS == 2 ? 64 : DV, false, FINE>(p, roles, s);
+   }
+}
 template<class T, int DK, int DV>
 hipError_t chunks_launches(const DecayParams& p, int roles, hipStream_t s)
 {
-   const bool whole = p.role[0].dk % 8 == 0 && p.role[0].dv % 8 == 0;
-   if(whole) return segments_launches<T, DK, DV, true>(p, roles, s);
-   if constexpr(DV == 64 || Cores<T>::PARTS == 1) return segments_launches<T, DK, DV, false>(p, roles, s);
-   else return segments_launches<T, DK, 64, false>(p, roles, s);        // two parts of everything leave no registers for more
+   if constexpr(Cores<T>::FINE_PARTS > 1)
+      for(int r = 0; r < roles; r++)
+         if(p.role[r].new_state) return chunks_fine<T, DK, DV, true>(p, roles, s);
+   return chunks_fine<T, DK, DV, false>(p, roles, s);
 }
 
 // roles whose keys have the same width

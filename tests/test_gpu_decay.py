@@ -197,6 +197,9 @@ def test_later_tokens_do_not_matter(dev, rng, kind):
     for t in x:
         t[:, 130:] = float("nan")
     out, new = torch.zeros_like(v), torch.empty(batch, heads, dk, dv, device=dev)
+    ff.decay_attention(*x, g, out, lens=n)
+    assert torch.equal(out[:, :130], clean[:, :130]) and not out[:, 130:].any()
+    ff.decay_attention(q, k, v, g, clean, new_state=new)
     ff.decay_attention(*x, g, out, new_state=new, lens=n)
     assert torch.equal(out[:, :130], clean[:, :130]) and not out[:, 130:].any() and bool(new.isfinite().all())
 
