@@ -260,7 +260,8 @@ decay_chunks(DecayParams p)
    if(first >= len && seg > 0) return;
    const int64_t most = LOCAL ? p.part : p.segment;
    const int left = (int)(len - first < most ? len - first : most);      // this segment's tokens
-   if(LOCAL && first + left >= len) return;                    // the last segment's part is not asked for
+   // the last part of all is only for the state behind the tokens
+   if(LOCAL && first + left >= len && !role.new_state) return;
    const int dk = role.dk, dv = role.dv, dv0 = slice * DV;
    if(dv0 >= dv) return;                                       // a role of fewer slices
    const int dvn = dv - dv0 < DV ? dv - dv0 : DV;
@@ -687,22 +688,27 @@ decay_scan(DecayParams p)
    }
    float g2 = p.log_decay[h] * 1.44269504f;
    g2 = g2 < -1e30f ? -1e30f : g2;
-   const float a = power(g2, (float)p.part);                  // every part but the last is whole
-   float s = 0.0f;
-   if(role.state) s = role.state[bh * count + (role.turned ? e % role.dv * role.dk + e / role.dv : e)];
+   const float a = power(g2, (float)p.part);                   // of every part but the last
+   const int64_t at = bh * count + (role.turned ? e % role.dv * role.dk + e / role.dv : e);
+   float s = role.state ? role.state[at] : 0.0f;
    float* const work = role.work + bh * count + e;
-   const int64_t pitch = p.pairs * count;
+   const int64_t pitch = p.pairs * count, last = role.new_state ? len : len - 1;     // parts that end up to there are there
    constexpr int AHEAD = 8;
    for(int64_t seg = 0; seg < p.parts && (seg == 0 || seg * p.part < len); seg += AHEAD) {
       float part[AHEAD];
 #pragma unroll
-      for(int i = 0; i < AHEAD; i++) part[i] = (seg + i + 1) * p.part < len ? work[(seg + i) * pitch] : 0.0f;
+      for(int i = 0; i < AHEAD; i++) {
+         const int64_t from = (seg + i) * p.part, to = from + p.part < len ? from + p.part : len;
+         part[i] = from < len && to <= last ? work[(seg + i) * pitch] : 0.0f;
+      }
 #pragma unroll
       for(int i = 0; i < AHEAD; i++) {
-         if(seg + i < p.parts && (seg + i == 0 || (seg + i) * p.part < len)) work[(seg + i) * pitch] = s;
-         s = a * s + part[i];
+         const int64_t from = (seg + i) * p.part;
+         if(seg + i < p.parts && (seg + i == 0 || from < len)) work[(seg + i) * pitch] = s;
+         if(from < len) s = (from + p.part <= len ? a : power(g2, (float)(len - from))) * s + part[i];
       }
    }
+   if(role.new_state) role.new_state[at] = s;
 }
 
 // ---- one token ------------------------------------------------------------------------------
@@ -815,7 +821,7 @@ hipError_t chunks_shape(DecayParams p, int roles, hipStream_t s)
    int most = 0;
    for(int r = 0; r < roles; r++) most = p.role[r].dv > most ? p.role[r].dv : most;
    p.slices = (most + DV - 1) / DV;
-   p.items = p.pairs * (LOCAL ? p.parts - 1 : p.segments);
+   p.items = p.pairs * (LOCAL ? p.parts : p.segments);         // the last part: where its sum is asked for
    const int64_t groups = (p.items + 7) / 8 * 8 * p.slices;
    if(!grid_ok(groups, kLanes)) return kTooLarge;
    decay_chunks<T, DK, DV, LOCAL, WHOLE, FINE><<<dim3((unsigned)groups, (unsigned)roles), kLanes, bytes, s>>>(p);
@@ -842,20 +848,21 @@ hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
    p.segment = p.part * parts;
    p.parts = chunks > 0 ? (chunks + each - 1) / each : 1;
    p.segments = (p.parts + parts - 1) / parts;
-   if(p.segments > 1) {
-      hipError_t e = chunks_shape<T, DK, DV, true, WHOLE, FINE>(p, roles, s);
-      if(e != hipSuccess) return e;
-      int64_t most = 0;
-      for(int r = 0; r < roles; r++) {
-         const int64_t per = ((int64_t)p.role[r].dk * p.role[r].dv + 255) / 256;
-         most = per > most ? per : most;
-      }
-      if(!grid_ok(p.pairs * most, 256)) return kTooLarge;
-      decay_scan<<<dim3((unsigned)(p.pairs * most), (unsigned)roles), 256, 0, s>>>(p);
-      e = hipGetLastError();
-      if(e != hipSuccess) return e;
+   if(p.segments == 1) return chunks_shape<T, DK, DV, false, WHOLE, FINE>(p, roles, s);
+   hipError_t e = chunks_shape<T, DK, DV, true, WHOLE, FINE>(p, roles, s);
+   if(e != hipSuccess) return e;
+   int64_t most = 0;
+   for(int r = 0; r < roles; r++) {
+      const int64_t per = ((int64_t)p.role[r].dk * p.role[r].dv + 255) / 256;
+      most = per > most ? per : most;
    }
-   return chunks_shape<T, DK, DV, false, WHOLE, FINE>(p, roles, s);
+   if(!grid_ok(p.pairs * most, 256)) return kTooLarge;
+   decay_scan<<<dim3((unsigned)(p.pairs * most), (unsigned)roles), 256, 0, s>>>(p);
+   e = hipGetLastError();
+   if(e != hipSuccess) return e;
+   // the state behind the tokens is there, from the parts' sums
+   for(int r = 0; r < roles; r++) p.role[r].new_state = nullptr;
+   return chunks_shape<T, DK, DV, false, WHOLE, false>(p, roles, s);
 }
 
 // WHOLE: heads of whole groups of 8 channels.  Two parts of everything leave neither registers nor LDS for 128 values
