@@ -304,6 +304,114 @@ inline int conv(const Cache& c, const void* taps, Type tap_type, int64_t tap_cou
 
 }  // namespace mx4
 
+// ---- norms, 8-bit rows and decaying linear attention (no reference counterpart; fufft.h) -------
+namespace layer {
+
+using mx4::Matrix;
+using mx4::MutableMatrix;
+using mx4::Type;
+
+inline int64_t padded(int64_t k) { return fufft_i8_padded(k); }
+inline std::size_t code_bytes(int64_t rows, int64_t k) { return (std::size_t)(rows * padded(k)); }
+
+// 8-bit rows and their scales
+struct Rows8 {
+   void*  codes  = nullptr;
+   float* scales = nullptr;
+};
+
+inline int quantize(const Matrix& x, Rows8 to, void* stream = nullptr)
+{
+   return fufft_i8_quantize(x.data, (int)x.type, x.stride(), x.rows, x.k, to.codes, to.scales, stream);
+}
+inline int dequantize(Rows8 b, const MutableMatrix& out, void* stream = nullptr)
+{
+   return fufft_i8_dequantize(b.codes, b.scales, out.data, (int)out.type, out.stride(), out.rows, out.k, stream);
+}
+// out (m x n) = a b^T + bias, a m rows and b n rows of k values
+inline int matmul(Rows8 a, Rows8 b, const MutableMatrix& out, int64_t k, void* stream = nullptr,
+                  const float* bias = nullptr)
+{
+   return fufft_i8_matmul(a.codes, a.scales, b.codes, b.scales, bias, out.data, (int)out.type, out.stride(), out.rows,
+                          out.k, k, stream);
+}
+
+// rows that a norm may leave out
+struct Optional {
+   void*   data = nullptr;
+   int64_t ld   = 0;
+};
+// out, or codes, or both are given; `sums`: the type of residual and total
+struct Norm {
+   Optional     residual = {}, total = {}, out = {};
+   Rows8        codes  = {};
+   const float* weight = nullptr;
+   float        eps    = 1e-6f;
+};
+inline int rms_norm(const Matrix& x, const Norm& n, Type sums, void* stream = nullptr)
+{
+   const auto ld = [&](const Optional& m) { return m.ld ? m.ld : x.k; };
+   return fufft_rms_norm(x.data, (int)x.type, x.stride(), n.residual.data, ld(n.residual), n.total.data, ld(n.total),
+                         (int)sums, n.weight, n.eps, n.out.data, ld(n.out), n.codes.codes, n.codes.scales, x.rows, x.k,
+                         stream);
+}
+// h's type is that of the sums; work: splits x k floats where dweight is given
+inline int rms_norm_grad(const Matrix& dy, const Matrix& h, const Optional& dtotal, const float* weight, float eps,
+                         const MutableMatrix& dx, float* dweight, float* work, int64_t splits, void* stream = nullptr)
+{
+   if(h.rows != dy.rows || h.k != dy.k || dx.rows != dy.rows || dx.k != dy.k) return FUFFT_ERR_INVALID;
+   return fufft_rms_norm_grad(dy.data, (int)dy.type, dy.stride(), h.data, h.stride(), dtotal.data,
+                              dtotal.ld ? dtotal.ld : dy.k, (int)h.type, weight, eps, dx.data, (int)dx.type, dx.stride(),
+                              dweight, work, splits, dy.rows, dy.k, stream);
+}
+
+// batch x tokens x heads x dim of the call's type
+struct Heads {
+   const void*   data;
+   fufft_strides strides;
+};
+struct MutableHeads {
+   void*         data;
+   fufft_strides strides;
+};
+// the sizes that a call's arrays share, and what it may be given besides
+struct Decay {
+   int64_t        batch, tokens, heads, dk, dv;
+   Type           type;
+   const float*   log_decay;
+   float          scale  = 1.0f;
+   const int32_t* lens   = nullptr;
+   float*         work   = nullptr;  // splits x batch x heads x dk x dv floats, three times that for the gradients
+   int64_t        splits = 0;
+};
+inline int attention(const Decay& d, const Heads& q, const Heads& k, const Heads& v, const MutableHeads& out,
+                     const float* state = nullptr, float* new_state = nullptr, void* stream = nullptr)
+{
+   return fufft_decay_attention(q.data, &q.strides, k.data, &k.strides, v.data, &v.strides, (int)d.type, d.log_decay,
+                                out.data, &out.strides, state, new_state, d.lens, d.scale, d.batch, d.tokens, d.heads,
+                                d.dk, d.dv, d.work, d.splits, stream);
+}
+inline int attention_grad(const Decay& d, const Heads& dout, const Heads& q, const Heads& k, const Heads& v,
+                          const MutableHeads& dq, const MutableHeads& dk, const MutableHeads& dv,
+                          const float* state = nullptr, const float* dnew_state = nullptr, float* dstate = nullptr,
+                          void* stream = nullptr)
+{
+   return fufft_decay_attention_grad(dout.data, &dout.strides, q.data, &q.strides, k.data, &k.strides, v.data, &v.strides,
+                                     (int)d.type, d.log_decay, dq.data, &dq.strides, dk.data, &dk.strides, dv.data,
+                                     &dv.strides, state, dnew_state, dstate, d.lens, d.scale, d.batch, d.tokens, d.heads,
+                                     d.dk, d.dv, d.work, d.splits, stream);
+}
+// one token of every sequence; tokens, lens, work and splits of `d` are unused
+inline int step(const Decay& d, const Heads& q, const Heads& k, const Heads& v, const MutableHeads& out, float* state,
+                int64_t slot_count, const int64_t* slots = nullptr, void* stream = nullptr)
+{
+   return fufft_decay_attention_step(q.data, &q.strides, k.data, &k.strides, v.data, &v.strides, (int)d.type, d.log_decay,
+                                     out.data, &out.strides, state, slot_count, slots, d.scale, d.batch, d.heads, d.dk,
+                                     d.dv, stream);
+}
+
+}  // namespace layer
+
 // ---- the reference's launch surface, by name --------------------------------------------
 // A caller of the reference instantiates a kernel template whose parameters
 // spell out the plan and launches it, e.g. (bench_fufft.cu:216-221)
