@@ -1166,7 +1166,7 @@ def rms_norm_grad(dy, h, weight, dx, dweight=None, work=None, *, dtotal=None, ep
 # ---- linear attention with a decay for each head ------------------------------------------
 # q, k (batch, tokens, heads, dk), v and out (batch, tokens, heads, dv) in one type (fp32, bf16, fp16), the
 # elements of a head adjacent and any strides otherwise (of an input 0 too); log_decay fp32 (heads),
-# <= 0; states fp32 (batch, heads, dk, dv), contiguous.
+# <= 0; states fp32 (batch, heads, dk, dv), contiguous.  A workspace belongs to one call at a time.
 
 class _Strides(C.Structure):
     _fields_ = [("batch", C.c_int64), ("token", C.c_int64), ("head", C.c_int64)]

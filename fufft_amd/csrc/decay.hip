@@ -44,13 +44,15 @@ constexpr int kChunk = 64, kLanes = 512;
 // of two results (with g = lane / 16), or whose block of 16 takes those of one.
 //
 //   fp32: everything in fp32, whose products run at a sixteenth of the others' rate and bound these kernels.
-//   bf16: what becomes an operand again, weighted keys among it, is rounded to it.
+//   bf16: what becomes an operand again is rounded to it, but for weighted keys, which are two parts (below): all three
+//     roundings, of keys, state and scores, would leave sqrt(3) of the error that bf16 results have anyway, two sqrt(2).
 //   fp16: scores in fp16 as they are.  fp16's range would not hold what becomes an operand again, so that
 //     and what meets it are sums of two bf16 parts, 16 bits of a value and all 11 of fp16; of the four products the
 //     smallest, of both second parts, is left out (2^-16).
 //
-// Where the state is returned, weighted keys are three bf16 parts in both, fp32's 24 bits (FINE; 4 x 4096 tokens x 16 heads
-// in bf16, gradients: 272 us with one part, 295 with two).
+// Where the state is returned, weighted keys are three bf16 parts in both, fp32's 24 bits (FINE): in the launch whose sums
+// become that state, which is the first one where tokens are split (65536 tokens x 16 heads in bf16 with its state: 490 us
+// with three parts in both launches, 462 so).
 template<class T> struct Cores {
    typedef float E;
    typedef f32x4 Frag, Plain;            // operands in E; of q and k as they are
@@ -67,7 +69,7 @@ template<class T> struct Cores {
 template<> struct Cores<bf16> {
    typedef bf16 E;
    typedef bf16x8 Frag, Plain;
-   static constexpr int KEY_PARTS = 1, FINE_PARTS = 3, PARTS = 1;
+   static constexpr int KEY_PARTS = 2, FINE_PARTS = 3, PARTS = 1;
    static __device__ inline f32x4 mma(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
    static __device__ inline f32x4 scores(Plain a, Plain b, f32x4 c) { return mma(a, b, c); }
 };
@@ -837,7 +839,7 @@ hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
    constexpr int64_t PARTS = 2;
    const int64_t chunks = (p.tokens + kChunk - 1) / kChunk;
    const int64_t groups = p.pairs * roles * ((p.role[0].dv + DV - 1) / DV);
-   const int64_t fit = 256 * (160 * 1024 / Room<T, DK, DV, false, FINE>::BYTES);
+   const int64_t fit = 256 * (160 * 1024 / Room<T, DK, DV, false, false>::BYTES);
    int64_t n = fit / (groups > 0 ? groups : 1);
    if(n > p.splits) n = p.splits;
    if(n > chunks) n = chunks;

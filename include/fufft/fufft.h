@@ -594,7 +594,8 @@ int fufft_mx4_cache_conv(const void* codes, const uint8_t* scales, int64_t pages
  * calls above.  Every sum, state and statistic is fp32 (integer sums int32), rounded
  * once to the output's type.  Outputs share no byte with another buffer of the call, but for
  * those named below that may be one of its inputs, the same address and strides.
- * Sizes that no launch can hold are FUFFT_ERR_UNSUPPORTED.
+ * Sizes that no launch can hold are FUFFT_ERR_UNSUPPORTED.  A workspace belongs to one call at
+ * a time: calls or graphs that may run together need one each.
  *
  * 8-bit rows: a row of k values is fufft_i8_padded(k) signed bytes (k up to a multiple of
  * 128; the padding holds zeros, and the quantizing calls write them) and one fp32 scale.
@@ -657,9 +658,9 @@ int fufft_rms_norm_grad(const void* dy, int type, int64_t ldy, const void* h, in
  *   work       fp32 space for `splits` states of every sequence and head (splits x batch x heads
  *              x dk x dv): the tokens are split over at most that many workgroups.
  *              0 (NULL) is allowed.  About 1024 / (batch * heads) are as many as help.
- * Sums are fp32.  Of bf16 inputs, weighted scores, the state that q meets and keys weighted on
- * their way into it are rounded to bf16 before their products; of fp16 inputs all of these
- * are kept to 16 bits; fp32 inputs are multiplied in fp32.  Where the state is asked for, weighted
+ * Sums are fp32.  Of bf16 inputs, weighted scores and the state that q meets are rounded to
+ * bf16 before their products, and keys weighted on their way into the state are kept to 16 bits; of
+ * fp16 inputs all of these are kept to 16 bits; fp32 inputs are multiplied in fp32.  Where the state is asked for, weighted
  * keys are kept to 24 bits (results can differ in their last bits from a call that does not ask).
  * A token's result does not depend on later tokens, whatever they hold.  An infinite key or value
  * of 16-bit inputs may make NaN of the state's element that would be infinite. */

@@ -131,7 +131,7 @@ def mixed_share(kind, tokens, dim, log_decay, carried=False):
     """The share of the magnitudes that the call's arithmetic may be off by, before the result's own rounding.
     fp32's part: sums of dim and of 64 terms a chunk, up to five products a term, the chunk's decay; powers whose exponent
     is off by its own rounding, 2^-23 of |log_decay| tokens.
-    bf16: weighted scores are rounded once, at 2^-8; in the state that q meets the weighted keys and the state itself, each once.
+    bf16: weighted scores are rounded once, at 2^-8, and so is the state that q meets; two bf16 parts of weighted keys leave 2^-16.
     fp16: two bf16 parts of a weight, of the state and of weighted keys each leave 2^-16, and a product of second parts that is left
     out 2^-16, so 2^-15 in the state and as much again where q meets it.
     A state that is returned (carried): three bf16 parts of weighted keys leave 2^-24, and the products of fp16's parts that
@@ -141,7 +141,7 @@ def mixed_share(kind, tokens, dim, log_decay, carried=False):
     chain = dim + 64 + (64 * 5 + 4) * chunks + 12 + 4 * decay * (tokens + 1)
     if carried:
         return (chain + 3) * EPS24
-    return chain * EPS24 + {"f32": 0.0, "bf16": 1.02 * 2.0 ** -8 * 2, "f16": 1.05 * 2.0 ** -14}[kind]
+    return chain * EPS24 + {"f32": 0.0, "bf16": 1.02 * 2.0 ** -8, "f16": 1.05 * 2.0 ** -14}[kind]
 
 
 def attention(q, k, v, log_decay, state, lens, scale, kind):
