@@ -850,7 +850,9 @@ hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
    p.segment = p.part * parts;
    p.parts = chunks > 0 ? (chunks + each - 1) / each : 1;
    p.segments = (p.parts + parts - 1) / parts;
-   if(p.segments == 1) return chunks_shape<T, DK, DV, false, WHOLE, FINE>(p, roles, s);
+   // two parts of everything and three of the keys of 128 values leave neither registers nor LDS
+   constexpr int ONE = Cores<T>::PARTS == 2 && FINE ? 64 : DV;
+   if(p.segments == 1) return chunks_shape<T, DK, ONE, false, WHOLE, FINE>(p, roles, s);
    hipError_t e = chunks_shape<T, DK, DV, true, WHOLE, FINE>(p, roles, s);
    if(e != hipSuccess) return e;
    int64_t most = 0;
@@ -868,17 +870,13 @@ hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
 }
 
 // WHOLE: heads of whole groups of 8 channels.  Two parts of everything leave neither registers nor LDS for 128 values
-// of other heads, or with three of the keys.
+// of other heads.
 template<class T, int DK, int DV, bool FINE>
 hipError_t chunks_fine(const DecayParams& p, int roles, hipStream_t s)
 {
-   if constexpr(Cores<T>::PARTS == 2 && DV == 128 && FINE) {
-      return chunks_fine<T, DK, 64, FINE>(p, roles, s);
-   } else {
-      const bool whole = p.role[0].dk % 8 == 0 && p.role[0].dv % 8 == 0;
-      if(whole) return segments_launches<T, DK, DV, true, FINE>(p, roles, s);
-      return segments_launches<T, DK, Cores<T>::PARTS == 2 ? 64 : DV, false, FINE>(p, roles, s);
-   }
+   const bool whole = p.role[0].dk % 8 == 0 && p.role[0].dv % 8 == 0;
+   if(whole) return segments_launches<T, DK, DV, true, FINE>(p, roles, s);
+   return segments_launches<T, DK, Cores<T>::PARTS == 2 ? 64 : DV, false, FINE>(p, roles, s);
 }
 template<class T, int DK, int DV>
 hipError_t chunks_launches(const DecayParams& p, int roles, hipStream_t s)
