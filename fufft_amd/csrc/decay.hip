@@ -833,18 +833,20 @@ hipError_t chunks_shape(DecayParams p, int roles, hipStream_t s)
 template<class T, int DK, int DV, bool WHOLE, bool FINE>
 hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
 {
-   // Segments so that each CU has as many workgroups as fit its LDS; below 4 chunks the two launches more cost what
-   // they save.  A segment of several chunks is PARTS parts in the first launch, which has room for more workgroups on
+   // Segments so that each CU has a workgroup, where that pays, with a chunk's time in the last launch for a unit: a chunk in the
+   // first launch half of it, the state of every part, which is written, read, written and read, 5 times its share of a
+   // chunk's bytes, the launches 3.5 (128 channels in bf16, out with its state, us unsplit / split: 64 pairs of a sequence and a head,
+   // 32 chunks, 141 / 88; 85 pairs 144 / 108; 128 pairs 160 / 147; 8 chunks 43 / 61; 64 pairs of 4 chunks 25 / 34).
+   // A segment of many chunks is two parts in the first launch, which has room for more workgroups on
    // a CU (65536 tokens x 16 heads: 197 us in one part, 152 in 3, 142 in 2).
-   constexpr int64_t PARTS = 2;
    const int64_t chunks = (p.tokens + kChunk - 1) / kChunk;
    const int64_t groups = p.pairs * roles * ((p.role[0].dv + DV - 1) / DV);
-   const int64_t fit = 256 * (160 * 1024 / Room<T, DK, DV, false, false>::BYTES);
-   int64_t n = fit / (groups > 0 ? groups : 1);
+   constexpr int64_t STATES = 10 * (4 * DK * DV) / (2 * kChunk * (DK + DV) * (int)sizeof(T));      // in halves of a chunk, as below
+   int64_t n = 256 / (groups > 0 ? groups : 1);
    if(n > p.splits) n = p.splits;
    if(n > chunks) n = chunks;
-   if(n < 1 || chunks < 4) n = 1;
-   const int64_t parts = p.splits / n >= PARTS && chunks / n >= 2 * PARTS ? PARTS : 1;
+   if(n < 2 || 3 * ((chunks + n - 1) / n) + 7 + STATES >= 2 * chunks) n = 1;
+   const int64_t parts = p.splits / n >= 2 && chunks / n >= 16 ? 2 : 1;
    const int64_t each = chunks > 0 ? (chunks + n * parts - 1) / (n * parts) : 1;       // chunks of a part
    p.part = each * kChunk;
    p.segment = p.part * parts;
