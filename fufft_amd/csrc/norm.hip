@@ -43,16 +43,31 @@ __device__ inline Eight<T> fetch8_whole(const T* row, int64_t col, int64_t k)
 {
    return *reinterpret_cast<const Eight<T>*>(row + (col < k ? col : 0));
 }
+// past: beyond the L2, of 16-bit elements
 template<class T>
-__device__ inline void put8(T* row, int64_t col, int64_t k, const float (&v)[8])
+__device__ inline void put8(T* row, int64_t col, int64_t k, const float (&v)[8], bool past = false)
 {
    if(col + 8 <= k) {
-      store8<T>(row + col, v);
+      if(sizeof(T) == 2 && past) {
+         typedef uint32_t V __attribute__((ext_vector_type(2 * sizeof(T)), aligned(sizeof(T))));
+         Eight<T> t;
+#pragma unroll
+         for(int i = 0; i < 8; i++) t.e[i] = (T)v[i];
+         __builtin_nontemporal_store(__builtin_bit_cast(V, t), reinterpret_cast<V*>(row + col));
+      } else {
+         store8<T>(row + col, v);
+      }
    } else {
 #pragma unroll
       for(int i = 0; i < 8; i++)
          if(col + i < k) row[col + i] = (T)v[i];
    }
+}
+
+__device__ inline void put_codes(int8_t* to, u32x2 c, bool past)
+{
+   if(past) __builtin_nontemporal_store(c, reinterpret_cast<u32x2*>(to));
+   else     *reinterpret_cast<u32x2*>(to) = c;
 }
 
 // ---- sums and maxima over the lanes of a row ----------------------------------------
@@ -252,11 +267,11 @@ __device__ inline u32x2 codes8(const float (&y)[8], const Step& s)
 // ---- the norm, and rows to 8 bits (NORM false: y = x) -----------------------------------
 //
 // LANES lanes have a row, V vectors of 8 elements each; a workgroup of 256 has 64 rows at 4 lanes, 16 at 16, 4 at 64.
-// 8192 x 4096 in bf16: norm 26.9 us (5.0 TB/s), with an fp32 residual, total and 8-bit rows 69 (5.3), rows to 8 bits
-// 20.5 (4.9); a torch copy runs at 5.3.
+// 8192 x 4096 in bf16: norm 21.7 us (6.2 TB/s), with an fp32 residual, total and 8-bit rows 69 (5.3), rows to 8 bits
+// 20 (5.0); a torch copy runs at 5.3.
 template<class X, class S, int LANES, int V, bool NORM>
-__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES)
-norm_rows(NormParams p, int64_t kp)
+__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES, LANES == 1024 && !NORM ? 8 : 1)     // two rows a CU
+norm_rows(NormParams p, int64_t kp, bool past)
 {
    __shared__ uint32_t side[2][16];
    constexpr int PER = LANES < 256 ? 256 / LANES : 1;
@@ -301,7 +316,7 @@ norm_rows(NormParams p, int64_t kp)
             h[v][i] = h[v][i] * f.c * f.r;
             if(p.weight) h[v][i] *= w.e[i];
          }
-         if(out) put8<X>(out, col, p.k, h[v]);
+         if(out) put8<X>(out, col, p.k, h[v], past);
       }
       if(!p.codes) return;
    }
@@ -321,16 +336,16 @@ norm_rows(NormParams p, int64_t kp)
       if(col >= kp) break;
       u32x2 c = {0, 0};
       if(finite) c = codes8(h[v], step);
-      *reinterpret_cast<u32x2*>(codes + col) = c;
+      put_codes(codes + col, c, past);
    }
 }
 
-// Rows too long for registers (32768 values in bf16 still fit: 4.3 TB/s): 1024 lanes go over their row once for the sum of squares, once for the
+// Rows too long for registers (32768 values in bf16 still fit: 4.6 TB/s): 1024 lanes go over their row once for the sum of squares, once for the
 // largest magnitude where codes are asked for, once to write.  What a lane writes it has read itself, in
 // the same trip, so total may still be residual and out x.
 template<class X, class S, bool NORM>
 __global__ void __launch_bounds__(1024)
-norm_long(NormParams p, int64_t kp)
+norm_long(NormParams p, int64_t kp, bool past)
 {
    __shared__ uint32_t side[2][16];
    const int64_t row = blockIdx.x;
@@ -387,19 +402,19 @@ norm_long(NormParams p, int64_t kp)
       sums(col, h);                                // zeros from k on
       if(NORM && p.total) put8<S>(static_cast<S*>(p.total) + row * p.ldt, col, p.k, h);
       normed(col, h);
-      if(NORM && p.out) put8<X>(static_cast<X*>(p.out) + row * p.ldo, col, p.k, h);
+      if(NORM && p.out) put8<X>(static_cast<X*>(p.out) + row * p.ldo, col, p.k, h, past);
       if(!p.codes) continue;
       u32x2 c = {0, 0};
       if(finite) c = codes8(h, step);
-      *reinterpret_cast<u32x2*>(p.codes + row * kp + col) = c;
+      put_codes(p.codes + row * kp + col, c, past);
    }
 }
 
-// one lane, eight values; a row of lanes as long as a padded row (8192 x 4096 to bf16 16.5 us, 6.1 TB/s)
+// one lane, eight values; a row of lanes as long as a padded row (8192 x 4096 to bf16 15.9 us, 6.3 TB/s)
 template<class O>
 __global__ void __launch_bounds__(256)
 dequantize_rows(const int8_t* codes, const float* scales, O* out, int64_t ld, int64_t first, int64_t rows, int64_t k,
-                int64_t kp)
+                int64_t kp, bool past)
 {
    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = kp / 8;
    const int64_t row = first + i / per, col = i % per * 8;
@@ -409,7 +424,7 @@ dequantize_rows(const int8_t* codes, const float* scales, O* out, int64_t ld, in
    float v[8];
 #pragma unroll
    for(int j = 0; j < 8; j++) v[j] = (float)(int8_t)(c[j / 4] >> (8 * (j % 4))) * s;
-   put8<O>(out + row * ld, col, k, v);
+   put8<O>(out + row * ld, col, k, v, past);
 }
 
 // ---- the norm's gradients ----------------------------------------------------------------
@@ -617,13 +632,24 @@ join_weight(const float* work, float* dweight, int64_t splits, int64_t k)
 
 // ---- launches --------------------------------------------------------------------------------
 
+// Results of half the L2s' 32 MiB and more are written past them, where they do not take the place of what comes in (8192 x 4096
+// in bf16: norm 27 / 21.7 us, back from 8 bits 16.5 / 15.9, residual, 8 bits and back 91 / 86; 2048 x 4096: norm 8.3 /
+// 6.6, but 8-bit rows and their way back 22.6 / 23.2).  Not so: fp32 results, whose lanes write two pieces (back from 8 bits 34
+// / 46.6), the gradients (67.5 / 69.2); and loads gain nothing.
+bool past_l2(int64_t bytes) { return bytes >= (int64_t)16 << 20; }
+template<class X>
+int64_t result_bytes(const NormParams& p)
+{
+   return (p.out ? p.rows * p.k * (int64_t)sizeof(X) : 0) + (p.codes ? p.rows * padded(p.k) : 0);
+}
+
 template<class X, class S, int LANES, int V, bool NORM>
 hipError_t norm_shape(const NormParams& p, hipStream_t s)
 {
    constexpr int PER = LANES < 256 ? 256 / LANES : 1, BLOCK = LANES < 256 ? 256 : LANES;
    const int64_t groups = (p.rows + PER - 1) / PER;
    if(!grid_ok(groups, BLOCK)) return kTooLarge;
-   norm_rows<X, S, LANES, V, NORM><<<(unsigned)groups, BLOCK, 0, s>>>(p, padded(p.k));
+   norm_rows<X, S, LANES, V, NORM><<<(unsigned)groups, BLOCK, 0, s>>>(p, padded(p.k), past_l2(result_bytes<X>(p)));
    return hipGetLastError();
 }
 
@@ -642,7 +668,7 @@ hipError_t norm_typed(const NormParams& p, hipStream_t s)
    if(p.k <= 16384) return norm_shape<X, S, 1024, 2, NORM>(p, s);
    if(p.k <= 32768) return norm_shape<X, S, 1024, 4, NORM>(p, s);
    if(!grid_ok(p.rows, 1024)) return kTooLarge;
-   norm_long<X, S, NORM><<<(unsigned)p.rows, 1024, 0, s>>>(p, padded(p.k));
+   norm_long<X, S, NORM><<<(unsigned)p.rows, 1024, 0, s>>>(p, padded(p.k), past_l2(result_bytes<X>(p)));
    return hipGetLastError();
 }
 
@@ -657,7 +683,7 @@ hipError_t dequantize_typed(const int8_t* codes, const float* scales, void* out,
    for(int64_t first = 0; first < rows; first += each) {
       const int64_t n = rows - first < each ? rows - first : each;
       dequantize_rows<O><<<(unsigned)((n * per + 255) / 256), 256, 0, s>>>(codes, scales, static_cast<O*>(out), ld, first,
-                                                                          first + n, k, kp);
+                                                                          first + n, k, kp, past_l2(rows * k * (int64_t)sizeof(O)));
       const hipError_t e = hipGetLastError();
       if(e != hipSuccess) return e;
    }
