@@ -1213,7 +1213,7 @@ def decay_attention(q, k, v, log_decay, out, *, state=None, new_state=None, lens
     state: S before the first token, None: zero; new_state: S after the last one (may be state).
     lens (int32, batch): tokens of each sequence; rows behind them are neither read nor written.
     work: fp32, room for splits * batch * heads * dk * dv values; the tokens are split over at most that
-    many workgroups, and about 1024 / (batch * heads) splits are as many as help."""
+    many workgroups, and about 512 / (batch * heads) splits are as many as help."""
     if _native(q):
         gpu = _current_device()
         status = _binding.decay_attention(q, k, v, log_decay, out, state, new_state, lens, work, scale, _handle(stream, gpu), gpu)

@@ -657,7 +657,7 @@ int fufft_rms_norm_grad(const void* dy, int type, int64_t ldy, const void* h, in
  *              be state;
  *   work       fp32 space for `splits` states of every sequence and head (splits x batch x heads
  *              x dk x dv): the tokens are split over at most that many workgroups.
- *              0 (NULL) is allowed.  About 1024 / (batch * heads) are as many as help.
+ *              0 (NULL) is allowed.  About 512 / (batch * heads) are as many as help.
  * Sums are fp32.  Of bf16 inputs, weighted scores and the state that q meets are rounded to
  * bf16 before their products, and keys weighted on their way into the state are kept to 16 bits; of
  * fp16 inputs all of these are kept to 16 bits; fp32 inputs are multiplied in fp32.  Where the state is asked for, weighted

@@ -140,3 +140,131 @@ def test_widths_between_kernels(dev, rng):
         back = codes[:, :k].double().cpu().numpy() * scales.double().cpu().numpy()[:, None]
         top = np.abs(want).max(1, keepdims=True)
         assert (np.abs(back - want) <= top / 254 * 1.0001 + np.abs(want) * 2 * share).all()
+
+
+def recurrence(q, k, v, g, lens, state=None, late=0):
+    """mixed of tests/layer_reference.py for all sequences and heads at once, in fp64 tensors: (out, state behind, their magnitudes)."""
+    import torch
+    batch, tokens, heads, dk = q.shape
+    a = torch.exp(g)[:, None, None]
+    s = torch.zeros(batch, heads, dk, v.shape[3], dtype=torch.float64, device=q.device) if state is None else state.clone()
+    m = s.abs()
+    out, mags = torch.zeros_like(v), torch.zeros_like(v)
+    for t in range(tokens):
+        there = (lens > t)[:, None, None, None]
+        f = torch.ones_like(a) if late and t == 0 else a
+        kv = k[:, t, :, :, None] * v[:, t, :, None, :]
+        s, m = torch.where(there, f * s + kv, s), torch.where(there, f * m + kv.abs(), m)
+        out[:, t], mags[:, t] = (q[:, t, :, :, None] * s).sum(2), (q[:, t, :, :, None].abs() * m).sum(2)
+    if late:
+        some = (lens > 0)[:, None, None, None]
+        s, m = torch.where(some, a * s, s), torch.where(some, a * m, m)
+    return out, s, mags, m
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
+@pytest.mark.parametrize("dk,dv", [(16, 24), (5, 9)])
+def test_long_split(dev, kind, dk, dv):
+    """Segments of two parts of several chunks each: 32 sequences and heads, lengths at and around the parts' ends."""
+    import torch
+    import fufft_amd as ff
+    tokens, heads = 8192, 2
+    lens = torch.tensor([8192, 0, 1, 511, 512, 513, 1024, 1025, 2047, 2048, 2049, 4096, 4097, 6144, 8128, 8191], device=dev)
+    batch = len(lens)
+    print(f"case decay long split {kind} {dk}x{dv}", flush=True)
+    gen = torch.Generator(device=dev).manual_seed(7)
+    q, k, v, do = (torch.randn(batch, tokens, heads, d, device=dev, generator=gen).to(R.torch_type(kind)) for d in (dk, dk, dv, dv))
+    state, dnew = (torch.randn(batch, heads, dk, dv, device=dev, generator=gen) for _ in range(2))
+    g = torch.tensor([-0.001, -0.3], device=dev)
+    work = torch.full((16 * 3, batch, heads, dk, dv), float("nan"), device=dev)
+    ld, scale = lens.int(), 0.25
+    x = [t.double() for t in (q, k, v, do)]
+    # a share for each head, of the longest sequence
+    share = lambda dim, carried=False: torch.tensor([R.mixed_share(kind, tokens, dim, float(h), carried) for h in g], dtype=torch.float64, device=dev)[:, None]
+    at = torch.arange(tokens, device=dev)
+    inside_len = (at[None, :] < lens[:, None])
+
+    def near(got, want, err):
+        # half a step of the type, and of its smallest number
+        eps = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[kind]
+        off = (got.double() - want).abs() - err - (want.abs() + err) * eps - 2.0 ** -25
+        assert bool((off[inside_len] <= 0).all()) and bool((got[~inside_len] == 5).all())
+
+    def carried(got, want, mags):
+        assert bool(((got.double() - want).abs() <= mags * share(0, True)[:, None] + want.abs() * 2.0 ** -24).all())
+    want, new, mags, nm = recurrence(x[0], x[1], x[2], g.double(), lens, state.double())
+    for behind in (None, torch.empty_like(state)):
+        out = torch.full_like(v, 5.0)
+        work.fill_(float("nan"))
+        ff.decay_attention(q, k, v, g, out, state=state, new_state=behind, lens=ld, work=work[:16], scale=scale)
+        near(out, scale * want, scale * mags * share(dk))
+        if behind is not None:
+            carried(behind, new, nm)
+    # the gradients, from the last token back
+    back = (lens[:, None] - 1 - at[None, :]).clamp(0)[:, :, None, None]
+    turned = [t.gather(1, back.expand_as(t)) for t in x]
+    wq, _, mq, _ = recurrence(x[3], x[2], x[1], g.double(), lens, state.double().transpose(2, 3))
+    wk, _, mk, _ = recurrence(turned[2], scale * turned[3], turned[0], g.double(), lens, dnew.double().transpose(2, 3), 1)
+    wv, ws, mv, ms = recurrence(turned[1], scale * turned[0], turned[3], g.double(), lens, dnew.double(), 1)
+    wk, mk, wv, mv = (t.gather(1, back.expand_as(t)) for t in (wk, mk, wv, mv))
+    got, ds = [torch.full_like(t, 5.0) for t in (q, k, v)], torch.empty_like(state)
+    work.fill_(float("nan"))
+    ff.decay_attention_grad(do, q, k, v, g, *got, state=state, dnew_state=dnew, dstate=ds, lens=ld, work=work, scale=scale)
+    near(got[0], scale * wq, scale * mq * share(dv))
+    near(got[1], wk, mk * share(dv))
+    near(got[2], wv, mv * share(dk))
+    carried(ds, ws, ms)
+
+
+def test_split_in_graphs(dev):
+    """Split calls captured into two graphs, each with a workspace of its own, replayed in turn and at once over changed inputs."""
+    import torch
+    import fufft_amd as ff
+    batch, tokens, heads, d = 2, 2500, 3, 40
+    g = torch.tensor([-0.05, 0.0, -2.0], device=dev)
+    lens = torch.tensor([2500, 1300], dtype=torch.int32, device=dev)
+
+    class One:
+        def __init__(self):
+            self.x = [torch.empty(batch, tokens, heads, d, dtype=torch.bfloat16, device=dev) for _ in range(4)]
+            self.out = [torch.zeros_like(self.x[0]) for _ in range(4)]
+            self.state = torch.zeros(batch, heads, d, d, device=dev)
+            self.work = torch.empty(6, 3, batch, heads, d, d, device=dev)
+
+        def fill(self, seed):
+            gen = torch.Generator(device=dev).manual_seed(seed)
+            for t in self.x:
+                t.copy_(torch.randn(t.shape, device=dev, generator=gen))
+            self.state.fill_(0.5)
+
+        def run(self):
+            q, k, v, do = self.x
+            ff.decay_attention(q, k, v, g, self.out[0], state=self.state, new_state=self.state, lens=lens, work=self.work)
+            ff.decay_attention_grad(do, q, k, v, g, *self.out[1:], dstate=None, lens=lens, work=self.work)
+    ones, graphs = [One(), One()], []
+    side = torch.cuda.Stream()
+    for o in ones:
+        o.fill(0)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            o.run()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            o.run()
+    for seed in (1, 2, 3):
+        for i, o in enumerate(ones):
+            o.fill(2 * seed + i)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in ones]
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for i, o in enumerate(ones):
+            want = One()
+            want.fill(2 * seed + i)
+            want.run()
+            torch.cuda.synchronize()
+            assert torch.equal(o.state, want.state) and all(torch.equal(a, b) for a, b in zip(o.out, want.out))
