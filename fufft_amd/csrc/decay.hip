@@ -44,20 +44,22 @@ constexpr int kChunk = 64, kLanes = 512;
 // of two results (with g = lane / 16), or whose block of 16 takes those of one.
 //
 //   fp32: everything in fp32, whose products run at a sixteenth of the others' rate and bound these kernels.
-//   bf16: what becomes an operand again is rounded to it, but for weighted keys, which are two parts (below): all three
-//     roundings, of keys, state and scores, would leave sqrt(3) of the error that bf16 results have anyway, two sqrt(2).
+//   bf16: what becomes an operand again (the state that q meets, weighted scores, weighted keys) is two bf16 parts, 16 bits,
+//     so that only the result's own rounding is left (0.00166 of results of Gaussian inputs; with the state and scores rounded
+//     to one part 0.00235, and 65536 tokens x 16 heads in 471 us, not 515).
 //   fp16: scores in fp16 as they are.  fp16's range would not hold what becomes an operand again, so that
 //     and what meets it are sums of two bf16 parts, 16 bits of a value and all 11 of fp16; of the four products the
 //     smallest, of both second parts, is left out (2^-16).
 //
 // Where the state is returned, weighted keys are three bf16 parts in both, fp32's 24 bits (FINE): in the launch whose sums
-// become that state, which is the first one where tokens are split (65536 tokens x 16 heads in bf16 with its state: 490 us
-// with three parts in both launches, 462 so).
+// become that state, which is the first one where tokens are split (65536 tokens x 16 heads in bf16 with its state: 527 us
+// with three parts in both launches, 512 so).
 template<class T> struct Cores {
    typedef float E;
    typedef f32x4 Frag, Plain;            // operands in E; of q and k as they are
    static constexpr int KEY_PARTS = 1, FINE_PARTS = 1;       // of weighted keys
-   static constexpr int PARTS = 1;       // of values, weights, the state, and q where it meets that
+   static constexpr int PARTS = 1;       // of values, and of q where it meets the state
+   static constexpr int MADE = 1;        // of weights and the state
    static __device__ inline f32x4 mma(Frag a, Frag b, f32x4 c)
    {
 #pragma unroll
@@ -69,7 +71,7 @@ template<class T> struct Cores {
 template<> struct Cores<bf16> {
    typedef bf16 E;
    typedef bf16x8 Frag, Plain;
-   static constexpr int KEY_PARTS = 2, FINE_PARTS = 3, PARTS = 1;
+   static constexpr int KEY_PARTS = 2, FINE_PARTS = 3, PARTS = 1, MADE = 2;
    static __device__ inline f32x4 mma(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
    static __device__ inline f32x4 scores(Plain a, Plain b, f32x4 c) { return mma(a, b, c); }
 };
@@ -77,7 +79,7 @@ template<> struct Cores<f16> {
    typedef bf16 E;
    typedef bf16x8 Frag;
    typedef f16x8 Plain;
-   static constexpr int KEY_PARTS = 2, FINE_PARTS = 3, PARTS = 2;
+   static constexpr int KEY_PARTS = 2, FINE_PARTS = 3, PARTS = 2, MADE = 2;
    static __device__ inline f32x4 mma(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
    static __device__ inline f32x4 scores(Plain a, Plain b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
@@ -209,7 +211,7 @@ template<class T, int DK, int DV, bool LOCAL, bool FINE> struct Room {
    static constexpr int E = sizeof(typename C::E), KEY_PARTS = FINE ? C::FINE_PARTS : C::KEY_PARTS;
    static constexpr int TP = kChunk * E, KP = pitch_of(DK * E);       // bytes of a row of tokens, of keys' channels
    static constexpr int VALUES = 0, KEYS_T = VALUES + C::PARTS * DV * TP, KEYS = KEYS_T + KEY_PARTS * DK * TP;
-   static constexpr int STATE = LOCAL ? KEYS : KEYS + kChunk * KP, FLAGS = LOCAL ? KEYS : STATE + C::PARTS * DV * KP;
+   static constexpr int STATE = LOCAL ? KEYS : KEYS + kChunk * KP, FLAGS = LOCAL ? KEYS : STATE + C::MADE * DV * KP;
    static constexpr int BYTES = FLAGS + 16;
 };
 
@@ -482,7 +484,7 @@ decay_chunks(DecayParams p)
             for(int c = 0; c < SB; c++) {
                float x[4] = {S[a][c][0], S[a][c][1], S[a][c][2], S[a][c][3]};
                put4<E>(to + c * 16 * KP + a * 16 * (int)sizeof(E), x);
-               if constexpr(C::PARTS == 2) {
+               if constexpr(C::MADE == 2) {
                   rest(x);
                   put4<E>(to + (DV + c * 16) * KP + a * 16 * (int)sizeof(E), x);
                }
@@ -522,11 +524,11 @@ decay_chunks(DecayParams p)
          f32x4 o[SB] = {};
 #pragma unroll
          for(int i = 0; i < NK; i++) {
-            Frag x[SB][C::PARTS], qs[C::PARTS];
+            Frag x[SB][C::MADE], qs[C::PARTS];
 #pragma unroll
             for(int c = 0; c < SB; c++)
 #pragma unroll
-               for(int part = 0; part < C::PARTS; part++) x[c][part] = state_frag(part * DV + v0 + c * 16, i);
+               for(int part = 0; part < C::MADE; part++) x[c][part] = state_frag(part * DV + v0 + c * 16, i);
             if constexpr(C::PARTS == 1) {
                qs[0] = qf[i];
             } else {
@@ -575,13 +577,13 @@ decay_chunks(DecayParams p)
 #pragma unroll
                   for(int r = 0; r < 4; r++) s[e][r] = tile * 16 + r <= reach ? s[e][r] : 0.0f;
             }
-            Frag w[C::PARTS];
+            Frag w[C::MADE];
 #pragma unroll
             for(int e = 0; e < EACH; e++)
 #pragma unroll
                for(int r = 0; r < 4; r++) {
                   w[0][e * 4 + r] = (E)s[e][r];
-                  if constexpr(C::PARTS == 2) w[1][e * 4 + r] = (E)(s[e][r] - (float)(E)s[e][r]);
+                  if constexpr(C::MADE == 2) w[1][e * 4 + r] = (E)(s[e][r] - (float)(E)s[e][r]);
                }
             if(!special) {
 #pragma unroll
@@ -834,18 +836,21 @@ template<class T, int DK, int DV, bool WHOLE, bool FINE>
 hipError_t segments_launches(DecayParams p, int roles, hipStream_t s)
 {
    // Segments so that each CU has a workgroup, where that pays, with a chunk's time in the last launch for a unit: a chunk in the
-   // first launch half of it, the state of every part, which is written, read, written and read, 5 times its share of a
-   // chunk's bytes, the launches 3.5 (128 channels in bf16, out with its state, us unsplit / split: 64 pairs of a sequence and a head,
-   // 32 chunks, 141 / 88; 85 pairs 144 / 108; 128 pairs 160 / 147; 8 chunks 43 / 61; 64 pairs of 4 chunks 25 / 34).
+   // first launch half of it, the state of every part, which is written, read, written and read, 2.5 times its share of a
+   // chunk's bytes in bf16, the launches 2; in the other types 5 and 3.5 (128 channels, out with its state, us unsplit / split.  bf16: 64
+   // pairs of a sequence and a head 32 chunks 181 / 93, 8 chunks 48 / 42, 4 chunks 28 / 34; 85 pairs 32 chunks 181 / 117; 128 pairs 32 chunks
+   // 188 / 169, 16 chunks 98 / 98, 8 chunks 48 / 62.  fp16: 64 pairs 32 chunks 154 / 105, 8 chunks 43 / 45; 128 pairs 32
+   // chunks 159 / 194).
    // A segment of many chunks is two parts in the first launch, which has room for more workgroups on
    // a CU (65536 tokens x 16 heads: 197 us in one part, 152 in 3, 142 in 2).
    const int64_t chunks = (p.tokens + kChunk - 1) / kChunk;
    const int64_t groups = p.pairs * roles * ((p.role[0].dv + DV - 1) / DV);
-   constexpr int64_t STATES = 10 * (4 * DK * DV) / (2 * kChunk * (DK + DV) * (int)sizeof(T));      // in halves of a chunk, as below
+   constexpr bool BF16 = std::is_same<T, bf16>::value;          // in halves of a chunk:
+   constexpr int64_t STATES = (BF16 ? 5 : 10) * (4 * DK * DV) / (2 * kChunk * (DK + DV) * (int)sizeof(T)), LAUNCHES = BF16 ? 4 : 7;
    int64_t n = 256 / (groups > 0 ? groups : 1);
    if(n > p.splits) n = p.splits;
    if(n > chunks) n = chunks;
-   if(n < 2 || 3 * ((chunks + n - 1) / n) + 7 + STATES >= 2 * chunks) n = 1;
+   if(n < 2 || 3 * ((chunks + n - 1) / n) + LAUNCHES + STATES >= 2 * chunks) n = 1;
    const int64_t parts = p.splits / n >= 2 && chunks / n >= 16 ? 2 : 1;
    const int64_t each = chunks > 0 ? (chunks + n * parts - 1) / (n * parts) : 1;       // chunks of a part
    p.part = each * kChunk;

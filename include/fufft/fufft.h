@@ -658,12 +658,11 @@ int fufft_rms_norm_grad(const void* dy, int type, int64_t ldy, const void* h, in
  *   work       fp32 space for `splits` states of every sequence and head (splits x batch x heads
  *              x dk x dv): the tokens are split over at most that many workgroups.
  *              0 (NULL) is allowed.  About 512 / (batch * heads) are as many as help.
- * Sums are fp32.  Of bf16 inputs, weighted scores and the state that q meets are rounded to
- * bf16 before their products, and keys weighted on their way into the state are kept to 16 bits; of
- * fp16 inputs all of these are kept to 16 bits; fp32 inputs are multiplied in fp32.  Where the state is asked for, weighted
+ * Sums are fp32; fp32 inputs are multiplied in fp32.  Of 16-bit inputs, weighted scores, the state that q meets and keys
+ * weighted on their way into the state are kept to 16 bits before their products.  Where the state is asked for, weighted
  * keys are kept to 24 bits (results can differ in their last bits from a call that does not ask).
- * A token's result does not depend on later tokens, whatever they hold.  An infinite key or value
- * of 16-bit inputs may make NaN of the state's element that would be infinite. */
+ * A token's result does not depend on later tokens, whatever they hold.  Infinite 16-bit inputs
+ * may make NaN of results and elements of the state that would be infinite. */
 typedef struct fufft_strides {
    int64_t batch, token, head;
 } fufft_strides;
