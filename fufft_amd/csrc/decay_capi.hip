@@ -115,16 +115,18 @@ struct Buffers {
       arrays[count] = a;
       written[count++] = out;
    }
-   void bytes(const void* p, int64_t n, uintptr_t align, bool out)
+   // the number of the buffer among the flat ones
+   int bytes(const void* p, int64_t n, uintptr_t align, bool out)
    {
-      if(status != FUFFT_OK) return;
+      if(status != FUFFT_OK) return -1;
       const Span s{p, n};
       status = span_status(s, align);
       flat[flats] = s;
-      flat_written[flats++] = out;
+      flat_written[flats] = out;
+      return flats++;
    }
-   // Outputs share no byte with anything else, but for the pair of flat buffers that may be one (same_a, same_b).
-   int check(const void* same_a, const void* same_b) const
+   // Outputs share no byte with anything else, but for one pair of flat buffers of a size, by their numbers, that may start at one address.
+   int check(int pair_a = -1, int pair_b = -1) const
    {
       if(status != FUFFT_OK) return status;
       for(int i = 0; i < count; i++) {
@@ -136,7 +138,7 @@ struct Buffers {
       for(int i = 0; i < flats; i++)
          for(int j = 0; j < i; j++) {
             if(!flat_written[i] && !flat_written[j]) continue;
-            const bool pair = same_a && same_a == same_b && ((flat[i].p == same_a && flat[j].p == same_a));
+            const bool pair = i == pair_b && j == pair_a && flat[i].p == flat[j].p;
             if(!pair && !disjoint(flat[i], flat[j])) return FUFFT_ERR_INVALID;
          }
       return FUFFT_OK;
@@ -165,11 +167,11 @@ int fufft_decay_attention(const void* q, const fufft_strides* q_strides, const v
    all.array(v, type, v_strides, z, dv, false);
    all.array(out, type, out_strides, z, dv, true);
    all.bytes(log_decay, heads * 4, 4, false);
-   all.bytes(state, state ? z.state_bytes() : 0, 4, false);
-   all.bytes(new_state, new_state ? z.state_bytes() : 0, 4, true);
+   const int before = all.bytes(state, state ? z.state_bytes() : 0, 4, false);
+   const int behind = all.bytes(new_state, new_state ? z.state_bytes() : 0, 4, true);
    all.bytes(lens, lens ? batch * 4 : 0, 4, false);
    all.bytes(work, z.state_bytes(splits), 4, true);
-   FUFFT_MX4_CHECK(all.check(state, new_state));
+   FUFFT_MX4_CHECK(all.check(before, behind));
    if(dk > kWidestHead || dv > kWidestHead || tokens > kLongestText) return FUFFT_ERR_UNSUPPORTED;
    DecayParams p{};
    p.role[0] = DecayRole{q, k, v, out, strides_of(q_strides), strides_of(k_strides), strides_of(v_strides), strides_of(out_strides),
@@ -209,7 +211,7 @@ int fufft_decay_attention_grad(const void* dout, const fufft_strides* dout_strid
    all.bytes(dstate, dstate ? z.state_bytes() : 0, 4, true);
    all.bytes(lens, lens ? batch * 4 : 0, 4, false);
    all.bytes(work, z.state_bytes(splits * 3), 4, true);
-   FUFFT_MX4_CHECK(all.check(nullptr, nullptr));
+   FUFFT_MX4_CHECK(all.check());
    if(dk > kWidestHead || dv > kWidestHead || tokens > kLongestText) return FUFFT_ERR_UNSUPPORTED;
    const Strides sd = strides_of(dout_strides), sq = strides_of(q_strides), sk = strides_of(k_strides), sv = strides_of(v_strides);
    const int64_t set = splits * batch * heads * dk * dv;
@@ -251,7 +253,7 @@ int fufft_decay_attention_step(const void* q, const fufft_strides* q_strides, co
    all.bytes(log_decay, heads * 4, 4, false);
    all.bytes(state, slot_count * heads * dk * dv * 4, 4, true);
    all.bytes(slots, slots ? batch * 8 : 0, 8, false);
-   FUFFT_MX4_CHECK(all.check(nullptr, nullptr));
+   FUFFT_MX4_CHECK(all.check());
    if(dk > kWidestHead || dv > kWidestHead) return FUFFT_ERR_UNSUPPORTED;
    StepParams p{};
    p.q = q;
