@@ -57,17 +57,20 @@ bool distinct(const Array& a)
 }
 // Whether the parts below axis i of two arrays share nothing, the second one's `by` elements behind the first
 // one's: far from each other, or, along an axis that both step through alike, each in the gaps of the other (parts
-// of one row a token, whose heads may have other widths).
+// of one row a token, whose heads may have other widths).  Parts longer than that step, which reach over several
+// of the other's, are not taken.
 bool parts_apart(const Array& a, const Array& b, int i, int64_t by)
 {
    const int64_t wa = extent(a, i), wb = extent(b, i);
    if(by >= wa || by + wb <= 0) return true;
    if(i >= a.axes || i >= b.axes || a.axis[i].stride != b.axis[i].stride) return false;
    const int64_t s = a.axis[i].stride;
-   if(s == 0) return false;
-   const int64_t r = (by % s + s) % s;                 // the second's first part in a step of the first
-   if(r < extent(a, i + 1) && !parts_apart(a, b, i + 1, r)) return false;
-   return r + extent(b, i + 1) <= s || parts_apart(a, b, i + 1, r - s);
+   const int64_t pa = extent(a, i + 1), pb = extent(b, i + 1);
+   if(pa > s || pb > s) return false;
+   // the second's first part in a step of the first: parts of at most a step meet that step's part and the next one's only
+   const int64_t r = (by % s + s) % s;
+   if(r < pa && !parts_apart(a, b, i + 1, r)) return false;
+   return r + pb <= s || parts_apart(a, b, i + 1, r - s);
 }
 bool arrays_apart(const Array& a, const Array& b)
 {

@@ -648,7 +648,8 @@ int fufft_rms_norm_grad(const void* dy, int type, int64_t ldy, const void* h, in
  * S, the state, is dk x dv in fp32; S[-1] is `state`, or zero.
  * q, k, v, out are arrays of batch x tokens x heads x dim, dim (dk of q and k, dv of v and
  * out) from 1 to 128 and tokens up to 2^30 (beyond: FUFFT_ERR_UNSUPPORTED), with adjacent elements and the strides
- * (elements, >= 0; of an input 0 too: one k for all heads) of a fufft_strides.  log_decay is
+ * (elements, >= 0; of an input 0 too: one k for all heads) of a fufft_strides.  In one array with another operand an output
+ * is taken where both step through the array alike, the parts of each between those of the other.  log_decay is
  * heads fp32 values, <= 0, -infinity included: only the token itself.
  *   lens       batch int32: tokens of each sequence, within 0 .. tokens; rows behind the last
  *              are neither read nor written.  NULL: tokens;
