@@ -25,6 +25,19 @@ using mx4::u32x4;
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
+// The scale of a row of a: a sum times a large one can leave fp32 where its product with the other scale does not,
+// so that such a scale is taken 2^-40 times, and the result 2^40 times.  Both are exact: the sum is below 2^31, so that the first
+// product stays below 2^119, and it is 2^24 at least, so that no scale of b brings the second one below the normal numbers.
+struct RowScale {
+   float s, up;
+};
+__device__ inline RowScale row_scale(float s)
+{
+   const bool large = fabsf(s) > 0x1p+64f;
+   return {large ? s * 0x1p-40f : s, large ? 0x1p+40f : 1.0f};
+}
+__device__ inline float scaled(int sum, RowScale a, float b) { return (float)sum * a.s * b * a.up; }
+
 // ---- single tokens: rows of b whole, products of four bytes -------------------------------
 //
 // A wavefront has 4 rows of b and M of a (those that are not there are zeros), the lanes 16 bytes each of 1 KiB
@@ -89,7 +102,7 @@ i8_tokens(I8Params p, int64_t row_bytes)
    if(threadIdx.x < kTokenRows * M && i < p.m && n < p.n) {
       int total = 0;
       for(int w = 0; w < waves; w++) total += join[w][threadIdx.x];
-      float v = row_bytes ? (float)total * p.a_scales[i] * p.b_scales[n] : 0.0f;
+      float v = row_bytes ? scaled(total, row_scale(p.a_scales[i]), p.b_scales[n]) : 0.0f;
       if(p.bias) v += p.bias[n];
       static_cast<O*>(p.out)[i * p.ld + n] = (O)v;
    }
@@ -174,7 +187,7 @@ i8_rows(I8Params p, int pieces, int waves)
       if(n >= p.n) continue;
       int sum = 0;
       for(int w2 = 0; w2 < waves; w2++) sum += join[w2 * ROWS * COLS + i];
-      float v = pieces ? (float)sum * p.a_scales[m] * p.b_scales[n] : 0.0f;
+      float v = pieces ? scaled(sum, row_scale(p.a_scales[m]), p.b_scales[n]) : 0.0f;
       if(p.bias) v += p.bias[n];
       out[m * p.ld + n] = (O)v;
    }
@@ -331,9 +344,9 @@ i8_tiles(I8Params p, uint32_t slabs, uint32_t tm, uint32_t tn)
    O* out = static_cast<O*>(p.out) + m0 * p.ld + n0;
 #pragma unroll
    for(int a0 = 0; a0 < FM; a0 += PASS) {
-      float sa[PASS];
+      RowScale sa[PASS];
 #pragma unroll
-      for(int a = 0; a < PASS; a++) sa[a] = load_float(rsa, wm + (a0 + a) * 32 + (lane & 31));
+      for(int a = 0; a < PASS; a++) sa[a] = row_scale(load_float(rsa, wm + (a0 + a) * 32 + (lane & 31)));
 #pragma unroll
       for(int b = 0; b < FN; b++)
 #pragma unroll
@@ -349,7 +362,7 @@ i8_tiles(I8Params p, uint32_t slabs, uint32_t tm, uint32_t tn)
             for(int a = a0; a < a0 + PASS; a++) {
                struct alignas(4 * sizeof(O)) Four { O e[4]; } v;
 #pragma unroll
-               for(int i = 0; i < 4; i++) v.e[i] = (O)((float)acc[a][b][q * 4 + i] * sa[a - a0] * sb[i] + bias[i]);
+               for(int i = 0; i < 4; i++) v.e[i] = (O)(scaled(acc[a][b][q * 4 + i], sa[a - a0], sb[i]) + bias[i]);
                *reinterpret_cast<Four*>(mine + ((a - a0) * 32 + (lane & 31)) * PITCH + j * sizeof(O)) = v;
             }
          }
