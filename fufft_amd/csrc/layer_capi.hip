@@ -18,12 +18,18 @@ struct Rows {
    int64_t     ld;
 };
 Span span_of(const Rows& m, int64_t rows, int64_t k) { return m.p ? matrix(m.p, m.type, m.ld, rows, k) : Span{nullptr, 0}; }
+// no byte shared: far from each other, or columns of one array
+bool rows_apart(const Rows& a, const Rows& b, int64_t rows, int64_t k)
+{
+   if(!a.p || !b.p) return true;
+   const int64_t ea = type_bytes(a.type), eb = type_bytes(b.type);
+   return matrices_apart(span_of(a, rows, k), a.ld * ea, k * ea, span_of(b, rows, k), b.ld * eb, k * eb, rows);
+}
 // an output that may be an input, element for element, and otherwise shares no byte with it
 bool same_or_apart(const Rows& out, const Rows& in, int64_t rows, int64_t k)
 {
-   if(!out.p || !in.p) return true;
-   if(out.p == in.p && out.type == in.type && (out.ld == in.ld || rows <= 1)) return true;
-   return disjoint(span_of(out, rows, k), span_of(in, rows, k));
+   if(out.p && out.p == in.p && out.type == in.type && (out.ld == in.ld || rows <= 1)) return true;
+   return rows_apart(out, in, rows, k);
 }
 bool eps_ok(float eps) { return eps >= 0.0f && eps < __builtin_inff(); }
 
@@ -117,7 +123,7 @@ int fufft_rms_norm(const void* x, int type, int64_t ldx, const void* residual, i
    FUFFT_MX4_CHECK(span_status(ss, 4));
    if(!apart(sc, {sx, sr, st, so, sw, ss}) || !apart(ss, {sx, sr, st, so, sw}) || !apart(sw, {st, so}) ||
       !same_or_apart(rt, rr, rows, k) || !same_or_apart(rt, rx, rows, k) || !same_or_apart(ro, rx, rows, k) ||
-      !apart(so, {sr, st}))
+      !rows_apart(ro, rr, rows, k) || !rows_apart(ro, rt, rows, k))
       return FUFFT_ERR_INVALID;
    const NormParams p{x,   residual, total, weight, out, static_cast<int8_t*>(codes), scales, ldx, ldr, ldt, ldo, rows, k,
                       eps, type,     sum_type};
@@ -148,8 +154,8 @@ int fufft_rms_norm_grad(const void* dy, int type, int64_t ldy, const void* h, in
    FUFFT_MX4_CHECK(span_status(sw, 4));
    FUFFT_MX4_CHECK(span_status(sd, 4));
    FUFFT_MX4_CHECK(span_status(sk, 4));
-   if(!apart(sd, {sy, sh, st, sx, sw, sk}) || !apart(sk, {sy, sh, st, sx, sw}) || !apart(sx, {sh, sw}) ||
-      !same_or_apart(rx, ry, rows, k) || !same_or_apart(rx, rt, rows, k))
+   if(!apart(sd, {sy, sh, st, sx, sw, sk}) || !apart(sk, {sy, sh, st, sx, sw}) || !apart(sx, {sw}) ||
+      !rows_apart(rx, rh, rows, k) || !same_or_apart(rx, ry, rows, k) || !same_or_apart(rx, rt, rows, k))
       return FUFFT_ERR_INVALID;
    const NormGradParams p{dy,  h,    dtotal, weight,   dx,     dweight, work, ldy, ldh, ldt, ldx, rows, k, splits,
                           eps, type, sum_type, dx_type};

@@ -593,7 +593,8 @@ int fufft_mx4_cache_conv(const void* codes, const uint8_t* scales, int64_t pages
  * Element types, leading dimensions, alignment and sizes of zero are as in the 4-bit
  * calls above.  Every sum, state and statistic is fp32 (integer sums int32), rounded
  * once to the output's type.  Outputs share no byte with another buffer of the call, but for
- * those named below that may be one of its inputs, the same address and strides.
+ * those named below that may be one of its inputs, the same address and strides; rows may be
+ * columns of one array, each with the same bytes from row to row.
  * Sizes that no launch can hold are FUFFT_ERR_UNSUPPORTED.  A workspace belongs to one call at
  * a time: calls or graphs that may run together need one each.
  *
