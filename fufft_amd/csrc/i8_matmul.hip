@@ -441,10 +441,12 @@ int64_t tiles(const I8Params& p, int64_t rows, int64_t cols)
 
 // The kernel for a size, on MI355X's 256 CUs; us at m x n x k.
 //   Up to 8 rows: four-byte products, 1 KiB of a row of b a load (16 rows on the matrix cores / so: 1 x 8192 x 8192
-//     18.8 / 12.3, 1 x 16384 x 8192 37.4 / 23.6, 8 x 16384 x 8192 37 / 29; 8 x 8192 x 8192 21.0 / 21.9).
+//     18.8 / 11.6, 1 x 16384 x 8192 37.4 / 23.6, 8 x 16384 x 8192 37 / 29, 8 x 8192 x 8192 20.4 / 17.7).
 //   K split over wavefronts, operands straight from memory, where at most 256 workgroups of 16 or 32 rows by 16
 //     columns have all results and K is long, and up to 16 rows by 8192 columns (against 64 x 64 staged: 24 x 4096 x
-//     4096 8.4 / 10.7, 100 x 100 x 1024 3.8 / 5.2, 16 x 8192 x 8192 19.9 / 21.5; but 16 x 16384 x 8192 37.2 / 24.9).
+//     4096 8.4 / 10.7, 100 x 100 x 1024 3.8 / 5.2; 16 rows by 4608, 6144, 8192 columns x K: 2048 5.7, 5.9, 6.1 / 6.7, 6.6, 6.6,
+//     4096 8.6, 8.9, 10.1 / 10.0, 10.1, 10.2, 16384 29.8, 31.4, 35.8 / 33.8, 35.1, 38.1, 8192 14.5, 16.7, 20.9 / 16.8, 16.9, 18.5,
+//     that last one the only size of them that loses; but 16 x 16384 x 8192 37.2 / 24.9).
 //   Staged tiles: 256 x 256, one a CU, against 128 x 128, two a CU, by the rounds that each needs; 64 x 64, four slabs
 //     on their way, below 256 tiles of 128 x 128 (128 x 4096 x 4096 10.9 / 21.8, 1001 x 2000 x 1504 9.7 / 12.7; with two
 //     slabs 128 x 4096 x 4096 16.8, 64 x 16384 x 8192 48.6 / 27.1).

@@ -693,7 +693,8 @@ int fufft_decay_attention_grad(const void* dout, const fufft_strides* dout_strid
  * state, `slot_count` x heads x dk x dv fp32, contiguous, updated in place.  slots: the state of
  * each sequence, int64, or NULL: its own number (slot_count >= batch then).  A sequence whose slot is outside
  * [0, slot_count) (-1: a place in the batch without a sequence), or is that of an earlier one
- * of the call, changes no state and has zeros for its result.  All in fp32. */
+ * of the call, changes no state and has zeros for its result.  (The earlier ones are looked through for
+ * every sequence and head: time that is felt from some thousand sequences of small states on.)  All in fp32. */
 int fufft_decay_attention_step(const void* q, const fufft_strides* q_strides, const void* k,
                                const fufft_strides* k_strides, const void* v,
                                const fufft_strides* v_strides, int type, const float* log_decay,
